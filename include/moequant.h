@@ -42,6 +42,7 @@ typedef enum {
 } mq_status;
 
 typedef enum { MQ_F32 = 0, MQ_BF16 = 1, MQ_F16 = 2 } mq_dtype;
+#define MQ_I8 3   /* activations that already are 8-bit codes, where an entry point says so */
 
 /* Arithmetic used for the dense contractions.
  *   MQ_MATH_FP32  : fp32 FMA on the CUDA cores (bit-for-bit the reference's
@@ -272,6 +273,56 @@ size_t mq_error_forms_workspace_bytes(int64_t R, int64_t C);
  *   packed  : (R, ceil(C/8)) int32 out.  */
 int mq_pack_int4(const uint8_t* codes, int64_t R, int64_t C, const int8_t* zero_i8, int64_t group,
                  int32_t* packed, void* stream);
+
+/* ------------------------------------------------------------------ running the quantized layers
+ * What serves a mixture-of-experts layer whose weights have 8-bit codes, one scale per output channel
+ * (GPTQ.quantize(8) with one group per row; code - 128 as int8): the router, the plan that groups the pairs of
+ * token and expert, the product in 8-bit integers, the experts' gated MLPs.  Forward only.  */
+
+/* Routing of T tokens to top_k of E experts.  logits (T, E) of `dtype`, row stride ld (elements).
+ *   score       : 0 softmax over the experts, 1 sigmoid
+ *   bias        : optional E floats, added to the scores for the choice alone
+ *   groups      : experts lie in `groups` equal runs, of which keep_groups stay: those with the largest value
+ *                 (group_score 0) or the largest sum of two values (1); 1 for none
+ *   choice      : the top_k largest values of what stays, ties to the lowest index, in falling order.  An expert whose
+ *                 logit is -inf or NaN or whose bias is -inf or NaN is never chosen; what is then missing has id -1 and weight 0.
+ *                 A logit of +inf counts as the largest finite fp32 number.
+ *   weights     : the scores (without bias), divided by their sum with renormalise, times scale
+ * ids (T, top_k) and weights (T, top_k) contiguous.  E <= 1024, top_k <= 32, groups <= 32.  */
+int mq_route_tokens(const void* logits, int dtype, int64_t T, int64_t E, int64_t ld, int top_k, int score, const float* bias,
+                    int groups, int keep_groups, int group_score, int renormalise, float scale, int32_t* ids, float* weights,
+                    void* stream);
+
+/* A stable counting sort of pairs by expert: ids[i] - first in [0, E) is the expert of pair i, every other id belongs to no expert here.
+ *   offsets (E + 1): where an expert's pairs begin;  order (pairs): the pairs, by (expert, i), -1 behind the last;
+ *   place (pairs): where pair i stands in order, -1 for none.  E <= 1024.  */
+int mq_expert_plan(const int32_t* ids, int64_t pairs, int64_t E, int64_t first, int32_t* offsets, int32_t* order, int32_t* place,
+                   void* workspace, size_t workspace_bytes, void* stream);
+size_t mq_expert_plan_workspace_bytes(int64_t pairs, int64_t E);
+
+/* 8-bit codes of each row of x (T, K): scale = max|x| / 127, code = round-half-even(127 x / max|x|).  A row of zeros has the scale
+ * 0; one with an infinity or a NaN the scale NaN and codes 0.  ldx in elements, ldc in bytes.  */
+int mq_quantize_tokens(const void* x, int dtype, int64_t T, int64_t K, int64_t ldx, int8_t* codes, int64_t ldc, float* scale,
+                       void* stream);
+
+/* y[t, n] = (sum over k of code[t, k] w[n, k]) x_scale[t] w_scale[n] + bias[n], the sum exact in 32-bit integers (K <= 131072).
+ * x (T, K) of x_dtype gets its codes as mq_quantize_tokens gives them (x_scale is not read), or is codes already (MQ_I8) with
+ * their scales.  w (N, K) int8; rows of codes start on 16-byte boundaries.  bias may be NULL.  y (T, N) of out_dtype.  */
+int mq_int8_matmul(const void* x, int x_dtype, const float* x_scale, int64_t T, int64_t K, int64_t ldx, const int8_t* w, int64_t N,
+                   int64_t ldw, const float* w_scale, const float* bias, int out_dtype, void* y, int64_t ldy, void* workspace,
+                   size_t workspace_bytes, void* stream);
+size_t mq_int8_matmul_workspace_bytes(int x_dtype, int64_t T, int64_t N, int64_t K);
+
+/* The experts' MLPs of T tokens (bf16 or fp16): y[t] = sum over slots s with ids[t, s] - first = e in [0, E) of
+ *   weights[t, s] * down_e(silu(gate_e(x[t])) * up_e(x[t])),
+ * every product as in mq_int8_matmul, the gated values kept in fp32 until they get their codes.  gate_up (E, 2 I, K): gate rows, then
+ * up rows; down (E, K, I); row strides ld_* and expert strides *_expert in bytes, multiples of 16; scales contiguous.
+ * A token without an expert here gets zeros.  */
+int mq_int8_experts(const void* x, int dtype, int64_t T, int64_t K, int64_t ldx, const int32_t* ids, const float* weights, int top_k,
+                    int64_t first, int64_t E, int64_t I, const int8_t* gate_up, int64_t ld_gate_up, int64_t gate_up_expert,
+                    const float* gate_up_scale, const int8_t* down, int64_t ld_down, int64_t down_expert, const float* down_scale,
+                    void* y, int64_t ldy, void* workspace, size_t workspace_bytes, void* stream);
+size_t mq_int8_experts_workspace_bytes(int64_t T, int top_k, int64_t E, int64_t K, int64_t I);
 
 #ifdef __cplusplus
 }

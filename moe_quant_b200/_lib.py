@@ -16,6 +16,7 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(_HERE, "libmoequant_sm100.so")
 
 MQ_F32, MQ_BF16, MQ_F16 = 0, 1, 2
+MQ_I8 = 3   # activations that already are 8-bit codes (mq_int8_matmul)
 MATH_FP32, MATH_TENSOR = 0, 1
 MATH_COMPACT = 0x100   # MQ_MATH_COMPACT: flag OR-ed into the math argument of the sweep / whole-layer calls
 MATH_MANY_TOKENS = 0x200   # MQ_MATH_MANY_TOKENS: flag OR-ed into the math argument of the factorisation / whole-layer calls
@@ -71,6 +72,18 @@ SIGNATURES = {
                                c_void_p]),
     "mq_error_forms_workspace_bytes": (c_size_t, [c_int64, c_int64]),
     "mq_permute_columns": (c_int, [c_void_p, c_int, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p]),
+    "mq_route_tokens": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_int, c_int, c_void_p, c_int, c_int, c_int, c_int, c_float,
+                                c_void_p, c_void_p, c_void_p]),
+    "mq_expert_plan": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p]),
+    "mq_expert_plan_workspace_bytes": (c_size_t, [c_int64, c_int64]),
+    "mq_quantize_tokens": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_void_p]),
+    "mq_int8_matmul": (c_int, [c_void_p, c_int, c_void_p, c_int64, c_int64, c_int64, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int,
+                               c_void_p, c_int64, c_void_p, c_size_t, c_void_p]),
+    "mq_int8_matmul_workspace_bytes": (c_size_t, [c_int, c_int64, c_int64, c_int64]),
+    "mq_int8_experts": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64,
+                                c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64,
+                                c_void_p, c_size_t, c_void_p]),
+    "mq_int8_experts_workspace_bytes": (c_size_t, [c_int64, c_int, c_int64, c_int64, c_int64]),
     "mq_pack_int4": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_void_p]),
 }
 

@@ -19,6 +19,8 @@ import torch.nn as nn
 from torch import Tensor
 
 from . import dist_utils, model_utils, quant_utils
+from ._lib import MoeQuantError
+from .int8 import int8_block
 from .gptq import GPTQ, quantize_many, quantize_shared
 
 ROUTED_EXPERTS_REGEX = r".*mlp\.experts\.\d+\.(down|gate|up)_proj$"   # quant.py:24
@@ -51,11 +53,17 @@ def quantize_block(
     log_error: bool = False,
     streams: int = 8,
     forward_kwargs: Optional[dict] = None,
+    int8_outputs: bool = False,
 ) -> Dict[str, object]:
     """Returns {'outputs': block outputs after quantization (the next block's inputs),
     'layers': names in quantization order, 'issues': {'zero_samples','nan_hessian','non_invertible'},
-    'relative_error': {name: float} when log_error}."""
+    'relative_error': {name: float} when log_error}.
+    int8_outputs: the outputs come from the block as it is served in 8-bit integers, activations rounded to 8 bits per token
+    (8 bits and one group per row; the dequantized weights stay in the block as ever)."""
     forward_kwargs = forward_kwargs or {}
+    if int8_outputs and (bits != 8 or group_size is not None):
+        raise MoeQuantError("int8_outputs needs bits=8 and group_size=None")
+    int8_results: Dict[str, tuple] = {}
     layers = model_utils.select_layers(block, "", ".*", model_utils.LINEAR_LAYERS)
     handles: Dict[str, GPTQ] = {}
     hooks = []
@@ -108,6 +116,8 @@ def quantize_block(
         if dist_utils.is_main() or not main_only:
             _save(save_dir, f"{prefix}{name}", q, s, z)
         h.layer.weight.data = deq.to(h.layer.weight.dtype).reshape(h.layer.weight.shape)     # quant.py:328
+        if int8_outputs:
+            int8_results[name] = result
         order.append(name)
 
     # shared layers first (quant.py:295-330).  With several ranks each layer's Hessian is reduced
@@ -130,7 +140,8 @@ def quantize_block(
     for name in experts:
         handles[name].reset()
 
-    outputs = [block(x, **forward_kwargs) for x in inputs]                                   # quant.py:414-416
+    with int8_block(block, int8_results):                                                    # as it is, without results
+        outputs = [block(x, **forward_kwargs) for x in inputs]                               # quant.py:414-416
     for o in outputs:
         if not bool(torch.isfinite(o).all()):
             raise RuntimeError("block outputs are not finite after quantization")

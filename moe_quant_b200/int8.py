@@ -1,0 +1,106 @@
+"""Layers that run in 8-bit integers on what `GPTQ(layer, None, ...).quantize(8)` returns: codes of 8 bits with one scale per
+output channel.  Activations get their codes token by token on the way in.  Forward only: the modules hold no
+parameters, and their calls refuse inputs that ask for gradients."""
+from __future__ import annotations
+
+import re
+from contextlib import contextmanager
+from typing import Mapping, Optional, Sequence, Tuple
+
+import torch
+import torch.nn as nn
+from torch import Tensor
+
+from . import ops
+from ._lib import MoeQuantError
+
+
+def int8_layout(qweight: Tensor, scale: Tensor, zero: Optional[Tensor] = None) -> Tuple[Tensor, Tensor]:
+    """(int8 codes, fp32 scales) as ops.int8_matmul takes them, from the uint8 codes (R, C), the scales (R, 1) and the zero points of a
+    symmetric 8-bit layer with one group per row.  Rows of the codes start 16 bytes apart or a multiple of it."""
+    if qweight.dtype != torch.uint8 or qweight.dim() != 2:
+        raise MoeQuantError("int8_layout: qweight must be a 2-D uint8 tensor")
+    R, C = qweight.shape
+    if scale.numel() != R:
+        raise MoeQuantError(f"int8_layout: {scale.numel()} scales for {R} rows: quantize with one group per row (group_size None)")
+    if zero is not None and not bool((zero == 128).all()):
+        raise MoeQuantError("int8_layout: the zero point of 8-bit symmetric codes is 128")
+    codes = torch.zeros(R, (C + 15) // 16 * 16, dtype=torch.uint8, device=qweight.device)[:, :C]
+    torch.bitwise_xor(qweight, 128, out=codes)   # q - 128 in two's complement
+    return codes.view(torch.int8), scale.reshape(R).to(torch.float32)
+
+
+class Int8Linear(nn.Module):
+    """Stands in for an nn.Linear whose weight has been quantized to 8 bits per output channel."""
+
+    def __init__(self, qweight: Tensor, scale: Tensor, zero: Optional[Tensor] = None, bias: Optional[Tensor] = None):
+        super().__init__()
+        codes, scale = int8_layout(qweight, scale, zero)
+        self.out_features, self.in_features = codes.shape
+        self.register_buffer("codes", codes, persistent=False)
+        self.register_buffer("scale", scale, persistent=False)
+        self.register_buffer("bias", None if bias is None else bias.detach().to(torch.float32), persistent=False)
+
+    def forward(self, x: Tensor) -> Tensor:
+        return ops.int8_matmul(x, self.codes, self.scale, bias=self.bias)
+
+
+class Int8Experts(nn.Module):
+    """The gated MLPs of the experts first .. first + E - 1, one (qweight, scale, zero) per projection and expert."""
+
+    def __init__(self, gate: Sequence, up: Sequence, down: Sequence, first: int = 0):
+        super().__init__()
+        if not len(gate) == len(up) == len(down) or not gate:
+            raise MoeQuantError("Int8Experts: as many gate as up and down projections, and at least one")
+        self.first = int(first)
+        gates, ups, downs = ([int8_layout(*r) for r in side] for side in (gate, up, down))
+        both = [(torch.cat([_whole(g), _whole(u)]), torch.cat([gs, us])) for (g, gs), (u, us) in zip(gates, ups)]
+        hidden, inner = gates[0][0].shape[1], gates[0][0].shape[0]
+        self.register_buffer("gate_up", torch.stack([c for c, _ in both])[..., :hidden], persistent=False)
+        self.register_buffer("gate_up_scale", torch.stack([s for _, s in both]), persistent=False)
+        self.register_buffer("down", torch.stack([_whole(c) for c, _ in downs])[..., :inner], persistent=False)
+        self.register_buffer("down_scale", torch.stack([s for _, s in downs]), persistent=False)
+
+    def forward(self, x: Tensor, ids: Tensor, weights: Tensor) -> Tensor:
+        return ops.int8_experts(x, ids, weights, self.gate_up, self.gate_up_scale, self.down, self.down_scale, first=self.first)
+
+
+def _whole(codes: Tensor) -> Tensor:
+    """A view of the rows with their padding."""
+    return codes.as_strided((codes.shape[0], codes.stride(0)), codes.stride())
+
+
+@contextmanager
+def int8_block(block: nn.Module, results: Mapping[str, Tuple[Tensor, Tensor, Tensor]]):
+    """Within the context the block's quantized layers run in 8-bit integers: `results` maps their names to what quantize(8)
+    returned.  A module whose experts are all among them, and which has a place for it (`int8_experts`), runs them through
+    ops.int8_experts; every other layer becomes an Int8Linear."""
+    undo = []
+    left = dict(results)
+    try:
+        for moe_name, moe in list(block.named_modules()):
+            if not hasattr(moe, "int8_experts"):
+                continue
+            prefix = f"{moe_name}.experts." if moe_name else "experts."
+            mine = {n[len(prefix):]: n for n in left if n.startswith(prefix)}
+            ids = sorted({int(m.group(1)) for m in (re.fullmatch(r"(\d+)\.(gate|up|down)_proj", n) for n in mine) if m})
+            sides = [[left.get(f"{prefix}{i}.{side}_proj") for i in ids] for side in ("gate", "up", "down")]
+            local = [i for i, e in enumerate(moe.experts) if e is not None]
+            if not ids or ids != local or ids != list(range(ids[0], ids[-1] + 1)) or any(r is None for side in sides for r in side):
+                continue
+            moe.int8_experts = Int8Experts(*sides, first=ids[0])
+            undo.append((moe, "int8_experts", None))
+            for n in mine.values():
+                del left[n]
+        for name, result in left.items():
+            parent, _, leaf = name.rpartition(".")
+            parent = block.get_submodule(parent)
+            layer = getattr(parent, leaf)
+            if not isinstance(layer, nn.Linear):
+                raise MoeQuantError(f"int8_block: {name} is no nn.Linear")
+            setattr(parent, leaf, Int8Linear(*result, bias=layer.bias))
+            undo.append((parent, leaf, layer))
+        yield block
+    finally:
+        for parent, leaf, was in reversed(undo):
+            setattr(parent, leaf, was)

@@ -12,7 +12,7 @@ import torch
 from torch import Tensor
 
 from . import _lib
-from ._lib import MATH_COMPACT, MATH_FP32, MATH_MANY_TOKENS, MATH_TENSOR, MoeQuantError, check, dtype_code, lib, ptr, require_cuda, require_one_device, stream_ptr
+from ._lib import MATH_COMPACT, MATH_FP32, MATH_MANY_TOKENS, MATH_TENSOR, MQ_I8, MoeQuantError, check, dtype_code, lib, ptr, require_cuda, require_one_device, stream_ptr
 
 
 @dataclass
@@ -374,3 +374,212 @@ def pack_int4(codes: Tensor, zero_i8: Optional[Tensor] = None, group: int = 0) -
     with _lib.on_device(codes.device):
         check(lib().mq_pack_int4(ptr(codes), R, C, ptr(zero_i8), group, ptr(out), stream_ptr(codes.device)))
     return out
+
+
+# ---------------------------------------------------------------- running the quantized layers
+# Forward only.  Scratch comes from the caching allocator with every call: a buffer kept per stream would be shared by two graphs captured
+# on one stream, whose replays may overlap.
+def _forward_only(what: str, *tensors: Optional[Tensor]) -> None:
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise MoeQuantError(f"{what} has no backward pass: call it under torch.no_grad() or detach its inputs")
+
+
+def _rows(t: Tensor, what: str) -> Tensor:
+    """(..., C) as rows of unit column stride, a view where the strides allow it."""
+    if t.dim() < 1:
+        raise MoeQuantError(f"{what} must have at least one dimension")
+    n = t.numel() // t.shape[-1] if t.shape[-1] else 0
+    t = t.reshape(n, t.shape[-1])
+    return t if t.shape[0] <= 1 and t.stride(1) == 1 or t.stride(1) == 1 and t.stride(0) >= t.shape[1] else t.contiguous()
+
+
+def _pitch(t: Tensor) -> int:
+    # the stride of a single row says nothing
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+
+
+def _scratch(device: torch.device, nbytes: int) -> Tensor:
+    return torch.empty(max(int(nbytes), 1), dtype=torch.uint8, device=device)
+
+
+def _int8_codes(t: Tensor, dims: int, what: str) -> Tensor:
+    require_cuda(t, what)
+    if t.dtype != torch.int8 or t.dim() != dims:
+        raise MoeQuantError(f"{what} must be a {dims}-D int8 tensor (got {t.dim()}-D {t.dtype})")
+    if t.shape[-1] > 0 and t.stride(-1) != 1:
+        raise MoeQuantError(f"{what} must have unit column stride")
+    return t
+
+
+def _code_pitch(t: Tensor) -> int:
+    """Bytes from one row of codes to the next; of a single row its padded length, which is never read."""
+    if t.shape[-2] > 1:
+        if t.stride(-2) < t.shape[-1]:
+            raise MoeQuantError("rows of 8-bit codes must not overlap")
+        return t.stride(-2)
+    return (t.shape[-1] + 15) // 16 * 16
+
+
+def _scales(t: Tensor, shape: Tuple[int, ...], what: str) -> Tensor:
+    require_cuda(t, what)
+    n = 1
+    for s in shape:
+        n *= s
+    if not t.is_floating_point() or t.numel() != n or tuple(d for d in t.shape if d != 1) != tuple(d for d in shape if d != 1):
+        raise MoeQuantError(f"{what} of shape {tuple(t.shape)} and {t.dtype}: expected {shape} numbers")
+    return t.to(torch.float32).reshape(shape).contiguous()
+
+
+@dataclass
+class ExpertPlan:
+    """Pairs (token * top_k + slot) grouped by expert: expert e has order[offsets[e]:offsets[e + 1]], in rising order;
+    place[token, slot] is where a pair stands in order.  Pairs without an expert here have place -1, and order ends with
+    as many -1."""
+
+    offsets: Tensor
+    order: Tensor
+    place: Tensor
+
+
+def route_tokens(logits: Tensor, top_k: int, *, score: str = "softmax", bias: Optional[Tensor] = None, groups: int = 1,
+                 keep_groups: Optional[int] = None, group_score: str = "max", renormalise: bool = True,
+                 scale: float = 1.0) -> Tuple[Tensor, Tensor]:
+    """Chooses top_k experts per token.  logits (..., E) fp32/bf16/fp16, bias (E) fp32, added for the choice alone.
+    score "softmax" or "sigmoid"; of `groups` equal runs of experts keep_groups stay, those with the largest value
+    (group_score "max") or sum of two values ("top2").  Returns (ids int32 (..., top_k) in falling order of value, ties to
+    the lowest index, and weights fp32: the scores without bias, divided by their sum with renormalise, times scale).
+    Experts whose logit is -inf or NaN or whose bias is -inf or NaN are never chosen: id -1, weight 0 where none is left."""
+    require_cuda(logits, "logits")
+    code = dtype_code(logits.dtype)
+    if score not in ("softmax", "sigmoid") or group_score not in ("max", "top2"):
+        raise MoeQuantError(f"route_tokens: unknown score {score!r} or group_score {group_score!r}")
+    _forward_only("route_tokens", logits, bias)
+    if logits.dim() < 1:
+        raise MoeQuantError("route_tokens: logits must be (..., E)")
+    E, lead = logits.shape[-1], logits.shape[:-1]
+    if bias is not None:
+        require_one_device("route_tokens", logits, bias)
+        if bias.shape != (E,):
+            raise MoeQuantError(f"route_tokens: bias of shape {tuple(bias.shape)} for {E} experts")
+        bias = bias.to(torch.float32).contiguous()
+    rows = _rows(logits, "logits")
+    T = rows.shape[0]
+    ids = torch.empty(*lead, top_k, dtype=torch.int32, device=logits.device)
+    weights = torch.empty(*lead, top_k, dtype=torch.float32, device=logits.device)
+    with _lib.on_device(logits.device):
+        check(lib().mq_route_tokens(ptr(rows), code, T, E, _pitch(rows), top_k, int(score == "sigmoid"), ptr(bias), groups,
+                                    groups if keep_groups is None else keep_groups, int(group_score == "top2"), int(renormalise), scale,
+                                    ptr(ids), ptr(weights), stream_ptr(logits.device)))
+    return ids, weights
+
+
+def _expert_ids(ids: Tensor) -> Tensor:
+    require_cuda(ids, "ids")
+    if ids.dtype not in (torch.int32, torch.int64):
+        raise MoeQuantError(f"ids must be int32 or int64 (got {ids.dtype})")
+    return ids.to(torch.int32).contiguous()
+
+
+def expert_plan(ids: Tensor, n_experts: int, first: int = 0) -> ExpertPlan:
+    """Groups the pairs of `ids` (..., top_k) by expert, for the experts first .. first + n_experts - 1 (all others, -1 among
+    them, are dropped)."""
+    ids = _expert_ids(ids)
+    dev, P = ids.device, ids.numel()
+    offsets = torch.empty(max(int(n_experts), 0) + 1, dtype=torch.int32, device=dev)
+    order = torch.empty(P, dtype=torch.int32, device=dev)
+    place = torch.empty(ids.shape, dtype=torch.int32, device=dev)
+    L = lib()
+    ws = _scratch(dev, L.mq_expert_plan_workspace_bytes(P, max(int(n_experts), 0)))
+    with _lib.on_device(dev):
+        check(L.mq_expert_plan(ptr(ids), P, n_experts, first, ptr(offsets), ptr(order), ptr(place), ptr(ws), ws.numel(), stream_ptr(dev)))
+    return ExpertPlan(offsets, order, place)
+
+
+def quantize_tokens(x: Tensor) -> Tuple[Tensor, Tensor]:
+    """8-bit codes and one fp32 scale per token of x (..., K): scale = max|x| / 127.  Rows of the codes start 16 bytes apart or a
+    multiple of it, as int8_matmul takes them."""
+    require_cuda(x, "x")
+    code = dtype_code(x.dtype)
+    _forward_only("quantize_tokens", x)
+    rows = _rows(x, "x")
+    T, K = rows.shape
+    lead = x.shape[:-1]
+    pitch = (K + 15) // 16 * 16
+    codes = torch.empty(*lead, pitch, dtype=torch.int8, device=x.device)
+    scale = torch.empty(lead, dtype=torch.float32, device=x.device)
+    with _lib.on_device(x.device):
+        check(lib().mq_quantize_tokens(ptr(rows), code, T, K, _pitch(rows), ptr(codes), pitch, ptr(scale), stream_ptr(x.device)))
+    return codes[..., :K], scale
+
+
+def int8_matmul(x: Tensor, weight: Tensor, weight_scale: Tensor, bias: Optional[Tensor] = None, x_scale: Optional[Tensor] = None,
+                out_dtype: Optional[torch.dtype] = None) -> Tensor:
+    """y = x @ (weight * weight_scale)^T + bias with x rounded to 8-bit codes per token and the sum taken in integers.
+    x (..., K) fp32/bf16/fp16, or int8 codes with their x_scale (...); weight (N, K) int8 with rows 16-byte aligned (int8_layout of
+    the int8 module makes it from GPTQ codes), weight_scale (N).  y has x's type, or out_dtype."""
+    require_cuda(x, "x")
+    _int8_codes(weight, 2, "weight")
+    _forward_only("int8_matmul", x, weight_scale, bias, x_scale)
+    N, K = weight.shape
+    if x.dim() < 1 or x.shape[-1] != K:
+        raise MoeQuantError(f"int8_matmul: x of shape {tuple(x.shape)} does not match weight of shape {tuple(weight.shape)}")
+    given = x.dtype == torch.int8
+    if given != (x_scale is not None):
+        raise MoeQuantError("int8_matmul: x_scale belongs to int8 codes, and they need it")
+    if given and out_dtype is None:
+        raise MoeQuantError("int8_matmul: int8 codes need an out_dtype")
+    out_dtype = x.dtype if out_dtype is None else out_dtype
+    x_code, out_code = MQ_I8 if given else dtype_code(x.dtype), dtype_code(out_dtype)
+    lead = x.shape[:-1]
+    dev = x.device
+    require_one_device("int8_matmul", *(t for t in (x, weight, weight_scale, bias, x_scale) if t is not None))
+    weight_scale = _scales(weight_scale, (N,), "weight_scale")
+    if bias is not None:
+        bias = _scales(bias, (N,), "bias")
+    rows = _rows(x, "x")
+    T = rows.shape[0]
+    if given:
+        x_scale = _scales(x_scale, tuple(lead), "x_scale")
+    y = torch.empty(*lead, N, dtype=out_dtype, device=dev)
+    L = lib()
+    ws = _scratch(dev, L.mq_int8_matmul_workspace_bytes(x_code, T, N, K))
+    with _lib.on_device(dev):
+        check(L.mq_int8_matmul(ptr(rows), x_code, ptr(x_scale), T, K, _code_pitch(rows) if given else _pitch(rows), ptr(weight), N,
+                               _code_pitch(weight), ptr(weight_scale), ptr(bias), out_code, ptr(y), N, ptr(ws), ws.numel(), stream_ptr(dev)))
+    return y
+
+
+def int8_experts(x: Tensor, ids: Tensor, weights: Tensor, gate_up: Tensor, gate_up_scale: Tensor, down: Tensor, down_scale: Tensor,
+                 first: int = 0) -> Tensor:
+    """Sum over a token's experts of weight * down(silu(gate(x)) * up(x)), the products in 8-bit integers as in int8_matmul.
+    x (..., K) bf16/fp16; ids and weights (..., top_k) as route_tokens gives them; gate_up (E, 2 I, K) int8, gate rows first, with
+    gate_up_scale (E, 2 I); down (E, K, I) int8 with down_scale (E, K).  The experts here are first .. first + E - 1, others'
+    pairs add nothing."""
+    require_cuda(x, "x")
+    _int8_codes(gate_up, 3, "gate_up")
+    _int8_codes(down, 3, "down")
+    _forward_only("int8_experts", x, weights, gate_up_scale, down_scale)
+    if x.dtype not in (torch.bfloat16, torch.float16):
+        raise MoeQuantError(f"int8_experts: x must be bf16 or fp16 (got {x.dtype})")
+    E, I2, K = gate_up.shape
+    I = I2 // 2
+    if x.dim() < 1 or x.shape[-1] != K or I2 % 2 or down.shape != (E, K, I):
+        raise MoeQuantError(f"int8_experts: x {tuple(x.shape)}, gate_up {tuple(gate_up.shape)} and down {tuple(down.shape)} do not match")
+    if ids.dim() != x.dim() or ids.shape[:-1] != x.shape[:-1] or weights.shape != ids.shape:
+        raise MoeQuantError(f"int8_experts: ids {tuple(ids.shape)} and weights {tuple(weights.shape)} do not match x {tuple(x.shape)}")
+    require_one_device("int8_experts", x, ids, weights, gate_up, gate_up_scale, down, down_scale)
+    ids = _expert_ids(ids)
+    weights = weights.to(torch.float32).contiguous()
+    gate_up_scale = _scales(gate_up_scale, (E, I2), "gate_up_scale")
+    down_scale = _scales(down_scale, (E, K), "down_scale")
+    rows = _rows(x, "x")
+    T, k = rows.shape[0], ids.shape[-1]
+    dev = x.device
+    y = torch.empty(*x.shape[:-1], K, dtype=x.dtype, device=dev)
+    L = lib()
+    ws = _scratch(dev, L.mq_int8_experts_workspace_bytes(T, k, E, K, I) if T and k and E else 0)
+    with _lib.on_device(dev):
+        check(L.mq_int8_experts(ptr(rows), dtype_code(x.dtype), T, K, _pitch(rows), ptr(ids), ptr(weights), k, first, E, I, ptr(gate_up),
+                                _code_pitch(gate_up), gate_up.stride(0) if E > 1 else 0, ptr(gate_up_scale), ptr(down), _code_pitch(down),
+                                down.stride(0) if E > 1 else 0, ptr(down_scale), ptr(y), K, ptr(ws), ws.numel(), stream_ptr(dev)))
+    return y

@@ -20,6 +20,8 @@ import torch.distributed as dist
 import torch.nn as nn
 import torch.nn.functional as F
 
+from . import ops
+
 
 class _RMSNorm(nn.Module):
     def __init__(self, dim: int, eps: float = 1e-6):
@@ -60,6 +62,15 @@ class _Router(nn.Module):
         w, idx = scores.topk(self.top_k, dim=-1)
         return idx, (w / w.sum(-1, keepdim=True)).to(x.dtype)
 
+    def route(self, x):
+        """The same choice by the engine's router; weights in fp32."""
+        logits = x.float() @ self.weight.float().t()
+        bias = None
+        if self.disabled_experts:
+            bias = logits.new_zeros(logits.shape[1])
+            bias[self.disabled_experts] = -float("inf")
+        return ops.route_tokens(logits, self.top_k, score="sigmoid", bias=bias)
+
 
 class _MoE(nn.Module):
     def __init__(self, hidden: int, inter: int, n_experts: int, top_k: int, expert_parallel: bool = False):
@@ -81,6 +92,7 @@ class _MoE(nn.Module):
         self.experts = nn.ModuleList([_MLP(hidden, inter) for _ in range(n_experts)])
         self._local = set(local)
         self.shared_experts = _MLP(hidden, inter)
+        self.int8_experts = None      # an int8.Int8Experts of the local experts: they then run in 8-bit integers
 
     def drop_remote_experts(self) -> None:
         for i in range(self.n_experts):
@@ -88,6 +100,8 @@ class _MoE(nn.Module):
                 self.experts[i] = None
 
     def _run_experts(self, tokens, expert_ids):
+        if self.int8_experts is not None:
+            return self.int8_experts(tokens, expert_ids[:, None], torch.ones(len(tokens), 1, device=tokens.device))
         out = torch.zeros_like(tokens)
         for e in sorted(self._local):
             rows = (expert_ids == e).nonzero(as_tuple=True)[0]
@@ -98,6 +112,9 @@ class _MoE(nn.Module):
 
     def forward(self, x):
         flat = x.reshape(-1, x.shape[-1])
+        if self.int8_experts is not None and not self.ep:
+            ids, w = self.gate.route(flat)
+            return (self.int8_experts(flat, ids, w) + self.shared_experts(flat)).reshape(x.shape)
         idx, w = self.gate(flat)
         n, k = idx.shape
         pair_token = torch.arange(n, device=flat.device).repeat_interleave(k)
