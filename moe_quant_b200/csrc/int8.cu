@@ -117,83 +117,9 @@ int quantize_rows(const void* x, int dtype, int64_t T, const int32_t* rows_end, 
 }
 
 // ---------------------------------------------------------------- products
-__device__ __forceinline__ float silu_times(float g, float u) { return g / (1.0f + expf(-g)) * u; }
-
-// 64 tokens x 64 weight rows per block, 64 of k at a time in shared memory, four by four results a thread with dp4a.
-constexpr int SIMPLE_TILE = 64, SIMPLE_PITCH = 17;   // words per row of a staged tile
-
-__device__ __forceinline__ void stage_codes(int (&tile)[SIMPLE_TILE][SIMPLE_PITCH], int r, int word, const int8_t* row, int k, int K) {
-  uint32_t v = 0;
-  if (row)
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      if (k + j < K) v |= (uint32_t)(uint8_t)row[k + j] << (8 * j);
-  tile[r][word] = (int)v;
-}
-
-template <int KIND>
-__global__ void __launch_bounds__(256) int8_simple_kernel(const Int8Product p, const Int8Out o) {
-  constexpr int SETS = KIND == INT8_GATED ? 2 : 1;
-  __shared__ int xs[SIMPLE_TILE][SIMPLE_PITCH], ws[SETS][SIMPLE_TILE][SIMPLE_PITCH];
-  const int e = blockIdx.z, n0 = blockIdx.x * SIMPLE_TILE;
-  const int64_t begin = p.offsets ? p.offsets[e] : 0, end = p.offsets ? p.offsets[e + 1] : p.T;
-  const int tx = threadIdx.x & 15, ty = threadIdx.x >> 4;
-  for (int64_t t0 = begin + (int64_t)blockIdx.y * SIMPLE_TILE; t0 < end; t0 += (int64_t)gridDim.y * SIMPLE_TILE) {
-    int acc[SETS][4][4] = {};
-    for (int k0 = 0; k0 < p.K; k0 += 64) {
-      __syncthreads();
-      for (int i = threadIdx.x; i < SIMPLE_TILE * 16; i += 256) {
-        const int r = i >> 4, word = i & 15, k = k0 + word * 4;
-        const int64_t t = t0 + r;
-        const int8_t* row = t < end ? p.x + (p.order ? (int64_t)(p.order[t] / p.top_k) : t) * p.ldx : nullptr;
-        stage_codes(xs, r, word, row, k, p.K);
-#pragma unroll
-        for (int s = 0; s < SETS; ++s)
-          stage_codes(ws[s], r, word, n0 + r < p.rows ? p.w + e * p.w_expert + ((int64_t)s * p.rows + n0 + r) * p.ldw : nullptr, k, p.K);
-      }
-      __syncthreads();
-      for (int w = 0; w < 16; ++w)
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int s = 0; s < SETS; ++s) acc[s][i][j] = __dp4a(xs[ty + 16 * i][w], ws[s][tx + 16 * j][w], acc[s][i][j]);
-    }
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int64_t t = t0 + ty + 16 * i;
-      if (t >= end) continue;
-      const float xsc = p.x_scale[p.order ? (int64_t)(p.order[t] / p.top_k) : t];
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int n = n0 + tx + 16 * j;
-        if (n >= p.rows) continue;
-        if (KIND == INT8_GATED) {
-          const float* sc = p.w_scale + (int64_t)e * 2 * p.rows;
-          const float g = (float)acc[0][i][j] * xsc * sc[n], u = (float)acc[SETS - 1][i][j] * xsc * sc[p.rows + n];
-          static_cast<float*>(o.y)[t * o.ldy + n] = silu_times(g, u);
-        } else {
-          float v = (float)acc[0][i][j] * xsc * p.w_scale[(int64_t)e * p.rows + n];
-          if (KIND == INT8_Y && o.bias) v += o.bias[n];
-          if (KIND == INT8_PAIRS || o.dtype == MQ_F32) static_cast<float*>(o.y)[t * o.ldy + n] = v;
-          else if (o.dtype == MQ_BF16) static_cast<__nv_bfloat16*>(o.y)[t * o.ldy + n] = __float2bfloat16_rn(v);
-          else static_cast<__half*>(o.y)[t * o.ldy + n] = __float2half_rn(v);
-        }
-      }
-    }
-  }
-}
-
 int int8_product(const Int8Product& p, const Int8Out& o, cudaStream_t st) {
   if (p.T == 0 || p.rows == 0) return MQ_OK;
-  const int64_t along = ceil_div(p.T, SIMPLE_TILE);
-  dim3 grid((unsigned)ceil_div(p.rows, SIMPLE_TILE), (unsigned)(along < 65535 ? along : 65535), (unsigned)p.E);
-  if (o.kind == INT8_GATED) int8_simple_kernel<INT8_GATED><<<grid, 256, 0, st>>>(p, o);
-  else if (o.kind == INT8_PAIRS) int8_simple_kernel<INT8_PAIRS><<<grid, 256, 0, st>>>(p, o);
-  else int8_simple_kernel<INT8_Y><<<grid, 256, 0, st>>>(p, o);
-  MQ_LAUNCH_CHECK();
-  return MQ_OK;
+  return int8_product_umma(p, o, st);
 }
 
 // y[t] = sum over the token's pairs, in the order of its slots, of weight * (the pair's down product)

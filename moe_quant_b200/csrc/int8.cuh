@@ -39,4 +39,6 @@ struct Int8Out {
   const float* bias;
 };
 
+int int8_product_umma(const Int8Product& p, const Int8Out& o, cudaStream_t st);   // on the tensor cores (int8_umma.cu)
+
 }  // namespace mq

@@ -1,0 +1,404 @@
+// The 8-bit integer product on the fifth-generation tensor cores (tcgen05.mma kind::i8, sums in 32-bit integers in tensor
+// memory: exact).
+//
+// The weights are the operand of 128 rows per CTA, the tokens the one of up to 256 columns, so a tile can be as narrow as the tokens
+// that there are (32 and up in steps of 32) while weights fill the tensor core.  Two CTAs of a cluster share a tile of 256 weight
+// rows (cta_group::2): each keeps 128 of them and half of the tokens, 32 KB per 128 of k instead of 48.
+//   warp 0 of either CTA : TMA, six stages of 32 KB; weights by tiles, tokens by tiles or, where the pairs' order says which
+//                          token comes where, four rows at a time (gather4); the bytes of both CTAs count on the leader's barrier
+//   warp 1 of the leader : tcgen05.mma for both SMs, two accumulators of 256 columns by turns
+//   warps 4 .. 11        : epilogue, a quarter of the CTA's weight rows each, chunks of 32 tokens by turns
+// Persistent: a pair of CTAs takes every 74th tile.  Eight tiles of weight rows at a time go with all tiles of tokens, so that the
+// SMs that run side by side share rows of either in the L2.
+#include "int8.cuh"
+#include "profile.cuh"
+#include "umma_pair.cuh"
+
+namespace mq {
+namespace {
+
+constexpr int I8_STAGES = 6, I8_THREADS = 384, I8_K = 128, I8_TILE_BYTES = 128 * I8_K, I8_MAX_WIDTH = 256, I8_ROW_GROUP = 8;
+constexpr int I8_PAIRS = 74;
+constexpr uint32_t I8_STAGE_BYTES = 2 * I8_TILE_BYTES;
+constexpr int I8_MAX_EXPERTS = 1024;
+constexpr size_t kInt8Smem = (size_t)I8_STAGES * I8_STAGE_BYTES + 1024;
+
+struct PairArgs {
+  Int8Product p;
+  Int8Out o;
+  int max_width, m_tiles;
+  int packed;      // two neighbouring results of a token are stored together
+  int* fault;
+};
+
+__device__ __forceinline__ void load_weights_pair(uint32_t dst, const CUtensorMap* map, uint32_t bar, int k, int row, int set, int e) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(k), "r"(row), "r"(set), "r"(e)
+      : "memory");
+}
+__device__ __forceinline__ void load_tokens_pair(uint32_t dst, const CUtensorMap* map, uint32_t bar, int k, int row) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(k), "r"(row)
+      : "memory");
+}
+__device__ __forceinline__ void gather_tokens_pair(uint32_t dst, const CUtensorMap* map, uint32_t bar, int k, int4 rows) {
+  asm volatile(
+      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
+      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(k), "r"(rows.x), "r"(rows.y), "r"(rows.z), "r"(rows.w)
+      : "memory");
+}
+__device__ __forceinline__ void umma_i8_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::i8 [%0], %1, %2, %3, p;\n\t}"
+      ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void tmem_ld32_int(uint32_t taddr, int (&r)[32]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+      "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
+        "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
+        "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+      : "r"(taddr)
+      : "memory");
+  asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+}
+
+// Tiles of tokens of an expert with `count` rows, and their width: as few as the widest tile allows, all of one width.
+__host__ __device__ __forceinline__ int token_tiles(int64_t count, int max_width) { return (int)((count + max_width - 1) / max_width); }
+__host__ __device__ __forceinline__ int tile_width(int64_t count, int tiles) { return (int)((((count + tiles - 1) / tiles) + 31) / 32 * 32); }
+
+// The tile that comes `unit`-th: which expert, which weight rows, which of its tokens.
+struct Unit {
+  int e, m, width;
+  int t0, t_end;     // rows of the result
+  __device__ __forceinline__ bool seek(int64_t unit, const PairArgs& a, const int* offsets, const int* tiles_before) {
+    if (unit >= (int64_t)tiles_before[a.p.E] * a.m_tiles) return false;
+    int lo = 0, hi = a.p.E;      // the last expert whose tiles begin at or in front of this one
+    while (hi - lo > 1) {
+      const int mid = (lo + hi) >> 1;
+      if ((int64_t)tiles_before[mid] * a.m_tiles <= unit) lo = mid;
+      else hi = mid;
+    }
+    e = lo;
+    const int begin = offsets[e], end = offsets[e + 1], n_tiles = tiles_before[e + 1] - tiles_before[e];
+    const int i = (int)(unit - (int64_t)tiles_before[e] * a.m_tiles);
+    const int g = i / (I8_ROW_GROUP * n_tiles), r = i - g * I8_ROW_GROUP * n_tiles;
+    const int in_group = min(I8_ROW_GROUP, a.m_tiles - g * I8_ROW_GROUP);
+    m = g * I8_ROW_GROUP + r % in_group;
+    width = tile_width(end - begin, n_tiles);
+    t0 = begin + r / in_group * width;
+    t_end = min(t0 + width, end);
+    return true;
+  }
+};
+
+__device__ __forceinline__ float gated(float g, float u) { return g / (1.0f + expf(-g)) * u; }
+
+template <int KIND>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
+    int8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const PairArgs a) {
+  constexpr int SETS = KIND == INT8_GATED ? 2 : 1;
+  constexpr int TILE_ROWS = 256 / SETS;            // result columns of a tile
+  const Int8Product& p = a.p;
+  const int rank = (int)(blockIdx.x & 1), pair = (int)(blockIdx.x >> 1), n_pairs = (int)(gridDim.x >> 1);
+  const int slabs = (p.K + I8_K - 1) / I8_K;
+
+  extern __shared__ uint8_t smem_raw[];
+  const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
+  __shared__ __align__(8) uint64_t bars[2 * I8_STAGES + 4];
+  __shared__ uint32_t tmem_slot;
+  __shared__ PairEnd end;
+  __shared__ int offsets[I8_MAX_EXPERTS + 1], tiles_before[I8_MAX_EXPERTS + 1];
+  __shared__ __align__(16) float token_scale[8][32];
+  const uint32_t full0 = smem_u32(&bars[0]), empty0 = smem_u32(&bars[I8_STAGES]);
+  const uint32_t acc_full = smem_u32(&bars[2 * I8_STAGES]), acc_empty = smem_u32(&bars[2 * I8_STAGES + 2]);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < I8_STAGES; ++s) {
+      mbar_init(full0 + 8 * s, 1);    // the leader's: its producer's arrival, then the bytes of both CTAs
+      mbar_init(empty0 + 8 * s, 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(acc_full + 8 * b, 1);
+      mbar_init(acc_empty + 8 * b, 16);  // the leader's: eight epilogue warps of either CTA
+    }
+    end.reset();
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) tmem_alloc_pair(smem_u32(&tmem_slot));
+  chain_wait();
+  chain_release();
+  if (warp == 2) {   // where each expert's rows and tiles begin
+    int before = 0;
+    for (int e0 = 0; e0 < p.E; e0 += 32) {
+      const int e = e0 + lane;
+      int tiles = 0;
+      if (e < p.E) {
+        const int begin = p.offsets ? __ldcg(p.offsets + e) : 0, last = p.offsets ? __ldcg(p.offsets + e + 1) : (int)p.T;
+        offsets[e] = begin;
+        if (e == p.E - 1) offsets[p.E] = last;
+        tiles = token_tiles(last - begin, a.max_width);
+      }
+      int sum = tiles;
+      for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += u;
+      }
+      if (e < p.E) tiles_before[e] = before + sum - tiles;
+      before += __shfl_sync(0xffffffffu, sum, 31);
+    }
+    if (lane == 0) tiles_before[p.E] = before;
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();   // either CTA's barriers and tensor memory exist before the other signals or writes them
+  tc_fence_after();
+  const uint32_t tmem_acc = tmem_slot;
+
+  if (warp == 0) {
+    const uint32_t full_leader = leader_addr(full0);
+    int it = 0;
+    bool ok = true;
+    Unit u;
+    for (int64_t unit = pair; ok && u.seek(unit, a, offsets, tiles_before); unit += n_pairs) {
+      const int half = u.width >> 1;
+      const int b_row = u.t0 + rank * half;
+      int4 rows = make_int4(0, 0, 0, 0);
+      if (p.order) {   // rows behind the last token repeat it; nothing is stored of them
+        const int t = b_row + 4 * lane, last = u.t_end - 1;
+        rows = make_int4(__ldcg(p.order + min(t, last)) / p.top_k, __ldcg(p.order + min(t + 1, last)) / p.top_k,
+                         __ldcg(p.order + min(t + 2, last)) / p.top_k, __ldcg(p.order + min(t + 3, last)) / p.top_k);
+      }
+      const int n_boxes = (half + 31) / 32;
+      const uint32_t bytes = 2 * (I8_TILE_BYTES + (uint32_t)(p.order ? half : n_boxes * 32) * I8_K);
+      for (int s = 0; s < slabs; ++s, ++it) {
+        const int st = it % I8_STAGES;
+        if (it >= I8_STAGES && !mbar_wait(empty0 + 8 * st, ((it / I8_STAGES) - 1) & 1, a.fault, 91)) { ok = false; break; }
+        const uint32_t dst = smem_base + (uint32_t)st * I8_STAGE_BYTES, bar = full_leader + 8 * st;
+        if (lane == 0) {
+          if (rank == 0) mbar_expect_tx(full0 + 8 * st, bytes);
+          if constexpr (KIND == INT8_GATED) {
+            // sixteen gate rows, then the sixteen up rows of the same results, for each quarter of the CTA's rows
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              load_weights_pair(dst + q * (I8_TILE_BYTES / 4), &map_w, bar, s * I8_K, u.m * TILE_ROWS + rank * 64 + q * 16, 0, u.e);
+          } else {
+            load_weights_pair(dst, &map_w, bar, s * I8_K, u.m * TILE_ROWS + rank * 128, 0, u.e);
+          }
+          if (!p.order)
+            for (int j = 0; j < n_boxes; ++j) load_tokens_pair(dst + I8_TILE_BYTES + j * 32 * I8_K, &map_x, bar, s * I8_K, b_row + 32 * j);
+        }
+        __syncwarp();
+        if (p.order && 4 * lane < half) gather_tokens_pair(dst + I8_TILE_BYTES + 4 * lane * I8_K, &map_x, bar, s * I8_K, rows);
+        __syncwarp();
+      }
+    }
+    ok = PairEnd::await_stages<I8_STAGES>(empty0, it, ok, a.fault, 95);
+    if (lane == 0) {
+      end.copied_by(rank, it);
+      if (!ok) end.give_up();
+    }
+  } else if (warp == 1) {
+    if (rank == 0) {
+      int it = 0, n = 0;
+      bool ok = true;
+      Unit u;
+      for (int64_t unit = pair; ok && u.seek(unit, a, offsets, tiles_before); unit += n_pairs, ++n) {
+        const int b = n & 1;
+        // sums of 32 bits, signed 8-bit operands, 256 rows, `width` columns
+        const uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(u.width >> 3) << 17) | ((uint32_t)(256 >> 4) << 24);
+        const uint32_t acc = tmem_acc + (uint32_t)(b * I8_MAX_WIDTH);
+        if (n >= 2) ok = mbar_wait(acc_empty + 8 * b, ((n >> 1) - 1) & 1, a.fault, 93);
+        tc_fence_after();
+        for (int s = 0; s < slabs && ok; ++s) {
+          const int st = it % I8_STAGES;
+          ok = mbar_wait(full0 + 8 * st, (it / I8_STAGES) & 1, a.fault, 92);
+          if (!ok) break;
+          tc_fence_after();
+          if (lane == 0) {
+            const uint32_t a_tile = smem_base + (uint32_t)st * I8_STAGE_BYTES;
+            const uint64_t a0 = kmajor_sw128_desc(a_tile), b0 = kmajor_sw128_desc(a_tile + I8_TILE_BYTES);
+#pragma unroll
+            for (int kk = 0; kk < I8_K / 32; ++kk)
+              umma_i8_pair(acc, a0 + (uint64_t)((kk * 32) >> 4), b0 + (uint64_t)((kk * 32) >> 4), idesc, (s | kk) > 0 ? 1u : 0u);
+            umma_commit_pair(empty0 + 8 * st);
+            if (s == slabs - 1) umma_commit_pair(acc_full + 8 * b);
+          }
+          __syncwarp();
+          ++it;
+        }
+        if (!ok) break;
+      }
+      if (lane == 0) {
+        end.multiplied(it, n);
+        if (!ok) end.give_up();
+      }
+    }
+  } else if (warp >= 4) {
+    const int h = (warp - 4) >> 2, q = warp & 3;   // which chunks of 32 tokens, TMEM lane quadrant
+    const uint32_t empty_leader = leader_addr(acc_empty);
+    const uint32_t t_lane = tmem_acc + ((uint32_t)(q * 32) << 16);
+    float* my_scale = token_scale[warp - 4];
+    bool ok = true;
+    int n = 0;
+    Unit u;
+    for (int64_t unit = pair; ok && u.seek(unit, a, offsets, tiles_before); unit += n_pairs, ++n) {
+      const int b = n & 1;
+      const int col = KIND == INT8_GATED ? u.m * TILE_ROWS + rank * 64 + q * 16 + (lane & 15) : u.m * TILE_ROWS + rank * 128 + q * 32 + lane;
+      const bool col_in = col < p.rows;
+      const int w_row = KIND == INT8_GATED ? (lane >> 4) * p.rows + col : col;
+      const float ws = col_in ? __ldg(p.w_scale + (int64_t)u.e * SETS * p.rows + w_row) : 0.0f;
+      const float bias = KIND == INT8_Y && a.o.bias && col_in ? __ldg(a.o.bias + col) : 0.0f;
+      const int chunks = u.width >> 5;
+      float xs[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int t = u.t0 + (2 * i + h) * 32 + lane;
+        xs[i] = 0.0f;
+        if (2 * i + h < chunks && t < u.t_end) xs[i] = __ldcg(p.x_scale + (p.order ? __ldcg(p.order + t) / p.top_k : t));
+      }
+      ok = mbar_wait(acc_full + 8 * b, (n >> 1) & 1, a.fault, 94);
+      if (!ok) break;
+      tc_fence_after();
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int c = 2 * i + h;
+        if (c >= chunks) break;
+        int r[32];
+        tmem_ld32_int(t_lane + (uint32_t)(b * I8_MAX_WIDTH + c * 32), r);
+        __syncwarp();
+        my_scale[lane] = xs[i];
+        __syncwarp();
+        const int t = u.t0 + c * 32, left = u.t_end - t;     // tokens of this chunk that exist
+        float v[32];
+#pragma unroll
+        for (int j = 0; j < 32; j += 4) {
+          const float4 s4 = *reinterpret_cast<const float4*>(my_scale + j);
+          v[j] = (float)r[j] * s4.x * ws;
+          v[j + 1] = (float)r[j + 1] * s4.y * ws;
+          v[j + 2] = (float)r[j + 2] * s4.z * ws;
+          v[j + 3] = (float)r[j + 3] * s4.w * ws;
+        }
+        if constexpr (KIND == INT8_GATED) {
+          // lanes 0 .. 15 hold the gate, 16 .. 31 the up of the same results: the former take the even tokens, the latter the odd
+          const bool up = lane >= 16;
+          float* out = static_cast<float*>(a.o.y) + (int64_t)(t + up) * a.o.ldy + col;
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) {
+            const float other = __shfl_xor_sync(0xffffffffu, up ? v[j] : v[j + 1], 16);
+            const float hv = up ? gated(other, v[j + 1]) : gated(v[j], other);
+            if (col_in && j + up < left) out[(int64_t)j * a.o.ldy] = hv;
+          }
+        } else {
+          if constexpr (KIND == INT8_Y) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j) v[j] += bias;
+          }
+          if (KIND == INT8_Y && a.packed) {
+            // neighbouring lanes hold neighbouring results of a token: the even one takes both of the even tokens, the odd one of the odd
+            const bool odd = lane & 1;
+            const int64_t at = (int64_t)(t + odd) * a.o.ldy + (col & ~1);
+#pragma unroll
+            for (int j = 0; j < 32; j += 2) {
+              const float other = __shfl_xor_sync(0xffffffffu, odd ? v[j] : v[j + 1], 1);
+              const float lo = odd ? other : v[j], hi = odd ? v[j + 1] : other;
+              if (col_in && j + odd < left) {
+                if (a.o.dtype == MQ_BF16) *reinterpret_cast<__nv_bfloat162*>(static_cast<__nv_bfloat16*>(a.o.y) + at + (int64_t)j * a.o.ldy) = __floats2bfloat162_rn(lo, hi);
+                else if (a.o.dtype == MQ_F16) *reinterpret_cast<__half2*>(static_cast<__half*>(a.o.y) + at + (int64_t)j * a.o.ldy) = __floats2half2_rn(lo, hi);
+                else *reinterpret_cast<float2*>(static_cast<float*>(a.o.y) + at + (int64_t)j * a.o.ldy) = make_float2(lo, hi);
+              }
+            }
+          } else {
+            const int64_t at = (int64_t)t * a.o.ldy + col;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              if (col_in && j < left) {
+                if (KIND == INT8_PAIRS || a.o.dtype == MQ_F32) static_cast<float*>(a.o.y)[at + (int64_t)j * a.o.ldy] = v[j];
+                else if (a.o.dtype == MQ_BF16) static_cast<__nv_bfloat16*>(a.o.y)[at + (int64_t)j * a.o.ldy] = __float2bfloat16_rn(v[j]);
+                else static_cast<__half*>(a.o.y)[at + (int64_t)j * a.o.ldy] = __float2half_rn(v[j]);
+              }
+            }
+          }
+        }
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(empty_leader + 8 * b);
+    }
+    if (lane == 0 && !ok) end.give_up();
+    __syncwarp();
+  }
+  tc_fence_before();
+  __syncthreads();
+  cluster_sync();   // neither CTA issues a copy, an MMA or an arrival any more
+  if (end.given_up) {   // the same in both CTAs
+    if (warp == 0) end.drain<I8_STAGES>(rank, full0, empty0, acc_full);
+    __syncthreads();
+    cluster_sync();   // the other CTA's copies signal the leader's barriers
+  }
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem_acc);
+  }
+}
+
+int encode(EncodeTiledFn enc, CUtensorMap* map, int rank, const void* base, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box) {
+  const cuuint32_t ones[4] = {1, 1, 1, 1};
+  const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, (cuuint32_t)rank, const_cast<void*>(base), dims, strides, box, ones,
+                         CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  MQ_REQUIRE(r == CUDA_SUCCESS, MQ_ERR_CUDA, "cuTensorMapEncodeTiled failed with %d for codes of %llu x %llu", (int)r, (unsigned long long)dims[1],
+             (unsigned long long)dims[0]);
+  return MQ_OK;
+}
+
+template <int KIND>
+int launch(const CUtensorMap& map_w, const CUtensorMap& map_x, const PairArgs& a, int pairs, cudaStream_t st) {
+  MQ_CUDA(cudaFuncSetAttribute(int8_pair_kernel<KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kInt8Smem));
+  MQ_CUDA(launch_chained(true, int8_pair_kernel<KIND>, dim3((unsigned)(2 * pairs)), dim3(I8_THREADS), kInt8Smem, st, map_w, map_x, a));
+  MQ_LAUNCH_CHECK();
+  return MQ_OK;
+}
+
+}  // namespace
+
+int int8_product_umma(const Int8Product& p, const Int8Out& o, cudaStream_t st) {
+  EncodeTiledFn enc;
+  MQ_TRY(get_encoder(&enc));
+  PairArgs a = {};
+  a.p = p;
+  a.o = o;
+  MQ_TRY(engine_fault_word(&a.fault));
+  const int sets = o.kind == INT8_GATED ? 2 : 1;
+  CUtensorMap map_w, map_x;
+  {
+    const cuuint64_t dims[4] = {(cuuint64_t)p.K, (cuuint64_t)p.rows, (cuuint64_t)sets, (cuuint64_t)p.E};
+    const cuuint64_t set = (cuuint64_t)p.ldw * p.rows, expert = p.E > 1 ? (cuuint64_t)p.w_expert : set * sets;
+    const cuuint64_t strides[3] = {(cuuint64_t)p.ldw, set, expert};
+    const cuuint32_t box[4] = {I8_K, sets == 2 ? 16u : 128u, (cuuint32_t)sets, 1};
+    MQ_TRY(encode(enc, &map_w, 4, p.w, dims, strides, box));
+  }
+  {
+    const cuuint64_t dims[2] = {(cuuint64_t)p.K, (cuuint64_t)p.x_rows};
+    const cuuint64_t strides[1] = {(cuuint64_t)p.ldx};
+    const cuuint32_t box[2] = {I8_K, p.order ? 1u : 32u};
+    MQ_TRY(encode(enc, &map_x, 2, p.x, dims, strides, box));
+  }
+  a.m_tiles = (int)ceil_div(p.rows, 256 / sets);
+  a.max_width = I8_MAX_WIDTH;
+  const int64_t most = (int64_t)a.m_tiles * (p.offsets ? ceil_div(p.T, a.max_width) + p.E : token_tiles(p.T, a.max_width));
+  const int pairs = (int)(most < I8_PAIRS ? most : I8_PAIRS);
+  const size_t size = o.kind != INT8_Y ? 4 : dtype_size(o.dtype);
+  a.packed = p.rows % 2 == 0 && o.ldy % 2 == 0 && aligned(o.y, 2 * size);
+  if (o.kind == INT8_GATED) return launch<INT8_GATED>(map_w, map_x, a, pairs, st);
+  if (o.kind == INT8_PAIRS) return launch<INT8_PAIRS>(map_w, map_x, a, pairs, st);
+  return launch<INT8_Y>(map_w, map_x, a, pairs, st);
+}
+
+}  // namespace mq

@@ -33,10 +33,24 @@
 #include "engine.cuh"
 #include "mbarrier.cuh"
 #include "profile.cuh"
+#include "umma_pair.cuh"
 
 namespace mq {
 
 __device__ int g_engine_fault = 0;
+
+int get_encoder(EncodeTiledFn* out) {
+  static EncodeTiledFn fn = nullptr;
+  if (!fn) {
+    void* sym = nullptr;
+    cudaDriverEntryPointQueryResult qres;
+    MQ_CUDA(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &sym, cudaEnableDefault, &qres));
+    MQ_REQUIRE(sym && qres == cudaDriverEntryPointSuccess, MQ_ERR_CUDA, "cuTensorMapEncodeTiled is not available in this driver");
+    fn = reinterpret_cast<EncodeTiledFn>(sym);
+  }
+  *out = fn;
+  return MQ_OK;
+}
 
 namespace {
 
@@ -79,9 +93,6 @@ struct UmmaParams {
 };
 
 // ---------------------------------------------------------------- PTX wrappers
-__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
-  asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-}
 // Bounded waits: they give up after about one second and record `code`.
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, int code) { return mq::mbar_wait(bar, parity, &g_engine_fault, code); }
 __device__ __forceinline__ bool mbar_wait_lane(uint32_t bar, uint32_t parity, int code) { return mq::mbar_wait_lane(bar, parity, &g_engine_fault, code); }
@@ -106,7 +117,6 @@ __device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.comm
 __device__ __forceinline__ void bulk_wait_read_1() { asm volatile("cp.async.bulk.wait_group.read 1;" ::: "memory"); }
 __device__ __forceinline__ void bulk_wait_all() { asm volatile("cp.async.bulk.wait_group 0;" ::: "memory"); }
 __device__ __forceinline__ void bulk_wait_read_all() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
-__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 __device__ __forceinline__ void tma_load_2d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
   asm volatile(
       "cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
@@ -130,9 +140,6 @@ __device__ __forceinline__ void umma_bf16(uint32_t tmem_d, uint64_t adesc, uint6
 __device__ __forceinline__ void umma_commit(uint32_t bar) {
   asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-
 __device__ __forceinline__ void tmem_ld32(uint32_t taddr, float (&v)[32]) {
   uint32_t r[32];
   asm volatile(
@@ -173,17 +180,6 @@ __device__ __forceinline__ void tmem_acc_row(uint32_t taddr, float f, float (&su
 #pragma unroll
     for (int j = 0; j < 32; ++j) sum[c * 32 + j] = fmaf(f, v[j], sum[c * 32 + j]);
   }
-}
-
-// Matrix descriptor of a K-major tile with the 128-byte swizzle: rows of 128 bytes,
-// groups of 8 rows 1024 bytes apart (stride byte offset), descriptor version 1.
-__device__ __forceinline__ uint64_t kmajor_sw128_desc(uint32_t smem_addr) {
-  uint64_t d = (uint64_t)((smem_addr & 0x3FFFFu) >> 4);
-  d |= (uint64_t)1 << 16;            // leading byte offset: unused with a swizzle
-  d |= (uint64_t)(1024 >> 4) << 32;  // stride byte offset
-  d |= (uint64_t)1 << 46;            // version
-  d |= (uint64_t)2 << 61;            // SWIZZLE_128B
-  return d;
 }
 
 // Matrix descriptor of an MN-major operand with the 128-byte swizzle, as a TMA box of
@@ -1138,22 +1134,6 @@ constexpr int PAIR_TILE = 256, PAIR_STAGES = 3, PAIR_THREADS = 384;
 constexpr uint32_t PAIR_STAGE_BYTES = 4 * PLANE_TILE_BYTES;
 constexpr size_t kPairSmem = (size_t)PAIR_STAGES * PAIR_STAGE_BYTES + 8 * 4096 + 1024;
 
-__device__ __forceinline__ uint32_t leader_addr(uint32_t local) {   // the same shared-memory location in the cluster's CTA 0
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(local));
-  return r;
-}
-__device__ __forceinline__ void set_in_cta(int* local, int rank, int v) {   // *local of the cluster's CTA `rank`
-  uint32_t r;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(local)), "r"(rank));
-  asm volatile("st.shared::cluster.s32 [%0], %1;" ::"r"(r), "r"(v) : "memory");
-}
-__device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
-  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
 __device__ __forceinline__ void tma_load_3d_pair(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2) {
   asm volatile(
       "cp.async.bulk.tensor.3d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];"
@@ -1167,68 +1147,12 @@ __device__ __forceinline__ void umma_f16_pair(uint32_t tmem_d, uint64_t adesc, u
       ::"r"(tmem_d), "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
       : "memory");
 }
-// arrives on this barrier of both CTAs once the MMAs issued so far have completed
-__device__ __forceinline__ void umma_commit_pair(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
-               ::"r"(bar), "h"((uint16_t)3) : "memory");
-}
-// A wait that only the clock ends (a fault elsewhere does not): for what is still under way after a wait was given up.
-__device__ __forceinline__ void mbar_drain(uint32_t bar, uint32_t parity) {
-  const uint64_t t0 = global_ns();
-  while (!mbar_try(bar, parity))
-    if (global_ns() - t0 > 100000000ull) return;
-}
-
 __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
   asm volatile(
       "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
       ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1)
       : "memory");
 }
-__device__ __forceinline__ void tmem_alloc_pair(uint32_t dst_smem) {   // all 512 columns of both CTAs
-  asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(dst_smem) : "memory");
-  asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void tmem_dealloc_pair(uint32_t taddr) {
-  asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(taddr) : "memory");
-}
-
-// What the two CTAs must know of each other before they leave: a wait of either was given up, slabs multiplied and accumulators handed over (set in
-// both), slabs whose copies either producer has issued (the leader's).  With every wait satisfied nothing is under way at the end: the
-// producers have seen the last commits on `empty` (await_stages), the epilogue warps all of those on `acc_full`, and the cluster barrier orders
-// the arrivals on the leader's `acc_empty`.  After a wait that was given up what is under way comes to its end first (drain): the MMAs through
-// their commits, of which the last use of every barrier is known, the copies through the leader's `full` (a stage that one
-// producer alone has filled never completes; the copy lands long before that wait runs out).
-struct PairEnd {
-  int given_up, n_multiplied, n_accs, n_copied[2];
-  __device__ __forceinline__ void reset() { given_up = n_multiplied = n_accs = n_copied[0] = n_copied[1] = 0; }
-  __device__ __forceinline__ void give_up() {
-    set_in_cta(&given_up, 0, 1);
-    set_in_cta(&given_up, 1, 1);
-  }
-  __device__ __forceinline__ void multiplied(int slabs, int accs) {
-    for (int c = 0; c < 2; ++c) {
-      set_in_cta(&n_multiplied, c, slabs);
-      set_in_cta(&n_accs, c, accs);
-    }
-  }
-  __device__ __forceinline__ void copied_by(int rank, int slabs) { set_in_cta(&n_copied[rank], 0, slabs); }
-  // by the producers' warps: the last use of every stage has been read (so its copies had landed) and its commit has arrived in this CTA
-  template <int NST>
-  static __device__ __forceinline__ bool await_stages(uint32_t empty0, int slabs, bool ok, int code) {
-    for (int j = slabs > NST ? slabs - NST : 0; j < slabs && ok; ++j) ok = mbar_wait(empty0 + 8 * (j % NST), (j / NST) & 1, code);
-    return ok;
-  }
-  template <int NST>
-  __device__ __forceinline__ void drain(int rank, uint32_t full0, uint32_t empty0, uint32_t acc_full) const {
-    for (int j = n_multiplied > NST ? n_multiplied - NST : 0; j < n_multiplied; ++j) mbar_drain(empty0 + 8 * (j % NST), (j / NST) & 1);
-    for (int j = n_accs > 2 ? n_accs - 2 : 0; j < n_accs; ++j) mbar_drain(acc_full + 8 * (j & 1), (j >> 1) & 1);
-    if (rank != 0) return;
-    const int c = n_copied[0] > n_copied[1] ? n_copied[0] : n_copied[1];
-    for (int j = c > NST ? c - NST : 0; j < c; ++j) mbar_drain(full0 + 8 * (j % NST), (j / NST) & 1);
-  }
-};
-
 // DOT: nothing is stored; B is upper triangular (rows past a tile's last column hold nothing: k stops there), tiles are
 // taken from the right, longest first, and the epilogue sums the tile's products with A in fp64.
 __device__ __forceinline__ void pair_tile(TileWalk& w, int idx, int n_tiles, int m_tiles, bool dot, int upper) {
@@ -1311,7 +1235,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
           __syncwarp();
         }
       }
-      ok = PairEnd::await_stages<PAIR_STAGES>(empty0, it, ok, 55);
+      ok = PairEnd::await_stages<PAIR_STAGES>(empty0, it, ok, &g_engine_fault, 55);
       if (lane == 0) {
         end.copied_by(rank, it);
         if (!ok) end.give_up();
@@ -1692,7 +1616,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(PAIR_THREADS, 1)
         __syncwarp();
       }
     }
-    ok = PairEnd::await_stages<GRAM_STAGES>(empty0, it, ok, 75);
+    ok = PairEnd::await_stages<GRAM_STAGES>(empty0, it, ok, &g_engine_fault, 75);
     if (lane == 0) {
       end.copied_by(rank, it);
       if (!ok) end.give_up();
@@ -2131,23 +2055,6 @@ __global__ void __launch_bounds__(256) transpose16_kernel(const uint16_t* __rest
 }
 
 // ---------------------------------------------------------------- host side
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-int get_encoder(EncodeTiledFn* out) {
-  static EncodeTiledFn fn = nullptr;
-  if (!fn) {
-    void* sym = nullptr;
-    cudaDriverEntryPointQueryResult qres;
-    MQ_CUDA(cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &sym, cudaEnableDefault, &qres));
-    MQ_REQUIRE(sym && qres == cudaDriverEntryPointSuccess, MQ_ERR_CUDA, "cuTensorMapEncodeTiled is not available in this driver");
-    fn = reinterpret_cast<EncodeTiledFn>(sym);
-  }
-  *out = fn;
-  return MQ_OK;
-}
-
 int encode_map(const PlaneSet& ps, CUtensorMap* map) {
   EncodeTiledFn enc;
   MQ_TRY(get_encoder(&enc));
