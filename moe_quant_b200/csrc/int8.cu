@@ -18,102 +18,178 @@ int expert_plan(const int32_t* ids, int64_t pairs, int E, int first, int32_t* of
 namespace {
 
 // ---------------------------------------------------------------- codes of tokens
-// code = round_half_even(127 x / top).  The product with 127 / top is off by less than 2.4e-5 of a code (three roundings of a number
-// up to 127); where that could decide between two codes, the quotient is formed in 64 bits, whose error of 127 * 2^-53 is below
-// the distance of any quotient of two fp32 numbers from a middle that it does not equal (at least 2^-25 / 254).
-__device__ __forceinline__ float code_of(float x, float top, float inv) {
-  const float q = x * inv;
-  float r = rintf(q);
-  if (fabsf(q - r) > 0.4999f) r = (float)rint(127.0 * (double)x / (double)top);
-  return r;
-}
+// code = round_half_even(127 x / top).  x * (127 / top) is formed and rounded to an integer in one fused step, by adding 1.5 * 2^23; the
+// one rounding in front, that of 127 / top, moves it by at most 127 * 2^-24 = 7.6e-6 of a code.  Where the fraction lies that near to a
+// middle the quotient is formed in 64 bits, whose error of 127 * 2^-53 is below the distance of any quotient of two fp32 numbers
+// from a middle that it does not equal (at least 2^-25 / 254).
+constexpr float TO_INTEGER = 12582912.0f;
+constexpr float NEAR_MIDDLE = 0.49999f;
 
 template <typename T>
 struct alignas(8 * sizeof(T)) Eight { T v[8]; };
-struct alignas(8) EightCodes { int8_t v[8]; };
 
-// G lanes per row (32, or the whole block), eight values per lane and step.  The row is read twice, the second time from the L1/L2.
-template <int DT, int G, bool VEC>
-__global__ void __launch_bounds__(256) quantize_rows_kernel(const void* __restrict__ x, int64_t ldx, int64_t T, const int32_t* __restrict__ rows_end,
-                                                            int K, int8_t* __restrict__ codes, int64_t ldc, float* __restrict__ scale) {
+// the largest |x| as bits, NaN above infinity above all numbers
+__device__ __forceinline__ uint32_t largest_bits(const Eight<float>& a) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(a.v[j]) & 0x7FFFFFFFu);
+  return m;
+}
+template <typename T, typename T2>
+__device__ __forceinline__ uint32_t largest_bits_16(const Eight<T>& a) {
+  const T2* p = reinterpret_cast<const T2*>(a.v);
+  const T2 m = __hmax2_nan(__hmax2_nan(__habs2(p[0]), __habs2(p[1])), __hmax2_nan(__habs2(p[2]), __habs2(p[3])));
+  return __float_as_uint(to_float(__hmax_nan(m.x, m.y))) & 0x7FFFFFFFu;
+}
+__device__ __forceinline__ uint32_t largest_bits(const Eight<__nv_bfloat16>& a) { return largest_bits_16<__nv_bfloat16, __nv_bfloat162>(a); }
+__device__ __forceinline__ uint32_t largest_bits(const Eight<__half>& a) { return largest_bits_16<__half, __half2>(a); }
+
+// the codes of eight values, four to a word
+template <typename T>
+__device__ __forceinline__ uint2 codes_of(const Eight<T>& a, float top, float inv, float lift) {
+  float r[8], off[8], far = 0.0f;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) {
+    const float x = to_float(a.v[j]) * lift;
+    r[j] = __fmaf_rn(x, inv, TO_INTEGER);
+    off[j] = fabsf(__fmaf_rn(x, inv, -(r[j] - TO_INTEGER)));
+    far = fmaxf(far, off[j]);
+  }
+  if (far > NEAR_MIDDLE) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+      if (off[j] > NEAR_MIDDLE) r[j] = (float)rint(127.0 * (double)(to_float(a.v[j]) * lift) / (double)top) + TO_INTEGER;
+  }
+  uint32_t b[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) b[j] = __float_as_uint(r[j]);    // the low byte is the code
+  return make_uint2(__byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410),
+                    __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410));
+}
+
+struct RowsParams {
+  const void* x;
+  int64_t ldx, T;
+  const int32_t* rows_end;   // optional: rows from *rows_end on are left alone
+  const int32_t* place;      // optional, (T, top_k): the codes of token t go to the rows place[t, :], but for those that are -1
+  int top_k;
+  int K;
+  int8_t* codes;
+  int64_t ldc;
+  float* scale;
+};
+
+// G threads per row, CH * 8 values a thread at a time; a row of up to G * CH * 8 values stays in registers between the search for its
+// largest and the rounding, a longer one is read twice (the second time from the L2).
+template <int DT, int G, int CH, bool VEC>
+__global__ void __launch_bounds__(256) quantize_rows_kernel(const RowsParams p) {
   using S = typename StorageOf<DT>::type;
-  __shared__ float part[8];
-  const int64_t t = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
+  __shared__ uint32_t part[2][8];
+  chain_wait();
+  chain_release();
   const int lane = threadIdx.x % G;
-  const int64_t end = rows_end ? min(T, (int64_t)*rows_end) : T;
-  if (G == 256 ? t >= end : false) return;
-  const bool in = t < end;
-  const S* row = static_cast<const S*>(x) + (in ? t : 0) * ldx;
-  float top = 0.0f;
-  bool broken = false;
-  if (in) {
-    for (int k = lane * 8; k < K; k += G * 8) {
-      float v[8];
-      if (VEC) {
-        const Eight<S> a = *reinterpret_cast<const Eight<S>*>(row + k);
+  const int64_t end = p.rows_end ? min(p.T, (int64_t)__ldcg(p.rows_end)) : p.T;
+  const int64_t stride = (int64_t)gridDim.x * (256 / G);
+  int turn = 0;
+  for (int64_t t = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G; t < end; t += stride) {
+    if (p.place) {
+      bool wanted = false;
+      for (int s = 0; s < p.top_k; ++s) wanted |= p.place[t * p.top_k + s] >= 0;
+      if (!wanted) continue;     // the same in all threads of the row
+    }
+    const S* row = static_cast<const S*>(p.x) + t * p.ldx;
+    Eight<S> raw[CH];
+    auto load = [&](int k0) {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = to_float(a.v[j]);
-      } else {
+      for (int c = 0; c < CH; ++c) {
+        const int k = k0 + (c * G + lane) * 8;
+        if (VEC) {
+          if (k < p.K) raw[c] = *reinterpret_cast<const Eight<S>*>(row + k);
+          else raw[c] = Eight<S>{};
+        } else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = k + j < K ? to_float(row[k + j]) : 0.0f;
+          for (int j = 0; j < 8; ++j) raw[c].v[j] = k + j < p.K ? row[k + j] : from_float<S>(0.0f);
+        }
       }
+    };
+    uint32_t bits = 0;
+    for (int k0 = 0; k0 < p.K; k0 += G * CH * 8) {
+      load(k0);
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        broken |= !(fabsf(v[j]) < CUDART_INF_F);
-        top = fmaxf(top, fabsf(v[j]));
+      for (int c = 0; c < CH; ++c) bits = max(bits, largest_bits(raw[c]));
+    }
+    bits = __reduce_max_sync(0xffffffffu, bits);
+    if (G == 256) {
+      if ((threadIdx.x & 31) == 0) part[turn][threadIdx.x >> 5] = bits;
+      __syncthreads();
+#pragma unroll
+      for (int w = 0; w < 8; ++w) bits = max(bits, part[turn][w]);
+      turn ^= 1;
+    }
+    const bool whole = bits < 0x7F800000u;
+    float top = __uint_as_float(bits);
+    const float scale = whole ? top / 127.0f : CUDART_NAN_F;
+    // tiny rows are lifted (exactly) so that 127 / top stays finite
+    const float lift = top < 0x1p-100f ? 0x1p60f : 1.0f;
+    const bool some = whole && top > 0.0f;
+    top *= lift;
+    const float inv = some ? 127.0f / top : 0.0f;
+    for (int k0 = 0; k0 < p.K; k0 += G * CH * 8) {
+      if (p.K > G * CH * 8) load(k0);
+#pragma unroll
+      for (int c = 0; c < CH; ++c) {
+        const int k = k0 + (c * G + lane) * 8;
+        if (k >= p.K) continue;
+        const uint2 word = some ? codes_of(raw[c], top, inv, lift) : make_uint2(0, 0);
+        auto store = [&](int64_t to) {
+          int8_t* out = p.codes + to * p.ldc + k;
+          if (VEC) *reinterpret_cast<uint2*>(out) = word;
+          else
+            for (int j = 0; j < 8 && k + j < p.K; ++j) out[j] = (int8_t)((j < 4 ? word.x : word.y) >> (8 * (j & 3)));
+        };
+        if (p.place) {
+          for (int s = 0; s < p.top_k; ++s) {
+            const int to = p.place[t * p.top_k + s];
+            if (to >= 0) store(to);
+          }
+        } else {
+          store(t);
+        }
       }
     }
-  }
-  if (broken) top = CUDART_INF_F;
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  if (G == 256) {
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = top;
-    __syncthreads();
-#pragma unroll
-    for (int w = 0; w < 8; ++w) top = fmaxf(top, part[w]);
-  }
-  if (!in) return;
-  if (lane == 0) scale[t] = top < CUDART_INF_F ? top / 127.0f : CUDART_NAN_F;
-  // tiny rows are lifted (exactly) so that 127 / top stays finite
-  const float lift = top < 0x1p-100f ? 0x1p60f : 1.0f;
-  const bool plain = top > 0.0f && top < CUDART_INF_F;
-  top *= lift;
-  const float inv = plain ? 127.0f / top : 0.0f;
-  int8_t* out = codes + t * ldc;
-  for (int k = lane * 8; k < K; k += G * 8) {
-    EightCodes c;
-    if (VEC) {
-      const Eight<S> a = *reinterpret_cast<const Eight<S>*>(row + k);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) c.v[j] = plain ? (int8_t)code_of(to_float(a.v[j]) * lift, top, inv) : (int8_t)0;
-      *reinterpret_cast<EightCodes*>(out + k) = c;
-    } else {
-      for (int j = 0; j < 8 && k + j < K; ++j) out[k + j] = plain ? (int8_t)code_of(to_float(row[k + j]) * lift, top, inv) : (int8_t)0;
+    if (p.place) {
+      if (lane < p.top_k) {
+        const int to = p.place[t * p.top_k + lane];
+        if (to >= 0) p.scale[to] = scale;
+      }
+    } else if (lane == 0) {
+      p.scale[t] = scale;
     }
   }
 }
 
-int quantize_rows(const void* x, int dtype, int64_t T, const int32_t* rows_end, int64_t K, int64_t ldx, int8_t* codes, int64_t ldc, float* scale,
-                  cudaStream_t st) {
-  if (T == 0) return MQ_OK;
-  const size_t size = dtype_size(dtype);
-  const bool vec = K % 8 == 0 && aligned(x, 8 * size) && ldx % 8 == 0 && aligned(codes, 8) && ldc % 8 == 0;
-  const bool warp_rows = K <= 1024;
-  const int64_t blocks = warp_rows ? ceil_div(T, 8) : T;
-  MQ_REQUIRE(blocks < (1ll << 31), MQ_ERR_UNSUPPORTED, "too many rows to quantize (%lld)", (long long)T);
-#define MQ_ROWS(DT, G, V) quantize_rows_kernel<DT, G, V><<<(unsigned)blocks, 256, 0, st>>>(x, ldx, T, rows_end, (int)K, codes, ldc, scale)
-#define MQ_ROWS_OF(DT)                                   \
-  do {                                                   \
-    if (warp_rows) { if (vec) MQ_ROWS(DT, 32, true); else MQ_ROWS(DT, 32, false); } \
-    else { if (vec) MQ_ROWS(DT, 256, true); else MQ_ROWS(DT, 256, false); }         \
-  } while (0)
-  if (dtype == MQ_F32) MQ_ROWS_OF(MQ_F32);
-  else if (dtype == MQ_BF16) MQ_ROWS_OF(MQ_BF16);
-  else MQ_ROWS_OF(MQ_F16);
-#undef MQ_ROWS_OF
+template <int DT>
+int launch_rows(const RowsParams& p, bool vec, cudaStream_t st) {
+  const int64_t blocks = p.K <= 1024 ? ceil_div(p.T, 8) : p.T;
+  const unsigned grid = (unsigned)(blocks < 148 * 16 ? blocks : 148 * 16);
+#define MQ_ROWS(G, CH) MQ_CUDA(launch_chained(true, vec ? quantize_rows_kernel<DT, G, CH, true> : quantize_rows_kernel<DT, G, CH, false>, dim3(grid), dim3(256), 0, st, p))
+  if (p.K <= 256) MQ_ROWS(32, 1);
+  else if (p.K <= 512) MQ_ROWS(32, 2);
+  else if (p.K <= 1024) MQ_ROWS(32, 4);
+  else if (p.K <= 2048) MQ_ROWS(256, 1);
+  else if (p.K <= 4096) MQ_ROWS(256, 2);
+  else MQ_ROWS(256, 4);
 #undef MQ_ROWS
   MQ_LAUNCH_CHECK();
   return MQ_OK;
+}
+
+int quantize_rows(int dtype, RowsParams p, cudaStream_t st) {
+  if (p.T == 0) return MQ_OK;
+  const bool vec = p.K % 8 == 0 && aligned(p.x, 8 * dtype_size(dtype)) && p.ldx % 8 == 0 && aligned(p.codes, 8) && p.ldc % 8 == 0;
+  if (dtype == MQ_F32) return launch_rows<MQ_F32>(p, vec, st);
+  if (dtype == MQ_BF16) return launch_rows<MQ_BF16>(p, vec, st);
+  return launch_rows<MQ_F16>(p, vec, st);
 }
 
 // ---------------------------------------------------------------- products
@@ -122,19 +198,70 @@ int int8_product(const Int8Product& p, const Int8Out& o, cudaStream_t st) {
   return int8_product_umma(p, o, st);
 }
 
-// y[t] = sum over the token's pairs, in the order of its slots, of weight * (the pair's down product)
-template <int DT>
-__global__ void __launch_bounds__(256) combine_kernel(const float* __restrict__ pairs, int64_t ldp, const int32_t* __restrict__ place,
-                                                      const float* __restrict__ weights, int k, int N, void* __restrict__ y, int64_t ldy) {
-  const int64_t t = blockIdx.x;
-  auto* out = static_cast<typename StorageOf<DT>::type*>(y) + t * ldy;
-  for (int n = threadIdx.x; n < N; n += 256) {
-    float sum = 0.0f;
-    for (int s = 0; s < k; ++s) {
-      const int at = place[t * k + s];
-      if (at >= 0) sum = fmaf(weights[t * k + s], pairs[(int64_t)at * ldp + n], sum);
+// y[t] = sum over the token's pairs, in the order of its slots, of weight * (the pair's down product).  The products are fp16, short of the
+// factor h_scale[pair] * power[expert, column / 32] (see INT8_PAIRS).  One block per token, eight columns a thread.
+struct CombineParams {
+  const __half* pairs;
+  int64_t ldp;
+  const float *power, *h_scale, *weights;
+  const int32_t *place, *ids;
+  int first, top_k, N, powers;   // powers per expert
+  int64_t T;
+  void* y;
+  int64_t ldy;
+};
+
+template <int DT, bool VEC>
+__global__ void __launch_bounds__(256) combine_kernel(const CombineParams p) {
+  using S = typename StorageOf<DT>::type;
+  __shared__ int row_of[2][32], power_of[2][32];
+  __shared__ float factor_of[2][32];
+  __shared__ int found[2];
+  chain_wait();
+  chain_release();
+  int turn = 0;
+  for (int64_t t = blockIdx.x; t < p.T; t += gridDim.x, turn ^= 1) {
+    if (threadIdx.x < 32) {
+      const int s = threadIdx.x;
+      const int at = s < p.top_k ? __ldcg(p.place + t * p.top_k + s) : -1;
+      const unsigned have = __ballot_sync(0xffffffffu, at >= 0);
+      if (at >= 0) {
+        const int i = __popc(have & ((1u << s) - 1u));
+        row_of[turn][i] = at;
+        power_of[turn][i] = (__ldcg(p.ids + t * p.top_k + s) - p.first) * p.powers;
+        factor_of[turn][i] = __ldcg(p.weights + t * p.top_k + s) * __ldcg(p.h_scale + at);
+      }
+      if (s == 0) found[turn] = __popc(have);
     }
-    out[n] = from_float<typename StorageOf<DT>::type>(sum);
+    __syncthreads();
+    const int n_pairs = found[turn];
+    for (int n = threadIdx.x * 8; n < p.N; n += 256 * 8) {
+      float sum[8] = {};
+      for (int i = 0; i < n_pairs; ++i) {
+        const __half* src = p.pairs + (int64_t)row_of[turn][i] * p.ldp + n;
+        const float f = factor_of[turn][i] * __ldcg(p.power + power_of[turn][i] + (n >> 5));
+        if (VEC) {
+          const Eight<__half> a = *reinterpret_cast<const Eight<__half>*>(src);
+#pragma unroll
+          for (int j = 0; j < 8; ++j) sum[j] = fmaf(f, __half2float(a.v[j]), sum[j]);
+        } else {
+#pragma unroll
+          for (int j = 0; j < 8; ++j)
+            if (n + j < p.N) sum[j] = fmaf(f, __half2float(src[j]), sum[j]);
+        }
+      }
+      S* out = static_cast<S*>(p.y) + t * p.ldy + n;
+      if (VEC) {
+        Eight<S> o;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) o.v[j] = from_float<S>(sum[j]);
+        *reinterpret_cast<Eight<S>*>(out) = o;
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+          if (n + j < p.N) out[j] = from_float<S>(sum[j]);
+      }
+    }
   }
 }
 
@@ -154,7 +281,7 @@ extern "C" int mq_quantize_tokens(const void* x, int dtype, int64_t T, int64_t K
              "mq_quantize_tokens: bad sizes T=%lld K=%lld ldx=%lld ldc=%lld", (long long)T, (long long)K, (long long)ldx, (long long)ldc);
   if (T == 0) return MQ_OK;
   MQ_REQUIRE(x && codes && scale, MQ_ERR_ARGUMENT, "mq_quantize_tokens: null pointer");
-  return quantize_rows(x, dtype, T, nullptr, K, ldx, codes, ldc, scale, static_cast<cudaStream_t>(stream));
+  return quantize_rows(dtype, RowsParams{x, ldx, T, nullptr, nullptr, 0, (int)K, codes, ldc, scale}, static_cast<cudaStream_t>(stream));
 }
 
 extern "C" size_t mq_int8_matmul_workspace_bytes(int x_dtype, int64_t T, int64_t N, int64_t K) {
@@ -191,15 +318,15 @@ extern "C" int mq_int8_matmul(const void* x, int x_dtype, const float* x_scale, 
     Workspace ws(workspace, workspace_bytes);
     int8_t* codes = ws.take<int8_t>((size_t)T * pitch_of(K));
     float* scale = ws.take<float>((size_t)T);
-    MQ_TRY(quantize_rows(x, x_dtype, T, nullptr, K, ldx, codes, pitch_of(K), scale, st));
+    MQ_TRY(quantize_rows(x_dtype, RowsParams{x, ldx, T, nullptr, nullptr, 0, (int)K, codes, pitch_of(K), scale}, st));
     p.x = codes;
     p.ldx = pitch_of(K);
     p.x_scale = scale;
   }
   p.x_rows = T;
   p.w = w; p.ldw = ldw; p.w_expert = 0; p.w_scale = w_scale;
-  p.E = 1; p.rows = (int)N; p.K = (int)K; p.T = T; p.top_k = 1;
-  return int8_product(p, Int8Out{INT8_Y, out_dtype, y, ldy, bias}, st);
+  p.E = 1; p.rows = (int)N; p.K = (int)K; p.T = T;
+  return int8_product(p, Int8Out{INT8_Y, out_dtype, y, ldy, bias, nullptr}, st);
 }
 
 namespace mq {
@@ -208,30 +335,44 @@ struct ExpertsBuffers {
   int32_t *offsets, *order, *place;
   void* plan;
   int8_t *x_codes, *h_codes;
-  float *x_scale, *h_scale, *h, *pairs;
+  float *x_scale, *h_scale, *h, *power;
+  __half* pairs;
 };
-// carves the buffers out of ws, or adds up their bytes where it has no base
+// Carves the buffers out of ws, or adds up their bytes where there is none.  The products of the pairs take the place of the tokens'
+// codes and of the gated values, which have been read by then.
 size_t experts_buffers(int64_t T, int k, int E, int64_t K, int64_t I, Workspace* ws, ExpertsBuffers* b) {
   const size_t P = (size_t)T * k;
   size_t total = 0;
-  auto take = [&](size_t bytes) -> void* {
+  auto take = [&](size_t bytes) -> char* {
     bytes = align_up(bytes, 256);
     total += bytes;
     return ws ? ws->take<char>(bytes) : nullptr;
   };
   ExpertsBuffers x;
-  x.offsets = static_cast<int32_t*>(take((size_t)(E + 1) * 4));
-  x.order = static_cast<int32_t*>(take(P * 4));
-  x.place = static_cast<int32_t*>(take(P * 4));
+  x.offsets = reinterpret_cast<int32_t*>(take((size_t)(E + 1) * 4));
+  x.order = reinterpret_cast<int32_t*>(take(P * 4));
+  x.place = reinterpret_cast<int32_t*>(take(P * 4));
   x.plan = take(mq_expert_plan_workspace_bytes((int64_t)P, E));
-  x.x_codes = static_cast<int8_t*>(take((size_t)T * pitch_of(K)));
-  x.x_scale = static_cast<float*>(take((size_t)T * 4));
-  x.h = static_cast<float*>(take(P * (size_t)I * 4));
-  x.h_codes = static_cast<int8_t*>(take(P * (size_t)pitch_of(I)));
-  x.h_scale = static_cast<float*>(take(P * 4));
-  x.pairs = static_cast<float*>(take(P * (size_t)K * 4));
+  x.x_scale = reinterpret_cast<float*>(take(P * 4));
+  x.h_scale = reinterpret_cast<float*>(take(P * 4));
+  x.power = reinterpret_cast<float*>(take((size_t)E * ceil_div(K, 32) * 4));
+  x.h_codes = reinterpret_cast<int8_t*>(take(P * (size_t)pitch_of(I)));
+  const size_t codes = align_up(P * (size_t)pitch_of(K), 256), h = align_up(P * (size_t)pitch_of(I) * 4, 256), pairs = align_up(P * (size_t)pitch_of(K) * 2, 256);
+  char* shared = take(codes + h > pairs ? codes + h : pairs);
+  x.x_codes = reinterpret_cast<int8_t*>(shared);
+  x.h = reinterpret_cast<float*>(shared + codes);
+  x.pairs = reinterpret_cast<__half*>(shared);
   if (b) *b = x;
   return total;
+}
+
+template <int DT>
+int launch_combine(const CombineParams& p, cudaStream_t st) {
+  const bool vec = p.N % 8 == 0 && p.ldy % 8 == 0 && aligned(p.y, 16);
+  const unsigned grid = (unsigned)(p.T < 148 * 16 ? p.T : 148 * 16);
+  MQ_CUDA(launch_chained(true, vec ? combine_kernel<DT, true> : combine_kernel<DT, false>, dim3(grid), dim3(256), 0, st, p));
+  MQ_LAUNCH_CHECK();
+  return MQ_OK;
 }
 }  // namespace
 }  // namespace mq
@@ -265,19 +406,18 @@ extern "C" int mq_int8_experts(const void* x, int dtype, int64_t T, int64_t K, i
   experts_buffers(T, top_k, (int)E, K, I, &ws, &b);
   const int64_t P = T * top_k;
   MQ_TRY(expert_plan(ids, P, (int)E, (int)first, b.offsets, b.order, b.place, b.plan, st));
-  MQ_TRY(quantize_rows(x, dtype, T, nullptr, K, ldx, b.x_codes, pitch_of(K), b.x_scale, st));
+  // the tokens' codes, once for each of their pairs, where the plan has them
+  MQ_TRY(quantize_rows(dtype, RowsParams{x, ldx, T, nullptr, b.place, top_k, (int)K, b.x_codes, pitch_of(K), b.x_scale}, st));
   Int8Product p = {};
-  p.x = b.x_codes; p.ldx = pitch_of(K); p.x_rows = T; p.x_scale = b.x_scale;
+  p.x = b.x_codes; p.ldx = pitch_of(K); p.x_rows = P; p.x_scale = b.x_scale;
   p.w = gate_up; p.ldw = ld_gate_up; p.w_expert = gate_up_expert; p.w_scale = gate_up_scale;
-  p.E = (int)E; p.rows = (int)I; p.K = (int)K; p.T = P; p.offsets = b.offsets; p.order = b.order; p.top_k = top_k;
-  MQ_TRY(int8_product(p, Int8Out{INT8_GATED, MQ_F32, b.h, I, nullptr}, st));
-  MQ_TRY(quantize_rows(b.h, MQ_F32, P, b.offsets + E, I, I, b.h_codes, pitch_of(I), b.h_scale, st));
-  p.x = b.h_codes; p.ldx = pitch_of(I); p.x_rows = P; p.x_scale = b.h_scale;
+  p.E = (int)E; p.rows = (int)I; p.K = (int)K; p.T = P; p.offsets = b.offsets;
+  MQ_TRY(int8_product(p, Int8Out{INT8_GATED, MQ_F32, b.h, pitch_of(I), nullptr, nullptr}, st));
+  MQ_TRY(quantize_rows(MQ_F32, RowsParams{b.h, pitch_of(I), P, b.offsets + E, nullptr, 0, (int)I, b.h_codes, pitch_of(I), b.h_scale}, st));
+  p.x = b.h_codes; p.ldx = pitch_of(I); p.x_scale = b.h_scale;
   p.w = down; p.ldw = ld_down; p.w_expert = down_expert; p.w_scale = down_scale;
-  p.rows = (int)K; p.K = (int)I; p.order = nullptr;
-  MQ_TRY(int8_product(p, Int8Out{INT8_PAIRS, MQ_F32, b.pairs, K, nullptr}, st));
-  if (dtype == MQ_BF16) combine_kernel<MQ_BF16><<<(unsigned)T, 256, 0, st>>>(b.pairs, K, b.place, weights, top_k, (int)K, y, ldy);
-  else combine_kernel<MQ_F16><<<(unsigned)T, 256, 0, st>>>(b.pairs, K, b.place, weights, top_k, (int)K, y, ldy);
-  MQ_LAUNCH_CHECK();
-  return MQ_OK;
+  p.rows = (int)K; p.K = (int)I;
+  MQ_TRY(int8_product(p, Int8Out{INT8_PAIRS, MQ_F16, b.pairs, pitch_of(K), nullptr, b.power}, st));
+  const CombineParams c = {b.pairs, pitch_of(K), b.power, b.h_scale, weights, b.place, ids, (int)first, top_k, (int)K, (int)ceil_div(K, 32), T, y, ldy};
+  return dtype == MQ_BF16 ? launch_combine<MQ_BF16>(c, st) : launch_combine<MQ_F16>(c, st);
 }

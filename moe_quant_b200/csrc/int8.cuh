@@ -6,10 +6,9 @@
 namespace mq {
 
 // One product of tokens with weights, both 8-bit codes, or one per expert.
-//   dense   : E == 1, offsets == nullptr, rows of x are tokens 0 .. T - 1
-//   experts : rows offsets[e] .. offsets[e + 1] - 1 belong to expert e; row i of x is row i itself, or, where `order` is given,
-//             token order[i] / top_k
-// Weights are (E, rows, K) with strides w_expert and ldw (bytes), scales (E, rows).
+//   dense   : E == 1, offsets == nullptr, rows 0 .. T - 1 of x
+//   experts : rows offsets[e] .. offsets[e + 1] - 1 of x belong to expert e
+// Weights are (E, rows, K) with strides w_expert and ldw (bytes), scales (E, rows); for INT8_GATED (E, 2 rows, K) and (E, 2 rows).
 struct Int8Product {
   const int8_t* x;
   int64_t ldx;
@@ -21,15 +20,18 @@ struct Int8Product {
   int E, rows, K;
   int64_t T;               // rows of the result: tokens, or at most this many pairs
   const int32_t* offsets;
-  const int32_t* order;
-  int top_k;
 };
 
 // where the sums go
 enum Int8Result {
   INT8_Y = 0,      // y = sum * x_scale * w_scale + bias, in the result's type
   INT8_GATED = 1,  // weights are gate rows and up rows, `rows` of either: h = silu(gate) * up, fp32
-  INT8_PAIRS = 2,  // sum * x_scale * w_scale of each pair, fp32
+  // The products of the pairs, short of x_scale and of a power of two per 32 columns, in fp16: sum * w_scale / power[e, n / 32] with
+  // power = 2^k p, p the power of two above the 32 scales and 2^k the one that brings any sum (at most 127 * 128 * K) to 2^15.  It cannot
+  // overflow, and keeps 11 bits down to a sum of 1 (for K up to 32768) times a scale of the column's neighbours; what is smaller
+  // is off by 2^-25 of the power.  Half the bytes of fp32; the sum over a token's pairs and the result's own rounding
+  // (2^-8, 2^-11) come after it.
+  INT8_PAIRS = 2,
 };
 
 struct Int8Out {
@@ -37,6 +39,7 @@ struct Int8Out {
   void* y;
   int64_t ldy;
   const float* bias;
+  float* power;    // INT8_PAIRS: (E, ceil(rows / 32)), written by the product
 };
 
 int int8_product_umma(const Int8Product& p, const Int8Out& o, cudaStream_t st);   // on the tensor cores (int8_umma.cu)

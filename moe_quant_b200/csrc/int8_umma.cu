@@ -4,8 +4,7 @@
 // The weights are the operand of 128 rows per CTA, the tokens the one of up to 256 columns, so a tile can be as narrow as the tokens
 // that there are (32 and up in steps of 32) while weights fill the tensor core.  Two CTAs of a cluster share a tile of 256 weight
 // rows (cta_group::2): each keeps 128 of them and half of the tokens, 32 KB per 128 of k instead of 48.
-//   warp 0 of either CTA : TMA, six stages of 32 KB; weights by tiles, tokens by tiles or, where the pairs' order says which
-//                          token comes where, four rows at a time (gather4); the bytes of both CTAs count on the leader's barrier
+//   warp 0 of either CTA : TMA, six stages of 32 KB; the bytes of both CTAs count on the leader's barrier
 //   warp 1 of the leader : tcgen05.mma for both SMs, two accumulators of 256 columns by turns
 //   warps 4 .. 11        : epilogue, a quarter of the CTA's weight rows each, chunks of 32 tokens by turns
 // Persistent: a pair of CTAs takes every 74th tile.  Eight tiles of weight rows at a time go with all tiles of tokens, so that the
@@ -27,6 +26,7 @@ struct PairArgs {
   Int8Product p;
   Int8Out o;
   int max_width, m_tiles;
+  int sum_shift;   // INT8_PAIRS: 2^sum_shift brings the largest sum down to 2^15
   int packed;      // two neighbouring results of a token are stored together
   int* fault;
 };
@@ -41,12 +41,6 @@ __device__ __forceinline__ void load_tokens_pair(uint32_t dst, const CUtensorMap
   asm volatile(
       "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
       ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(k), "r"(row)
-      : "memory");
-}
-__device__ __forceinline__ void gather_tokens_pair(uint32_t dst, const CUtensorMap* map, uint32_t bar, int k, int4 rows) {
-  asm volatile(
-      "cp.async.bulk.tensor.2d.shared::cluster.global.tile::gather4.mbarrier::complete_tx::bytes.cta_group::2 [%0], [%1, {%3, %4, %5, %6, %7}], [%2];"
-      ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(k), "r"(rows.x), "r"(rows.y), "r"(rows.z), "r"(rows.w)
       : "memory");
 }
 __device__ __forceinline__ void umma_i8_pair(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t accumulate) {
@@ -170,14 +164,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
     for (int64_t unit = pair; ok && u.seek(unit, a, offsets, tiles_before); unit += n_pairs) {
       const int half = u.width >> 1;
       const int b_row = u.t0 + rank * half;
-      int4 rows = make_int4(0, 0, 0, 0);
-      if (p.order) {   // rows behind the last token repeat it; nothing is stored of them
-        const int t = b_row + 4 * lane, last = u.t_end - 1;
-        rows = make_int4(__ldcg(p.order + min(t, last)) / p.top_k, __ldcg(p.order + min(t + 1, last)) / p.top_k,
-                         __ldcg(p.order + min(t + 2, last)) / p.top_k, __ldcg(p.order + min(t + 3, last)) / p.top_k);
-      }
       const int n_boxes = (half + 31) / 32;
-      const uint32_t bytes = 2 * (I8_TILE_BYTES + (uint32_t)(p.order ? half : n_boxes * 32) * I8_K);
+      const uint32_t bytes = 2 * (I8_TILE_BYTES + (uint32_t)n_boxes * 32 * I8_K);
       for (int s = 0; s < slabs; ++s, ++it) {
         const int st = it % I8_STAGES;
         if (it >= I8_STAGES && !mbar_wait(empty0 + 8 * st, ((it / I8_STAGES) - 1) & 1, a.fault, 91)) { ok = false; break; }
@@ -192,11 +180,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
           } else {
             load_weights_pair(dst, &map_w, bar, s * I8_K, u.m * TILE_ROWS + rank * 128, 0, u.e);
           }
-          if (!p.order)
-            for (int j = 0; j < n_boxes; ++j) load_tokens_pair(dst + I8_TILE_BYTES + j * 32 * I8_K, &map_x, bar, s * I8_K, b_row + 32 * j);
+          for (int j = 0; j < n_boxes; ++j) load_tokens_pair(dst + I8_TILE_BYTES + j * 32 * I8_K, &map_x, bar, s * I8_K, b_row + 32 * j);
         }
-        __syncwarp();
-        if (p.order && 4 * lane < half) gather_tokens_pair(dst + I8_TILE_BYTES + 4 * lane * I8_K, &map_x, bar, s * I8_K, rows);
         __syncwarp();
       }
     }
@@ -254,7 +239,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
       const int col = KIND == INT8_GATED ? u.m * TILE_ROWS + rank * 64 + q * 16 + (lane & 15) : u.m * TILE_ROWS + rank * 128 + q * 32 + lane;
       const bool col_in = col < p.rows;
       const int w_row = KIND == INT8_GATED ? (lane >> 4) * p.rows + col : col;
-      const float ws = col_in ? __ldg(p.w_scale + (int64_t)u.e * SETS * p.rows + w_row) : 0.0f;
+      float ws = col_in ? __ldg(p.w_scale + (int64_t)u.e * SETS * p.rows + w_row) : 0.0f;
+      if constexpr (KIND == INT8_PAIRS) {
+        const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(ws) & 0x7FFFFFFFu);
+        // the power of two above the 32 scales; nothing to take out of zeros, and nothing that helps infinities and NaN
+        const int e2 = most == 0u || most >= 0x7F800000u ? 127 : min((int)(most >> 23) + 1, 253);
+        const float power = __uint_as_float((uint32_t)max(e2, 1) << 23);
+        ws = ws / power * __uint_as_float((uint32_t)(127 - a.sum_shift) << 23);
+        // (all tiles of the expert's tokens write the same)
+        if (lane == 0 && col_in) a.o.power[(int64_t)u.e * ((p.rows + 31) >> 5) + (col >> 5)] = power * __uint_as_float((uint32_t)(127 + a.sum_shift) << 23);
+      }
       const float bias = KIND == INT8_Y && a.o.bias && col_in ? __ldg(a.o.bias + col) : 0.0f;
       const int chunks = u.width >> 5;
       float xs[4];
@@ -262,7 +256,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
       for (int i = 0; i < 4; ++i) {
         const int t = u.t0 + (2 * i + h) * 32 + lane;
         xs[i] = 0.0f;
-        if (2 * i + h < chunks && t < u.t_end) xs[i] = __ldcg(p.x_scale + (p.order ? __ldcg(p.order + t) / p.top_k : t));
+        if (2 * i + h < chunks && t < u.t_end) xs[i] = KIND == INT8_PAIRS ? 1.0f : __ldcg(p.x_scale + t);
       }
       ok = mbar_wait(acc_full + 8 * b, (n >> 1) & 1, a.fault, 94);
       if (!ok) break;
@@ -281,10 +275,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
 #pragma unroll
         for (int j = 0; j < 32; j += 4) {
           const float4 s4 = *reinterpret_cast<const float4*>(my_scale + j);
-          v[j] = (float)r[j] * s4.x * ws;
-          v[j + 1] = (float)r[j + 1] * s4.y * ws;
-          v[j + 2] = (float)r[j + 2] * s4.z * ws;
-          v[j + 3] = (float)r[j + 3] * s4.w * ws;
+          if (KIND == INT8_PAIRS) {
+#pragma unroll
+            for (int i4 = 0; i4 < 4; ++i4) v[j + i4] = (float)r[j + i4] * ws;
+          } else {
+            v[j] = (float)r[j] * s4.x * ws;
+            v[j + 1] = (float)r[j + 1] * s4.y * ws;
+            v[j + 2] = (float)r[j + 2] * s4.z * ws;
+            v[j + 3] = (float)r[j + 3] * s4.w * ws;
+          }
         }
         if constexpr (KIND == INT8_GATED) {
           // lanes 0 .. 15 hold the gate, 16 .. 31 the up of the same results: the former take the even tokens, the latter the odd
@@ -301,7 +300,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] += bias;
           }
-          if (KIND == INT8_Y && a.packed) {
+          if (a.packed) {
             // neighbouring lanes hold neighbouring results of a token: the even one takes both of the even tokens, the odd one of the odd
             const bool odd = lane & 1;
             const int64_t at = (int64_t)(t + odd) * a.o.ldy + (col & ~1);
@@ -320,7 +319,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
 #pragma unroll
             for (int j = 0; j < 32; ++j) {
               if (col_in && j < left) {
-                if (KIND == INT8_PAIRS || a.o.dtype == MQ_F32) static_cast<float*>(a.o.y)[at + (int64_t)j * a.o.ldy] = v[j];
+                if (a.o.dtype == MQ_F32) static_cast<float*>(a.o.y)[at + (int64_t)j * a.o.ldy] = v[j];
                 else if (a.o.dtype == MQ_BF16) static_cast<__nv_bfloat16*>(a.o.y)[at + (int64_t)j * a.o.ldy] = __float2bfloat16_rn(v[j]);
                 else static_cast<__half*>(a.o.y)[at + (int64_t)j * a.o.ldy] = __float2half_rn(v[j]);
               }
@@ -387,14 +386,15 @@ int int8_product_umma(const Int8Product& p, const Int8Out& o, cudaStream_t st) {
   {
     const cuuint64_t dims[2] = {(cuuint64_t)p.K, (cuuint64_t)p.x_rows};
     const cuuint64_t strides[1] = {(cuuint64_t)p.ldx};
-    const cuuint32_t box[2] = {I8_K, p.order ? 1u : 32u};
+    const cuuint32_t box[2] = {I8_K, 32};
     MQ_TRY(encode(enc, &map_x, 2, p.x, dims, strides, box));
   }
   a.m_tiles = (int)ceil_div(p.rows, 256 / sets);
   a.max_width = I8_MAX_WIDTH;
   const int64_t most = (int64_t)a.m_tiles * (p.offsets ? ceil_div(p.T, a.max_width) + p.E : token_tiles(p.T, a.max_width));
   const int pairs = (int)(most < I8_PAIRS ? most : I8_PAIRS);
-  const size_t size = o.kind != INT8_Y ? 4 : dtype_size(o.dtype);
+  const size_t size = dtype_size(o.dtype);
+  while ((int64_t)p.K > (2ll << a.sum_shift)) ++a.sum_shift;   // 127 * 128 * K / 2^shift < 2^14 K / 2^shift <= 2^15
   a.packed = p.rows % 2 == 0 && o.ldy % 2 == 0 && aligned(o.y, 2 * size);
   if (o.kind == INT8_GATED) return launch<INT8_GATED>(map_w, map_x, a, pairs, st);
   if (o.kind == INT8_PAIRS) return launch<INT8_PAIRS>(map_w, map_x, a, pairs, st);

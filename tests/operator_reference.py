@@ -89,8 +89,9 @@ def experts(x, ids, weights, gate_up, gate_up_scale, down, down_scale, first=0):
     bound: h has a relative error of 4 roundings each for gate and up, the exponential (2 steps, and its argument's 4 roundings times
     |gate|), sum, division and two products: less than (16 + 5 |gate|) 2^-24.  Its code is then off by at most 127 times that relative error (plus as
     much again for the largest value's): where the exact quotient lies nearer to a middle, the code may differ by one, and the
-    result by that times the weights' scales.  The sum of a pair's products is kept to 2^-11 (fp16, scaled by powers of two)
-    or better, with 2^-24 of the bound of all sums at least; the rest are fp32 roundings and the result's own."""
+    result by that times the weights' scales.  The sum of a pair's products may be kept in fp16 scaled by powers of two: to 2^-11, or,
+    below fp16's normal range, to 2^-25 of 2^k p, with 2^k < I the power that brings 127 * 128 * I to 2^15 and p <= 2 max(scales of the
+    32 columns), so to 2^-24 I max(scales); the rest are fp32 roundings and the result's own."""
     T, k = ids.shape
     E, I = gate_up.shape[0], gate_up.shape[1] // 2
     q, s = codes(x.cpu())
@@ -111,7 +112,8 @@ def experts(x, ids, weights, gate_up, gate_up_scale, down, down_scale, first=0):
         w = weights[token, slot, None]
         part = hq @ d.t() * hs[:, None] * ds * w
         flips = near.double() @ d.abs().t() * hs[:, None] * ds.abs() * w.abs()
-        floor = 127 * d.abs().sum(1) * hs[:, None] * ds.abs() * w.abs() * 2.0 ** -24
+        near_scales = torch.nn.functional.pad(ds.abs(), (0, -len(ds) % 32)).view(-1, 32).amax(1).repeat_interleave(32)[: len(ds)]
+        floor = 2.0 ** -24 * I * near_scales * hs[:, None] * w.abs()
         y.index_add_(0, token, part)
         bound.index_add_(0, token, flips + part.abs() * (2.0 ** -11 + (60 + 5 * 60) * 2.0 ** -24) + floor + 1e-40)
     return y, bound + HALF_STEP[x.dtype] * 1.01 * (y.abs() + bound) + SMALLEST[x.dtype]
