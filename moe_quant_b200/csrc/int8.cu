@@ -8,6 +8,7 @@
 #include <math_constants.h>
 
 #include "int8.cuh"
+#include "int8_codes.cuh"
 #include "profile.cuh"
 
 namespace mq {
@@ -18,55 +19,6 @@ int expert_plan(const int32_t* ids, int64_t pairs, int E, int first, int32_t* of
 namespace {
 
 // ---------------------------------------------------------------- codes of tokens
-// code = round_half_even(127 x / top).  x * (127 / top) is formed and rounded to an integer in one fused step, by adding 1.5 * 2^23; the
-// one rounding in front, that of 127 / top, moves it by at most 127 * 2^-24 = 7.6e-6 of a code.  Where the fraction lies that near to a
-// middle the quotient is formed in 64 bits, whose error of 127 * 2^-53 is below the distance of any quotient of two fp32 numbers
-// from a middle that it does not equal (at least 2^-25 / 254).
-constexpr float TO_INTEGER = 12582912.0f;
-constexpr float NEAR_MIDDLE = 0.49999f;
-
-template <typename T>
-struct alignas(8 * sizeof(T)) Eight { T v[8]; };
-
-// the largest |x| as bits, NaN above infinity above all numbers
-__device__ __forceinline__ uint32_t largest_bits(const Eight<float>& a) {
-  uint32_t m = 0;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) m = max(m, __float_as_uint(a.v[j]) & 0x7FFFFFFFu);
-  return m;
-}
-template <typename T, typename T2>
-__device__ __forceinline__ uint32_t largest_bits_16(const Eight<T>& a) {
-  const T2* p = reinterpret_cast<const T2*>(a.v);
-  const T2 m = __hmax2_nan(__hmax2_nan(__habs2(p[0]), __habs2(p[1])), __hmax2_nan(__habs2(p[2]), __habs2(p[3])));
-  return __float_as_uint(to_float(__hmax_nan(m.x, m.y))) & 0x7FFFFFFFu;
-}
-__device__ __forceinline__ uint32_t largest_bits(const Eight<__nv_bfloat16>& a) { return largest_bits_16<__nv_bfloat16, __nv_bfloat162>(a); }
-__device__ __forceinline__ uint32_t largest_bits(const Eight<__half>& a) { return largest_bits_16<__half, __half2>(a); }
-
-// the codes of eight values, four to a word
-template <typename T>
-__device__ __forceinline__ uint2 codes_of(const Eight<T>& a, float top, float inv, float lift) {
-  float r[8], off[8], far = 0.0f;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const float x = to_float(a.v[j]) * lift;
-    r[j] = __fmaf_rn(x, inv, TO_INTEGER);
-    off[j] = fabsf(__fmaf_rn(x, inv, -(r[j] - TO_INTEGER)));
-    far = fmaxf(far, off[j]);
-  }
-  if (far > NEAR_MIDDLE) {
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-      if (off[j] > NEAR_MIDDLE) r[j] = (float)rint(127.0 * (double)(to_float(a.v[j]) * lift) / (double)top) + TO_INTEGER;
-  }
-  uint32_t b[8];
-#pragma unroll
-  for (int j = 0; j < 8; ++j) b[j] = __float_as_uint(r[j]);    // the low byte is the code
-  return make_uint2(__byte_perm(__byte_perm(b[0], b[1], 0x0040), __byte_perm(b[2], b[3], 0x0040), 0x5410),
-                    __byte_perm(__byte_perm(b[4], b[5], 0x0040), __byte_perm(b[6], b[7], 0x0040), 0x5410));
-}
-
 struct RowsParams {
   const void* x;
   int64_t ldx, T;
@@ -80,105 +32,106 @@ struct RowsParams {
 };
 
 // G threads per row, CH * 8 values a thread at a time; a row of up to G * CH * 8 values stays in registers between the search for its
-// largest and the rounding, a longer one is read twice (the second time from the L2).
+// largest and the rounding, and the block's next row is on its way meanwhile; a longer one is read twice (the second time from the L2).
+// Blocks per SM: what a thread holds of a row, as values and as codes, beside what it needs anyway.
+constexpr int rows_blocks(int dt, int ch) { return dt == MQ_F32 ? (ch >= 8 ? 1 : ch >= 4 ? 3 : 4) : (ch >= 8 ? 2 : ch >= 4 ? 4 : 5); }
 template <int DT, int G, int CH, bool VEC>
-__global__ void __launch_bounds__(256) quantize_rows_kernel(const RowsParams p) {
+__global__ void __launch_bounds__(256, rows_blocks(DT, CH)) quantize_rows_kernel(const RowsParams p) {
   using S = typename StorageOf<DT>::type;
   __shared__ uint32_t part[2][8];
   chain_wait();
   chain_release();
-  const int lane = threadIdx.x % G;
+  const int lane = threadIdx.x % G, warp_lane = threadIdx.x & 31;
   const int64_t end = p.rows_end ? min(p.T, (int64_t)__ldcg(p.rows_end)) : p.T;
   const int64_t stride = (int64_t)gridDim.x * (256 / G);
-  int turn = 0;
-  for (int64_t t = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G; t < end; t += stride) {
-    if (p.place) {
-      bool wanted = false;
-      for (int s = 0; s < p.top_k; ++s) wanted |= p.place[t * p.top_k + s] >= 0;
-      if (!wanted) continue;     // the same in all threads of the row
-    }
+  const bool once = p.K <= G * CH * 8;
+  // lane s of a warp: where the token's s-th copy goes
+  auto places = [&](int64_t t) { return p.place ? (t < end && warp_lane < p.top_k ? p.place[t * p.top_k + warp_lane] : -1) : t < end ? 0 : -1; };
+  Eight<S> raw[CH];
+  auto load = [&](int64_t t, int k0) {
     const S* row = static_cast<const S*>(p.x) + t * p.ldx;
-    Eight<S> raw[CH];
-    auto load = [&](int k0) {
 #pragma unroll
-      for (int c = 0; c < CH; ++c) {
-        const int k = k0 + (c * G + lane) * 8;
-        if (VEC) {
-          if (k < p.K) raw[c] = *reinterpret_cast<const Eight<S>*>(row + k);
-          else raw[c] = Eight<S>{};
-        } else {
+    for (int c = 0; c < CH; ++c) raw[c] = eight_of<VEC>(row, k0 + (c * G + lane) * 8, p.K);
+  };
+  int turn = 0;
+  int64_t t = (int64_t)blockIdx.x * (256 / G) + threadIdx.x / G;
+  int to = places(t), to_next = places(t + stride);
+  unsigned copies = __ballot_sync(0xffffffffu, to >= 0);
+  if (copies && once) load(t, 0);
+  for (; t < end; t += stride) {
+    const int to_after = places(t + 2 * stride);
+    const unsigned copies_next = __ballot_sync(0xffffffffu, to_next >= 0);
+    if (copies) {       // the same in all threads of the row
+      uint32_t bits = 0;
+      for (int k0 = 0; k0 < p.K; k0 += G * CH * 8) {
+        if (!once) load(t, k0);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) raw[c].v[j] = k + j < p.K ? row[k + j] : from_float<S>(0.0f);
-        }
+        for (int c = 0; c < CH; ++c) bits = max(bits, largest_bits(raw[c]));
       }
-    };
-    uint32_t bits = 0;
-    for (int k0 = 0; k0 < p.K; k0 += G * CH * 8) {
-      load(k0);
+      bits = __reduce_max_sync(0xffffffffu, bits);
+      if (G > 32) {
+        constexpr int W = G / 32;
+        if (warp_lane == 0) part[turn][threadIdx.x >> 5] = bits;
+        asm volatile("bar.sync %0, %1;" ::"r"((int)threadIdx.x / G + 1), "n"(G) : "memory");   // the row's threads
 #pragma unroll
-      for (int c = 0; c < CH; ++c) bits = max(bits, largest_bits(raw[c]));
-    }
-    bits = __reduce_max_sync(0xffffffffu, bits);
-    if (G == 256) {
-      if ((threadIdx.x & 31) == 0) part[turn][threadIdx.x >> 5] = bits;
-      __syncthreads();
+        for (int w = 0; w < W; ++w) bits = max(bits, part[turn][(int)threadIdx.x / G * W + w]);
+        turn ^= 1;
+      }
+      const RowCodes code(bits);
+      for (int k0 = 0; k0 < p.K; k0 += G * CH * 8) {
+        if (!once) load(t, k0);
+        uint2 word[CH];
 #pragma unroll
-      for (int w = 0; w < 8; ++w) bits = max(bits, part[turn][w]);
-      turn ^= 1;
-    }
-    const bool whole = bits < 0x7F800000u;
-    float top = __uint_as_float(bits);
-    const float scale = whole ? top / 127.0f : CUDART_NAN_F;
-    // tiny rows are lifted (exactly) so that 127 / top stays finite
-    const float lift = top < 0x1p-100f ? 0x1p60f : 1.0f;
-    const bool some = whole && top > 0.0f;
-    top *= lift;
-    const float inv = some ? 127.0f / top : 0.0f;
-    for (int k0 = 0; k0 < p.K; k0 += G * CH * 8) {
-      if (p.K > G * CH * 8) load(k0);
+        for (int c = 0; c < CH; ++c) word[c] = code.of(raw[c]);
+        if (once && copies_next) load(t + stride, 0);
+        for (unsigned left = copies; left; left &= left - 1) {
+          const int64_t row = p.place ? __shfl_sync(0xffffffffu, to, __ffs(left) - 1) : t;
 #pragma unroll
-      for (int c = 0; c < CH; ++c) {
-        const int k = k0 + (c * G + lane) * 8;
-        if (k >= p.K) continue;
-        const uint2 word = some ? codes_of(raw[c], top, inv, lift) : make_uint2(0, 0);
-        auto store = [&](int64_t to) {
-          int8_t* out = p.codes + to * p.ldc + k;
-          if (VEC) *reinterpret_cast<uint2*>(out) = word;
-          else
-            for (int j = 0; j < 8 && k + j < p.K; ++j) out[j] = (int8_t)((j < 4 ? word.x : word.y) >> (8 * (j & 3)));
-        };
-        if (p.place) {
-          for (int s = 0; s < p.top_k; ++s) {
-            const int to = p.place[t * p.top_k + s];
-            if (to >= 0) store(to);
+          for (int c = 0; c < CH; ++c) {
+            const int k = k0 + (c * G + lane) * 8;
+            int8_t* out = p.codes + row * p.ldc + k;
+            if (VEC) {
+              if (k < p.K) *reinterpret_cast<uint2*>(out) = word[c];
+            } else {
+#pragma unroll
+              for (int j = 0; j < 8; ++j)
+                if (k + j < p.K) out[j] = (int8_t)((j < 4 ? word[c].x : word[c].y) >> (8 * (j & 3)));
+            }
           }
-        } else {
-          store(t);
+          if (!p.place) break;
         }
       }
-    }
-    if (p.place) {
-      if (lane < p.top_k) {
-        const int to = p.place[t * p.top_k + lane];
-        if (to >= 0) p.scale[to] = scale;
+      if (lane < 32) {
+        if (p.place) {
+          if (to >= 0) p.scale[to] = code.scale;
+        } else if (lane == 0) {
+          p.scale[t] = code.scale;
+        }
       }
-    } else if (lane == 0) {
-      p.scale[t] = scale;
+    } else if (once && copies_next) {
+      load(t + stride, 0);
     }
+    to = to_next;
+    to_next = to_after;
+    copies = copies_next;
   }
 }
 
 template <int DT>
 int launch_rows(const RowsParams& p, bool vec, cudaStream_t st) {
-  const int64_t blocks = p.K <= 1024 ? ceil_div(p.T, 8) : p.T;
-  const unsigned grid = (unsigned)(blocks < 148 * 16 ? blocks : 148 * 16);
-#define MQ_ROWS(G, CH) MQ_CUDA(launch_chained(true, vec ? quantize_rows_kernel<DT, G, CH, true> : quantize_rows_kernel<DT, G, CH, false>, dim3(grid), dim3(256), 0, st, p))
+#define MQ_ROWS(G, CH)                                                                                                      \
+  do {                                                                                                                      \
+    const int64_t blocks = ceil_div(p.T, 256 / G), most = 148 * rows_blocks(DT, CH);                                        \
+    MQ_CUDA(launch_chained(true, vec ? quantize_rows_kernel<DT, G, CH, true> : quantize_rows_kernel<DT, G, CH, false>,      \
+                           dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, st, p));                          \
+  } while (0)
   if (p.K <= 256) MQ_ROWS(32, 1);
   else if (p.K <= 512) MQ_ROWS(32, 2);
   else if (p.K <= 1024) MQ_ROWS(32, 4);
-  else if (p.K <= 2048) MQ_ROWS(256, 1);
-  else if (p.K <= 4096) MQ_ROWS(256, 2);
-  else MQ_ROWS(256, 4);
+  else if (p.K <= 2048) MQ_ROWS(64, 4);
+  else if (p.K <= 4096) MQ_ROWS(128, 4);
+  else if (p.K <= 8192) MQ_ROWS(256, 4);
+  else MQ_ROWS(256, 8);
 #undef MQ_ROWS
   MQ_LAUNCH_CHECK();
   return MQ_OK;
