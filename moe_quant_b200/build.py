@@ -18,7 +18,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 OUT = os.path.join(HERE, "libmoequant_sm100.so")
 SOURCES = ["api.cu", "pack.cu", "prepare.cu", "gemm_simt.cu", "hinv.cu", "sweep.cu", "sweep_super.cu", "umma_gemm.cu", "profile.cu", "metrics.cu",
-           "route.cu", "int8.cu", "int8_umma.cu"]
+           "route.cu", "int8.cu", "int8_umma.cu", "int8_few.cu"]
 FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "-Xcompiler", "-fPIC", "-Xptxas", "-v",

@@ -34,7 +34,7 @@ struct RowsParams {
 // G threads per row, CH * 8 values a thread at a time; a row of up to G * CH * 8 values stays in registers between the search for its
 // largest and the rounding, and the block's next row is on its way meanwhile; a longer one is read twice (the second time from the L2).
 // Blocks per SM: what a thread holds of a row, as values and as codes, beside what it needs anyway.
-constexpr int rows_blocks(int dt, int ch) { return dt == MQ_F32 ? (ch >= 8 ? 1 : ch >= 4 ? 3 : 4) : (ch >= 8 ? 2 : ch >= 4 ? 4 : 5); }
+constexpr int rows_blocks(int dt, int ch) { return dt == MQ_F32 ? (ch >= 8 ? 1 : ch >= 4 ? 3 : 4) : (ch >= 8 ? 3 : ch >= 4 ? 4 : 5); }
 template <int DT, int G, int CH, bool VEC>
 __global__ void __launch_bounds__(256, rows_blocks(DT, CH)) quantize_rows_kernel(const RowsParams p) {
   using S = typename StorageOf<DT>::type;
@@ -146,11 +146,6 @@ int quantize_rows(int dtype, RowsParams p, cudaStream_t st) {
 }
 
 // ---------------------------------------------------------------- products
-int int8_product(const Int8Product& p, const Int8Out& o, cudaStream_t st) {
-  if (p.T == 0 || p.rows == 0) return MQ_OK;
-  return int8_product_umma(p, o, st);
-}
-
 // y[t] = sum over the token's pairs, in the order of its slots, of weight * (the pair's down product).  The products are fp16, short of the
 // factor h_scale[pair] * power[expert, column / 32] (see INT8_PAIRS).  One block per token, eight columns a thread.
 struct CombineParams {
@@ -239,7 +234,7 @@ extern "C" int mq_quantize_tokens(const void* x, int dtype, int64_t T, int64_t K
 
 extern "C" size_t mq_int8_matmul_workspace_bytes(int x_dtype, int64_t T, int64_t N, int64_t K) {
   (void)N;
-  if (x_dtype == MQ_I8) return 0;
+  if (x_dtype == MQ_I8 || int8_few_fits(T, K)) return 0;
   return align_up((size_t)T * (size_t)pitch_of(K), 256) + align_up((size_t)T * 4, 256);
 }
 
@@ -263,10 +258,15 @@ extern "C" int mq_int8_matmul(const void* x, int x_dtype, const float* x_scale, 
   MQ_REQUIRE(need == 0 || (workspace && aligned(workspace, 16) && workspace_bytes >= need), MQ_ERR_WORKSPACE,
              "mq_int8_matmul: the workspace has %zu bytes and needs %zu", workspace_bytes, need);
   Int8Product p = {};
+  p.x_scale = x_scale;
+  p.w = w; p.ldw = ldw; p.w_expert = 0; p.w_scale = w_scale;
+  p.E = 1; p.rows = (int)N; p.K = (int)K; p.T = T;
+  p.x_rows = T;
+  const Int8Out o = {INT8_Y, out_dtype, y, ldy, bias, nullptr};
+  if (int8_few_fits(T, K)) return int8_few(x, x_dtype, ldx, p, o, st);
   if (x_dtype == MQ_I8) {
     p.x = static_cast<const int8_t*>(x);
     p.ldx = ldx;
-    p.x_scale = x_scale;
   } else {
     Workspace ws(workspace, workspace_bytes);
     int8_t* codes = ws.take<int8_t>((size_t)T * pitch_of(K));
@@ -276,10 +276,7 @@ extern "C" int mq_int8_matmul(const void* x, int x_dtype, const float* x_scale, 
     p.ldx = pitch_of(K);
     p.x_scale = scale;
   }
-  p.x_rows = T;
-  p.w = w; p.ldw = ldw; p.w_expert = 0; p.w_scale = w_scale;
-  p.E = 1; p.rows = (int)N; p.K = (int)K; p.T = T;
-  return int8_product(p, Int8Out{INT8_Y, out_dtype, y, ldy, bias, nullptr}, st);
+  return int8_product_umma(p, o, st);
 }
 
 namespace mq {
@@ -358,19 +355,20 @@ extern "C" int mq_int8_experts(const void* x, int dtype, int64_t T, int64_t K, i
   ExpertsBuffers b;
   experts_buffers(T, top_k, (int)E, K, I, &ws, &b);
   const int64_t P = T * top_k;
+  Int8Product up = {}, dn = {};
+  up.w = gate_up; up.ldw = ld_gate_up; up.w_expert = gate_up_expert; up.w_scale = gate_up_scale;
+  up.E = (int)E; up.rows = (int)I; up.K = (int)K; up.T = P;
+  dn.w = down; dn.ldw = ld_down; dn.w_expert = down_expert; dn.w_scale = down_scale;
+  dn.E = (int)E; dn.rows = (int)K; dn.K = (int)I; dn.T = P;
+  if (T == 1 && int8_one_token_fits(top_k, K, I)) return int8_one_token(x, dtype, ids, weights, top_k, (int)first, up, dn, b.h, y, st);
   MQ_TRY(expert_plan(ids, P, (int)E, (int)first, b.offsets, b.order, b.place, b.plan, st));
   // the tokens' codes, once for each of their pairs, where the plan has them
   MQ_TRY(quantize_rows(dtype, RowsParams{x, ldx, T, nullptr, b.place, top_k, (int)K, b.x_codes, pitch_of(K), b.x_scale}, st));
-  Int8Product p = {};
-  p.x = b.x_codes; p.ldx = pitch_of(K); p.x_rows = P; p.x_scale = b.x_scale;
-  p.w = gate_up; p.ldw = ld_gate_up; p.w_expert = gate_up_expert; p.w_scale = gate_up_scale;
-  p.E = (int)E; p.rows = (int)I; p.K = (int)K; p.T = P; p.offsets = b.offsets;
-  MQ_TRY(int8_product(p, Int8Out{INT8_GATED, MQ_F32, b.h, pitch_of(I), nullptr, nullptr}, st));
+  up.x = b.x_codes; up.ldx = pitch_of(K); up.x_rows = P; up.x_scale = b.x_scale; up.offsets = b.offsets;
+  MQ_TRY(int8_product_umma(up, Int8Out{INT8_GATED, MQ_F32, b.h, pitch_of(I), nullptr, nullptr}, st));
   MQ_TRY(quantize_rows(MQ_F32, RowsParams{b.h, pitch_of(I), P, b.offsets + E, nullptr, 0, (int)I, b.h_codes, pitch_of(I), b.h_scale}, st));
-  p.x = b.h_codes; p.ldx = pitch_of(I); p.x_scale = b.h_scale;
-  p.w = down; p.ldw = ld_down; p.w_expert = down_expert; p.w_scale = down_scale;
-  p.rows = (int)K; p.K = (int)I;
-  MQ_TRY(int8_product(p, Int8Out{INT8_PAIRS, MQ_F16, b.pairs, pitch_of(K), nullptr, b.power}, st));
+  dn.x = b.h_codes; dn.ldx = pitch_of(I); dn.x_rows = P; dn.x_scale = b.h_scale; dn.offsets = b.offsets;
+  MQ_TRY(int8_product_umma(dn, Int8Out{INT8_PAIRS, MQ_F16, b.pairs, pitch_of(K), nullptr, b.power}, st));
   const CombineParams c = {b.pairs, pitch_of(K), b.power, b.h_scale, weights, b.place, ids, (int)first, top_k, (int)K, (int)ceil_div(K, 32), T, y, ldy};
   return dtype == MQ_BF16 ? launch_combine<MQ_BF16>(c, st) : launch_combine<MQ_F16>(c, st);
 }

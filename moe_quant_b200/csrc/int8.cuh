@@ -44,4 +44,13 @@ struct Int8Out {
 
 int int8_product_umma(const Int8Product& p, const Int8Out& o, cudaStream_t st);   // on the tensor cores (int8_umma.cu)
 
+// A few tokens (int8_few.cu): x of any type, codes made on the way (p.x is not read; p.x_scale for MQ_I8 alone).
+constexpr int64_t INT8_FEW_TOKENS = 4;
+bool int8_few_fits(int64_t T, int64_t K);
+int int8_few(const void* x, int dtype, int64_t ldx, const Int8Product& p, const Int8Out& o, cudaStream_t st);
+// The experts of one token, without a plan; h holds top_k rows of up.rows numbers.
+bool int8_one_token_fits(int top_k, int64_t K, int64_t I);
+int int8_one_token(const void* x, int dtype, const int32_t* ids, const float* weights, int top_k, int first, const Int8Product& up,
+                   const Int8Product& down, float* h, void* y, cudaStream_t st);
+
 }  // namespace mq

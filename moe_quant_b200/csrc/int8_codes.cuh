@@ -91,22 +91,23 @@ struct RowCodes {
   }
   template <typename T>
   __device__ __forceinline__ uint2 of(const Eight<T>& a) const {
-    float r[8], off[8];
+    float r[8];
     if constexpr (sizeof(T) == 2) {
       if (careful_from < 0.0f) return careful_codes(a, top, inv, lift);
 #pragma unroll
       for (int j = 0; j < 8; ++j)
         r[j] = __uint_as_float((__float_as_uint(to_float(a.v[j]) * inv) + 8u) & ~15u) + TO_INTEGER;
-      return low_bytes(r);
-    }
+    } else {
+      float off[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float x = to_float(a.v[j]);
-      r[j] = __fmaf_rn(x, inv, TO_INTEGER);
-      off[j] = __fmaf_rn(x, inv, TO_INTEGER - r[j]);
+      for (int j = 0; j < 8; ++j) {
+        const float x = to_float(a.v[j]);
+        r[j] = __fmaf_rn(x, inv, TO_INTEGER);
+        off[j] = __fmaf_rn(x, inv, TO_INTEGER - r[j]);
+      }
+      const float far = max3_abs_nan(max3_abs_nan(off[0], off[1], off[2]), max3_abs_nan(off[3], off[4], off[5]), max3_abs_nan(off[6], off[7], 0.0f));
+      if (!(far <= careful_from)) return careful_codes(a, top, inv, lift);
     }
-    const float far = max3_abs_nan(max3_abs_nan(off[0], off[1], off[2]), max3_abs_nan(off[3], off[4], off[5]), max3_abs_nan(off[6], off[7], 0.0f));
-    if (!(far <= careful_from)) return careful_codes(a, top, inv, lift);
     return low_bytes(r);
   }
 };

@@ -359,7 +359,13 @@ int encode(EncodeTiledFn enc, CUtensorMap* map, int rank, const void* base, cons
 
 template <int KIND>
 int launch(const CUtensorMap& map_w, const CUtensorMap& map_x, const PairArgs& a, int pairs, cudaStream_t st) {
-  MQ_CUDA(cudaFuncSetAttribute(int8_pair_kernel<KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kInt8Smem));
+  static bool ready[64] = {};
+  int dev = 0;
+  MQ_CUDA(cudaGetDevice(&dev));
+  if (dev >= 64 || !ready[dev]) {
+    MQ_CUDA(cudaFuncSetAttribute(int8_pair_kernel<KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kInt8Smem));
+    if (dev < 64) ready[dev] = true;
+  }
   MQ_CUDA(launch_chained(true, int8_pair_kernel<KIND>, dim3((unsigned)(2 * pairs)), dim3(I8_THREADS), kInt8Smem, st, map_w, map_x, a));
   MQ_LAUNCH_CHECK();
   return MQ_OK;

@@ -312,7 +312,8 @@ extern "C" int mq_route_tokens(const void* logits, int dtype, int64_t T, int64_t
 }
 
 extern "C" size_t mq_expert_plan_workspace_bytes(int64_t pairs, int64_t E) {
-  return (size_t)plan_blocks(pairs) * (size_t)E * 4;
+  const int blocks = plan_blocks(pairs);
+  return blocks > 1 ? (size_t)blocks * (size_t)E * 4 : 0;
 }
 
 namespace mq {

@@ -386,6 +386,8 @@ def _forward_only(what: str, *tensors: Optional[Tensor]) -> None:
 
 def _rows(t: Tensor, what: str) -> Tensor:
     """(..., C) as rows of unit column stride, a view where the strides allow it."""
+    if t.dim() == 2 and t.is_contiguous():
+        return t
     if t.dim() < 1:
         raise MoeQuantError(f"{what} must have at least one dimension")
     n = t.numel() // t.shape[-1] if t.shape[-1] else 0
@@ -398,15 +400,28 @@ def _pitch(t: Tensor) -> int:
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
-def _scratch(device: torch.device, nbytes: int) -> Tensor:
-    return torch.empty(max(int(nbytes), 1), dtype=torch.uint8, device=device)
+def _scratch(device: torch.device, nbytes: int) -> Optional[Tensor]:
+    return torch.empty(nbytes, dtype=torch.uint8, device=device) if nbytes else None
+
+
+def _int32(t: Tensor, what: str) -> Tensor:
+    require_cuda(t, what)
+    if t.dtype == torch.int32 and t.is_contiguous():
+        return t
+    if t.dtype not in (torch.int32, torch.int64):
+        raise MoeQuantError(f"{what} must be int32 or int64 (got {t.dtype})")
+    return t.to(torch.int32).contiguous()
+
+
+def _fp32(t: Tensor) -> Tensor:
+    return t if t.dtype == torch.float32 and t.is_contiguous() else t.to(torch.float32).contiguous()
 
 
 def _int8_codes(t: Tensor, dims: int, what: str) -> Tensor:
     require_cuda(t, what)
     if t.dtype != torch.int8 or t.dim() != dims:
         raise MoeQuantError(f"{what} must be a {dims}-D int8 tensor (got {t.dim()}-D {t.dtype})")
-    if t.shape[-1] > 0 and t.stride(-1) != 1:
+    if t.stride(-1) != 1 and t.shape[-1] > 0:
         raise MoeQuantError(f"{what} must have unit column stride")
     return t
 
@@ -421,6 +436,8 @@ def _code_pitch(t: Tensor) -> int:
 
 
 def _scales(t: Tensor, shape: Tuple[int, ...], what: str) -> Tensor:
+    if t.dtype == torch.float32 and t.is_cuda and t.shape == shape and t.is_contiguous():
+        return t
     require_cuda(t, what)
     n = 1
     for s in shape:
@@ -461,7 +478,7 @@ def route_tokens(logits: Tensor, top_k: int, *, score: str = "softmax", bias: Op
         require_one_device("route_tokens", logits, bias)
         if bias.shape != (E,):
             raise MoeQuantError(f"route_tokens: bias of shape {tuple(bias.shape)} for {E} experts")
-        bias = bias.to(torch.float32).contiguous()
+        bias = _fp32(bias)
     rows = _rows(logits, "logits")
     T = rows.shape[0]
     ids = torch.empty(*lead, top_k, dtype=torch.int32, device=logits.device)
@@ -473,25 +490,19 @@ def route_tokens(logits: Tensor, top_k: int, *, score: str = "softmax", bias: Op
     return ids, weights
 
 
-def _expert_ids(ids: Tensor) -> Tensor:
-    require_cuda(ids, "ids")
-    if ids.dtype not in (torch.int32, torch.int64):
-        raise MoeQuantError(f"ids must be int32 or int64 (got {ids.dtype})")
-    return ids.to(torch.int32).contiguous()
-
-
 def expert_plan(ids: Tensor, n_experts: int, first: int = 0) -> ExpertPlan:
     """Groups the pairs of `ids` (..., top_k) by expert, for the experts first .. first + n_experts - 1 (all others, -1 among
     them, are dropped)."""
-    ids = _expert_ids(ids)
+    ids = _int32(ids, "ids")
     dev, P = ids.device, ids.numel()
-    offsets = torch.empty(max(int(n_experts), 0) + 1, dtype=torch.int32, device=dev)
+    offsets = torch.empty(max(n_experts, 0) + 1, dtype=torch.int32, device=dev)
     order = torch.empty(P, dtype=torch.int32, device=dev)
-    place = torch.empty(ids.shape, dtype=torch.int32, device=dev)
+    place = torch.empty_like(ids)
     L = lib()
-    ws = _scratch(dev, L.mq_expert_plan_workspace_bytes(P, max(int(n_experts), 0)))
+    nbytes = L.mq_expert_plan_workspace_bytes(P, max(n_experts, 0))
+    ws = _scratch(dev, nbytes)
     with _lib.on_device(dev):
-        check(L.mq_expert_plan(ptr(ids), P, n_experts, first, ptr(offsets), ptr(order), ptr(place), ptr(ws), ws.numel(), stream_ptr(dev)))
+        check(L.mq_expert_plan(ptr(ids), P, n_experts, first, ptr(offsets), ptr(order), ptr(place), ptr(ws), nbytes, stream_ptr(dev)))
     return ExpertPlan(offsets, order, place)
 
 
@@ -542,10 +553,11 @@ def int8_matmul(x: Tensor, weight: Tensor, weight_scale: Tensor, bias: Optional[
         x_scale = _scales(x_scale, tuple(lead), "x_scale")
     y = torch.empty(*lead, N, dtype=out_dtype, device=dev)
     L = lib()
-    ws = _scratch(dev, L.mq_int8_matmul_workspace_bytes(x_code, T, N, K))
+    nbytes = L.mq_int8_matmul_workspace_bytes(x_code, T, N, K)
+    ws = _scratch(dev, nbytes)
     with _lib.on_device(dev):
         check(L.mq_int8_matmul(ptr(rows), x_code, ptr(x_scale), T, K, _code_pitch(rows) if given else _pitch(rows), ptr(weight), N,
-                               _code_pitch(weight), ptr(weight_scale), ptr(bias), out_code, ptr(y), N, ptr(ws), ws.numel(), stream_ptr(dev)))
+                               _code_pitch(weight), ptr(weight_scale), ptr(bias), out_code, ptr(y), N, ptr(ws), nbytes, stream_ptr(dev)))
     return y
 
 
@@ -568,8 +580,8 @@ def int8_experts(x: Tensor, ids: Tensor, weights: Tensor, gate_up: Tensor, gate_
     if ids.dim() != x.dim() or ids.shape[:-1] != x.shape[:-1] or weights.shape != ids.shape:
         raise MoeQuantError(f"int8_experts: ids {tuple(ids.shape)} and weights {tuple(weights.shape)} do not match x {tuple(x.shape)}")
     require_one_device("int8_experts", x, ids, weights, gate_up, gate_up_scale, down, down_scale)
-    ids = _expert_ids(ids)
-    weights = weights.to(torch.float32).contiguous()
+    ids = _int32(ids, "ids")
+    weights = _fp32(weights)
     gate_up_scale = _scales(gate_up_scale, (E, I2), "gate_up_scale")
     down_scale = _scales(down_scale, (E, K), "down_scale")
     rows = _rows(x, "x")
@@ -577,9 +589,10 @@ def int8_experts(x: Tensor, ids: Tensor, weights: Tensor, gate_up: Tensor, gate_
     dev = x.device
     y = torch.empty(*x.shape[:-1], K, dtype=x.dtype, device=dev)
     L = lib()
-    ws = _scratch(dev, L.mq_int8_experts_workspace_bytes(T, k, E, K, I) if T and k and E else 0)
+    nbytes = L.mq_int8_experts_workspace_bytes(T, k, E, K, I) if T and k and E else 0
+    ws = _scratch(dev, nbytes)
     with _lib.on_device(dev):
         check(L.mq_int8_experts(ptr(rows), dtype_code(x.dtype), T, K, _pitch(rows), ptr(ids), ptr(weights), k, first, E, I, ptr(gate_up),
                                 _code_pitch(gate_up), gate_up.stride(0) if E > 1 else 0, ptr(gate_up_scale), ptr(down), _code_pitch(down),
-                                down.stride(0) if E > 1 else 0, ptr(down_scale), ptr(y), K, ptr(ws), ws.numel(), stream_ptr(dev)))
+                                down.stride(0) if E > 1 else 0, ptr(down_scale), ptr(y), K, ptr(ws), nbytes, stream_ptr(dev)))
     return y
