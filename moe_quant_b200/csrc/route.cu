@@ -5,7 +5,9 @@
 // the scores without bias, normalised over the chosen ones where asked.  An expert whose logit is -inf or NaN, or whose bias is
 // -inf or NaN, is never chosen.  +inf counts as the largest finite number.
 //
-// One warp per token, the token's experts spread over its lanes.
+// One warp per token, a run of experts per lane.  Which experts come first is decided on fp32 scores wherever these lie further apart than
+// they can be off, and in 64 bits in the rows where some do not (without a bias the logits themselves order the experts: exactly).
+// 65536 tokens, 256 experts in 8 groups with a bias: 192 us with every row in 64 bits.
 #include <math_constants.h>
 
 #include "common.cuh"
@@ -24,6 +26,8 @@ struct RouteParams {
   const float* bias;
   int32_t* ids;
   float* weights;
+  bool vec;               // rows of logits can be read 16 bytes at a time
+  int lanes_per_group;    // lanes that hold a group, 0 where lanes and groups do not match
 };
 
 __device__ __forceinline__ float finite_logit(float l) { return l != l ? -CUDART_INF_F : fminf(l, 3.402823466e38f); }
@@ -55,7 +59,8 @@ __device__ __forceinline__ void warp_argmax(double& v, int& i) {
 __device__ int choose(const RouteParams& p, const float* row, double* value, int lane) {
   const bool by_logit = p.bias == nullptr;   // sigmoid and softmax are increasing
   double top = -CUDART_INF, total = 0.0;
-  if (!p.sigmoid && (p.groups > 1 || !by_logit)) {
+  const bool by_score = !by_logit || (p.groups > 1 && p.top2);
+  if (!p.sigmoid && by_score) {
     for (int e = lane; e < p.E; e += 32) top = max(top, (double)row[e]);
     top = warp_max(top);
     for (int e = lane; e < p.E; e += 32)
@@ -66,7 +71,7 @@ __device__ int choose(const RouteParams& p, const float* row, double* value, int
     const double l = row[e];
     double v = -CUDART_INF;
     if (row[e] > -CUDART_INF_F) {
-      if (by_logit && p.groups == 1) v = l;
+      if (!by_score) v = l;
       else v = p.sigmoid ? 1.0 / (1.0 + exp(-l)) : exp(l - top) / total;
       if (!by_logit) v += (double)p.bias[e];
       if (v != v) v = -CUDART_INF;
@@ -120,7 +125,20 @@ __device__ int choose(const RouteParams& p, const float* row, double* value, int
   return mine;
 }
 
-template <int DT>
+// fp32 numbers as unsigned integers of the same order; 0 stands for an expert that cannot be chosen
+__device__ __forceinline__ uint32_t ordered(float v) {
+  const uint32_t b = __float_as_uint(v);
+  return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+__device__ __forceinline__ float from_ordered(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k); }
+
+// Whether a value that came out as `a` may in truth not lie above one that came out as `b` <= a.  Sigmoid: exponential, quotient and sum are
+// off by 4e-7 at most, the bias' sum by 2^-24 |v|; softmax: the sum over up to 1024 experts (32 in a lane, five levels of lanes) and the
+// exponentials by 3.2e-6.  Two values, or two sums of two.
+__device__ __forceinline__ bool too_near(float a, float b, float tolerance) { return !(a - b > tolerance * (1.0f + fmaxf(fabsf(a), fabsf(b)))); }
+
+// VPL experts per lane: VPL lane .. VPL lane + VPL - 1
+template <int DT, int VPL>
 __global__ void __launch_bounds__(ROUTE_WARPS * 32) route_kernel(const void* __restrict__ logits, const RouteParams p) {
   using T = typename StorageOf<DT>::type;
   extern __shared__ double route_smem[];
@@ -128,40 +146,207 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32) route_kernel(const void* __r
   double* value = route_smem + (size_t)warp * p.E;
   float* row = reinterpret_cast<float*>(route_smem + (size_t)ROUTE_WARPS * p.E) + (size_t)warp * p.E;
   const int64_t t = (int64_t)blockIdx.x * ROUTE_WARPS + warp;
+  chain_wait();
+  chain_release();
   if (t >= p.T) return;
   const T* src = static_cast<const T*>(logits) + t * p.ld;
-  for (int e = lane; e < p.E; e += 32) row[e] = finite_logit(to_float(src[e]));
-  __syncwarp();
-  const int mine = choose(p, row, value, lane);
-  // the weights, lane j the j-th: softmax over all experts, or without its common factor where the sum divides it out; sigmoid
-  // times e^-m for m = min(0, largest chosen logit), which cannot underflow as a whole
-  const float l = mine >= 0 ? row[mine] : -CUDART_INF_F;
-  float w;
-  if (p.sigmoid) {
-    const float m = p.renormalise ? fminf(0.0f, warp_max(l)) : 0.0f;
-    w = mine >= 0 ? 1.0f / (expf(m) + expf(m - l)) : 0.0f;
+  const int e0 = lane * VPL;
+  float l[VPL];
+  constexpr int WORD = VPL * sizeof(T) >= 16 ? 16 / sizeof(T) : 1;     // values per load
+  if (WORD > 1 && p.vec) {
+#pragma unroll
+    for (int j = 0; j < VPL; j += WORD) {
+      struct alignas(WORD * sizeof(T)) Word { T v[WORD]; } w;
+      if (e0 + j < p.E) {     // E is a multiple of WORD
+        w = *reinterpret_cast<const Word*>(src + e0 + j);
+#pragma unroll
+        for (int i = 0; i < WORD; ++i) l[j + i] = finite_logit(to_float(w.v[i]));
+      } else {
+#pragma unroll
+        for (int i = 0; i < WORD; ++i) l[j + i] = -CUDART_INF_F;
+      }
+    }
   } else {
-    float top = l;
-    if (!p.renormalise)
-      for (int e = lane; e < p.E; e += 32) top = fmaxf(top, row[e]);
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) l[j] = e0 + j < p.E ? finite_logit(to_float(src[e0 + j])) : -CUDART_INF_F;
+  }
+
+  const bool by_logit = p.bias == nullptr;   // sigmoid and softmax are increasing
+  const bool by_sum = p.groups > 1 && p.top2;
+  const float tolerance = p.sigmoid ? 4e-6f : 2e-5f;
+  // softmax: its largest logit and sum, where scores are needed
+  float top = 0.0f, total = 1.0f;
+  if (!p.sigmoid && (!by_logit || by_sum || !p.renormalise)) {
+    top = l[0];
+#pragma unroll
+    for (int j = 1; j < VPL; ++j) top = fmaxf(top, l[j]);
     top = warp_max(top);
-    w = mine >= 0 ? expf(l - top) : 0.0f;
-    if (!p.renormalise) {
-      float total = 0.0f;
-      for (int e = lane; e < p.E; e += 32)
-        if (row[e] > -CUDART_INF_F) total += expf(row[e] - top);
-      total = warp_sum(total);
-      if (mine >= 0) w /= total;
+    total = 0.0f;
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) total += l[j] > -CUDART_INF_F ? expf(l[j] - top) : 0.0f;
+    total = warp_sum(total);
+  }
+  // v: what groups and, with a bias, experts are compared by
+  float v[VPL];
+  if (by_logit && !by_sum) {
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) v[j] = l[j];
+  } else {
+    const float inv = __fdividef(1.0f, total);
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) {
+      v[j] = p.sigmoid ? __fdividef(1.0f, 1.0f + __expf(-l[j])) : __expf(l[j] - top) * inv;
+      if (!by_logit && e0 + j < p.E) v[j] += __ldg(p.bias + e0 + j);
+      if (!(l[j] > -CUDART_INF_F) || v[j] != v[j]) v[j] = -CUDART_INF_F;
     }
   }
+  bool near = false;
+  unsigned kept = 0xffffffffu;      // bit per group
+  if (p.groups > 1) {
+    float mine = -CUDART_INF_F;     // the value of group `group`
+    int group, first_of = 1;        // group g is held by lane g * first_of
+    if (p.lanes_per_group) {        // whole lanes, 2^n of them, to a group
+      first_of = p.lanes_per_group;
+      group = lane / first_of;
+      float a = -CUDART_INF_F, b = -CUDART_INF_F;
+#pragma unroll
+      for (int j = 0; j < VPL; ++j) {
+        b = fmaxf(b, fminf(a, v[j]));
+        a = fmaxf(a, v[j]);
+      }
+      for (int o = 1; o < first_of; o <<= 1) {
+        const float a2 = __shfl_xor_sync(0xffffffffu, a, o), b2 = __shfl_xor_sync(0xffffffffu, b, o);
+        b = fmaxf(fminf(a, a2), fmaxf(b, b2));
+        a = fmaxf(a, a2);
+      }
+      mine = by_sum && b > -CUDART_INF_F ? a + b : a;
+    } else {
+      group = lane;
+#pragma unroll
+      for (int j = 0; j < VPL; ++j)
+        if (e0 + j < p.E) row[e0 + j] = v[j];
+      __syncwarp();
+      if (lane < p.groups) {
+        float b = -CUDART_INF_F;
+        for (int i = 0; i < p.group_size; ++i) {
+          const float u = row[lane * p.group_size + i];
+          b = fmaxf(b, fminf(mine, u));
+          mine = fmaxf(mine, u);
+        }
+        if (by_sum && b > -CUDART_INF_F) mine += b;
+      }
+      __syncwarp();
+    }
+    int better = 0;
+    for (int g = 0; g < p.groups; ++g) {
+      const float u = __shfl_sync(0xffffffffu, mine, g * first_of);
+      better += u > mine || (u == mine && g < group);
+    }
+    const bool real = group < p.groups, stays = real && better < p.keep;
+    const unsigned lanes = __ballot_sync(0xffffffffu, stays);
+    if (first_of == 1) kept = lanes;
+    else {
+      kept = 0;
+      for (int g = 0; g < p.groups; ++g) kept |= (lanes >> (g * first_of) & 1u) << g;
+    }
+    if (!by_logit || by_sum) {
+      const float least = from_ordered(__reduce_min_sync(0xffffffffu, stays ? ordered(mine) : 0xffffffffu));
+      const float most = from_ordered(__reduce_max_sync(0xffffffffu, real && !stays ? ordered(mine) : ordered(-CUDART_INF_F)));
+      near = most > -CUDART_INF_F && too_near(least, most, tolerance);
+    }
+  }
+  uint32_t key[VPL], largest = 0;
+  {
+    int group = p.groups > 1 ? e0 / p.group_size : 0, left = p.groups > 1 ? (group + 1) * p.group_size - e0 : VPL;
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) {
+      if (left == 0) {
+        ++group;
+        left = p.group_size;
+      }
+      --left;
+      const float by = by_logit ? l[j] : v[j];
+      key[j] = by > -CUDART_INF_F && (kept >> (group & 31) & 1u) ? ordered(by) : 0u;
+      largest = max(largest, key[j]);
+    }
+  }
+  // the k largest, one by one; with scores that may be off also the one behind them
+  int mine = -1;
+  uint32_t before = 0;
+  const int rounds = by_logit ? p.k : p.k + 1;
+  for (int r = 0; r < rounds && !near; ++r) {
+    const uint32_t m = __reduce_max_sync(0xffffffffu, largest);
+    if (m == 0) break;
+    if (!by_logit && r > 0) near = too_near(from_ordered(before), from_ordered(m), tolerance);
+    before = m;
+    const int from = __ffs(__ballot_sync(0xffffffffu, largest == m)) - 1;
+    int j_of = 0;
+    if (lane == from) {
+      largest = 0;
+      bool done = false;
+#pragma unroll
+      for (int j = 0; j < VPL; ++j) {
+        if (!done && key[j] == m) {
+          done = true;
+          j_of = j;
+          key[j] = 0;
+        }
+        largest = max(largest, key[j]);
+      }
+    }
+    j_of = __shfl_sync(0xffffffffu, j_of, from);
+    if (lane == r && r < p.k) mine = from * VPL + j_of;
+  }
+  if (near) {
+#pragma unroll
+    for (int j = 0; j < VPL; ++j)
+      if (e0 + j < p.E) row[e0 + j] = l[j];
+    __syncwarp();
+    mine = choose(p, row, value, lane);
+  }
+  // the weights, lane j the j-th: softmax over all experts, or without its common factor where the sum divides it out; sigmoid
+  // times e^-m for m = min(0, largest chosen logit), which cannot underflow as a whole
+  const float chosen = mine >= 0 ? finite_logit(to_float(src[mine])) : -CUDART_INF_F;
+  float w = 0.0f;
+  if (p.sigmoid) {
+    const float m = p.renormalise ? fminf(0.0f, warp_max(chosen)) : 0.0f;
+    if (mine >= 0) w = 1.0f / (expf(m) + expf(m - chosen));
+  } else {
+    if (p.renormalise) top = warp_max(chosen);
+    if (mine >= 0) w = expf(chosen - top);
+    if (!p.renormalise && mine >= 0) w /= total;
+  }
   if (p.renormalise) {
-    const float total = warp_sum(w);
-    if (mine >= 0) w /= total;
+    const float sum = warp_sum(w);
+    if (mine >= 0) w /= sum;
   }
   if (lane < p.k) {
     p.ids[t * p.k + lane] = mine;
     p.weights[t * p.k + lane] = w * p.scale;
   }
+}
+
+template <int DT>
+int launch_route(const void* logits, RouteParams p, cudaStream_t st) {
+  const size_t smem = (size_t)ROUTE_WARPS * p.E * 12;
+  const int64_t word = 16 / (int64_t)dtype_size(DT);
+  p.vec = aligned(logits, 16) && p.E % word == 0 && (p.ld % word == 0 || p.T == 1);
+#define MQ_ROUTE(VPL)                                                                                                     \
+  do {                                                                                                                    \
+    const int lanes = p.group_size / VPL;                                                                                 \
+    p.lanes_per_group = p.group_size % VPL == 0 && (lanes & (lanes - 1)) == 0 && lanes * p.groups <= 32 ? lanes : 0;      \
+    if (smem > 48 * 1024) MQ_CUDA(cudaFuncSetAttribute(route_kernel<DT, VPL>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)); \
+    MQ_CUDA(launch_chained(true, route_kernel<DT, VPL>, dim3((unsigned)ceil_div(p.T, ROUTE_WARPS)), dim3(ROUTE_WARPS * 32), smem, st, logits, p)); \
+  } while (0)
+  if (p.E <= 32) MQ_ROUTE(1);
+  else if (p.E <= 64) MQ_ROUTE(2);
+  else if (p.E <= 128) MQ_ROUTE(4);
+  else if (p.E <= 256) MQ_ROUTE(8);
+  else if (p.E <= 512) MQ_ROUTE(16);
+  else MQ_ROUTE(32);
+#undef MQ_ROUTE
+  MQ_LAUNCH_CHECK();
+  return MQ_OK;
 }
 
 // ---------------------------------------------------------------- the plan
@@ -189,6 +374,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_count_kernel(const PlanPara
   extern __shared__ int plan_smem[];
   for (int e = threadIdx.x; e < p.E; e += PLAN_THREADS) plan_smem[e] = 0;
   __syncthreads();
+  chain_wait();
+  chain_release();
   const int64_t begin = (int64_t)blockIdx.x * p.run, end = min(begin + p.run, p.pairs);
   for (int64_t i = begin + threadIdx.x; i < end; i += PLAN_THREADS) {
     const int e = expert_of(p, i, end);
@@ -199,7 +386,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_count_kernel(const PlanPara
 }
 
 __global__ void __launch_bounds__(PLAN_THREADS) plan_place_kernel(const PlanParams p) {
-  extern __shared__ int plan_smem[];                 // next[warp][e]: where this warp's next pair of e goes
+  extern __shared__ int plan_smem[];                 // next[warp][e]: where this warp's next pair of e goes; total[e], before[e]
   __shared__ int warp_total[PLAN_WARPS];
   __shared__ int all_pairs;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -207,8 +394,29 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_place_kernel(const PlanPara
   const int per_warp = p.run / PLAN_WARPS;
   const int64_t w_begin = begin + (int64_t)warp * per_warp, w_end = min(w_begin + per_warp, end);
   int* next = plan_smem + warp * p.E;
-  for (int i = threadIdx.x; i < p.E * PLAN_WARPS; i += PLAN_THREADS) plan_smem[i] = 0;
+  int *totals = plan_smem + PLAN_WARPS * p.E, *befores = totals + p.E;
+  for (int i = threadIdx.x; i < p.E * (PLAN_WARPS + 2); i += PLAN_THREADS) plan_smem[i] = 0;
   __syncthreads();
+  chain_wait();
+  chain_release();
+  if (p.counts) {
+    // all blocks' counts: every warp a share of the blocks, its loads independent of one another (one thread per expert that walks
+    // through the blocks waits for each in turn: 18 us for 524288 pairs)
+    for (int e0 = 0; e0 < p.E; e0 += 32) {
+      const int e = e0 + lane;
+      int total = 0, before = 0;
+      if (e < p.E) {
+#pragma unroll 10
+        for (int b = warp; b < (int)gridDim.x; b += PLAN_WARPS) {
+          const int c = __ldcg(p.counts + (int64_t)b * p.E + e);
+          total += c;
+          before += b < (int)blockIdx.x ? c : 0;
+        }
+        atomicAdd(&totals[e], total);
+        atomicAdd(&befores[e], before);
+      }
+    }
+  }
   for (int64_t i = w_begin + lane; i < w_end; i += 32) {
     const int e = expert_of(p, i, w_end);
     if (e >= 0) atomicAdd(&next[e], 1);
@@ -221,11 +429,8 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_place_kernel(const PlanPara
     int total = 0, before = 0;
     if (e < p.E) {
       if (p.counts) {
-        for (int b = 0; b < (int)gridDim.x; ++b) {
-          const int c = p.counts[(int64_t)b * p.E + e];
-          if (b < (int)blockIdx.x) before += c;
-          total += c;
-        }
+        total = totals[e];
+        before = befores[e];
       } else {
         for (int w = 0; w < PLAN_WARPS; ++w) total += plan_smem[w * p.E + e];
       }
@@ -302,13 +507,9 @@ extern "C" int mq_route_tokens(const void* logits, int dtype, int64_t T, int64_t
   if (T == 0) return MQ_OK;
   MQ_REQUIRE(logits && ids && weights, MQ_ERR_ARGUMENT, "mq_route_tokens: null pointer");
   MQ_REQUIRE(ceil_div(T, ROUTE_WARPS) < (1ll << 31), MQ_ERR_UNSUPPORTED, "mq_route_tokens: too many tokens");
-  RouteParams p = {T, ld, (int)E, top_k, groups, keep_groups, (int)(E / groups), score == 1, group_score == 1, renormalise != 0, scale, bias, ids, weights};
-  const size_t smem = (size_t)ROUTE_WARPS * E * 12;
-  auto kernel = dtype == MQ_F32 ? route_kernel<MQ_F32> : dtype == MQ_BF16 ? route_kernel<MQ_BF16> : route_kernel<MQ_F16>;
-  if (smem > 48 * 1024) MQ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  kernel<<<(unsigned)ceil_div(T, ROUTE_WARPS), ROUTE_WARPS * 32, smem, static_cast<cudaStream_t>(stream)>>>(logits, p);
-  MQ_LAUNCH_CHECK();
-  return MQ_OK;
+  RouteParams p = {T, ld, (int)E, top_k, groups, keep_groups, (int)(E / groups), score == 1, group_score == 1, renormalise != 0, scale, bias, ids, weights, false, 0};
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return dtype == MQ_F32 ? launch_route<MQ_F32>(logits, p, st) : dtype == MQ_BF16 ? launch_route<MQ_BF16>(logits, p, st) : launch_route<MQ_F16>(logits, p, st);
 }
 
 extern "C" size_t mq_expert_plan_workspace_bytes(int64_t pairs, int64_t E) {
@@ -324,12 +525,12 @@ int expert_plan(const int32_t* ids, int64_t pairs, int E, int first, int32_t* of
   PlanParams p = {ids, pairs, E, first, (int)(ceil_div(ceil_div(pairs > 0 ? pairs : 1, blocks), unit) * unit), nullptr, offsets, order, place};
   if (blocks > 1) {
     p.counts = static_cast<int32_t*>(workspace);
-    plan_count_kernel<<<blocks, PLAN_THREADS, (size_t)E * 4, st>>>(p);
+    MQ_CUDA(launch_chained(true, plan_count_kernel, dim3(blocks), dim3(PLAN_THREADS), (size_t)E * 4, st, p));
     MQ_LAUNCH_CHECK();
   }
-  const size_t smem = (size_t)E * PLAN_WARPS * 4;
+  const size_t smem = (size_t)E * (PLAN_WARPS + 2) * 4;
   if (smem > 48 * 1024) MQ_CUDA(cudaFuncSetAttribute(plan_place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
-  plan_place_kernel<<<blocks, PLAN_THREADS, smem, st>>>(p);
+  MQ_CUDA(launch_chained(true, plan_place_kernel, dim3(blocks), dim3(PLAN_THREADS), smem, st, p));
   MQ_LAUNCH_CHECK();
   return MQ_OK;
 }

@@ -34,8 +34,10 @@ def route(logits, k, score="softmax", bias=None, groups=1, keep=None, group_scor
         if groups > 1:
             size = E // groups
             of = []
+            # largest values without a bias: in the order of the logits, also where the scores are below the smallest number
+            worth = order if group_score == "max" else value
             for g in range(groups):
-                v = sorted((value[e] for e in can if e // size == g), reverse=True)
+                v = sorted((worth[e] for e in can if e // size == g), reverse=True)
                 of.append(sum(v[:2] if group_score == "top2" else v[:1]) if v else -math.inf)
             kept = sorted(range(groups), key=lambda g: (-of[g], g))[:keep]
             can = [e for e in can if e // size in kept]
