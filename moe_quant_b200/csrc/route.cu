@@ -132,10 +132,41 @@ __device__ __forceinline__ uint32_t ordered(float v) {
 }
 __device__ __forceinline__ float from_ordered(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k); }
 
-// Whether a value that came out as `a` may in truth not lie above one that came out as `b` <= a.  Sigmoid: exponential, quotient and sum are
-// off by 4e-7 at most, the bias' sum by 2^-24 |v|; softmax: the sum over up to 1024 experts (32 in a lane, five levels of lanes) and the
-// exponentials by 3.2e-6.  Two values, or two sums of two.
-__device__ __forceinline__ bool too_near(float a, float b, float tolerance) { return !(a - b > tolerance * (1.0f + fmaxf(fabsf(a), fabsf(b)))); }
+// Scores for the choice: exponential and reciprocal as the hardware has them.
+__device__ __forceinline__ float quick_exp(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x * 1.44269504f));
+  return y;
+}
+__device__ __forceinline__ float quick_sigmoid(float l) {
+  float y;
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(1.0f + quick_exp(-l)));
+  return y;
+}
+
+// Whether a value that came out as `a` may in truth not lie above one that came out as `b` <= a; `size` bounds what the values were summed
+// from.  quick_sigmoid is off by 4e-7 at most (the exponential by 2^-22 and by 9e-8 |l|, times s (1 - s); sum and reciprocal by
+// 2^-23 each), the sum with the bias by 2^-24 |v|, a softmax score by 3.2e-6 (its sum over up to 1024 experts, 32 in a lane and five levels of
+// lanes, and the exponentials), and the low bits that give way to an index by 2^-23 VPL |v|.  Two values, or two sums of two.
+__device__ __forceinline__ bool too_near(float a, float b, float tolerance, float size) { return !(a - b > tolerance * (1.0f + size)); }
+
+// Descending, by a network of compare-exchanges (odd-even merges).
+template <int N>
+__device__ __forceinline__ void sort_descending(uint32_t (&k)[N]) {
+#pragma unroll
+  for (int p = 1; p < N; p <<= 1)
+#pragma unroll
+    for (int q = p; q >= 1; q >>= 1)
+#pragma unroll
+      for (int j = q % p; j + q < N; j += 2 * q)
+#pragma unroll
+        for (int i = 0; i < q; ++i)
+          if (j + i + q < N && (j + i) / (2 * p) == (j + i + q) / (2 * p)) {
+            const uint32_t a = k[j + i], b = k[j + i + q];
+            k[j + i] = max(a, b);
+            k[j + i + q] = min(a, b);
+          }
+}
 
 // VPL experts per lane: VPL lane .. VPL lane + VPL - 1
 template <int DT, int VPL>
@@ -173,7 +204,7 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32) route_kernel(const void* __r
 
   const bool by_logit = p.bias == nullptr;   // sigmoid and softmax are increasing
   const bool by_sum = p.groups > 1 && p.top2;
-  const float tolerance = p.sigmoid ? 4e-6f : 2e-5f;
+  const float tolerance = !p.sigmoid ? 2e-5f : VPL <= 8 ? 4e-6f : 1e-5f;
   // softmax: its largest logit and sum, where scores are needed
   float top = 0.0f, total = 1.0f;
   if (!p.sigmoid && (!by_logit || by_sum || !p.renormalise)) {
@@ -195,20 +226,20 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32) route_kernel(const void* __r
     const float inv = __fdividef(1.0f, total);
 #pragma unroll
     for (int j = 0; j < VPL; ++j) {
-      v[j] = p.sigmoid ? __fdividef(1.0f, 1.0f + __expf(-l[j])) : __expf(l[j] - top) * inv;
+      v[j] = p.sigmoid ? quick_sigmoid(l[j]) : quick_exp(l[j] - top) * inv;
       if (!by_logit && e0 + j < p.E) v[j] += __ldg(p.bias + e0 + j);
       if (!(l[j] > -CUDART_INF_F) || v[j] != v[j]) v[j] = -CUDART_INF_F;
     }
   }
   bool near = false;
-  unsigned kept = 0xffffffffu;      // bit per group
+  bool whole_lane = true;           // groups keep or drop all of a lane's experts
+  unsigned kept = 0xffffffffu;      // otherwise: bit per group
   if (p.groups > 1) {
-    float mine = -CUDART_INF_F;     // the value of group `group`
-    int group, first_of = 1;        // group g is held by lane g * first_of
-    if (p.lanes_per_group) {        // whole lanes, 2^n of them, to a group
+    float a = -CUDART_INF_F, b = -CUDART_INF_F;     // the two largest of group `group`
+    int group, first_of = 1;                        // group g is held by lane g * first_of
+    if (p.lanes_per_group) {                        // whole lanes, 2^n of them, to a group
       first_of = p.lanes_per_group;
       group = lane / first_of;
-      float a = -CUDART_INF_F, b = -CUDART_INF_F;
 #pragma unroll
       for (int j = 0; j < VPL; ++j) {
         b = fmaxf(b, fminf(a, v[j]));
@@ -219,7 +250,6 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32) route_kernel(const void* __r
         b = fmaxf(fminf(a, a2), fmaxf(b, b2));
         a = fmaxf(a, a2);
       }
-      mine = by_sum && b > -CUDART_INF_F ? a + b : a;
     } else {
       group = lane;
 #pragma unroll
@@ -227,75 +257,81 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32) route_kernel(const void* __r
         if (e0 + j < p.E) row[e0 + j] = v[j];
       __syncwarp();
       if (lane < p.groups) {
-        float b = -CUDART_INF_F;
         for (int i = 0; i < p.group_size; ++i) {
           const float u = row[lane * p.group_size + i];
-          b = fmaxf(b, fminf(mine, u));
-          mine = fmaxf(mine, u);
+          b = fmaxf(b, fminf(a, u));
+          a = fmaxf(a, u);
         }
-        if (by_sum && b > -CUDART_INF_F) mine += b;
       }
       __syncwarp();
     }
+    const float mine = by_sum && b > -CUDART_INF_F ? a + b : a;
     int better = 0;
     for (int g = 0; g < p.groups; ++g) {
       const float u = __shfl_sync(0xffffffffu, mine, g * first_of);
       better += u > mine || (u == mine && g < group);
     }
     const bool real = group < p.groups, stays = real && better < p.keep;
-    const unsigned lanes = __ballot_sync(0xffffffffu, stays);
-    if (first_of == 1) kept = lanes;
-    else {
-      kept = 0;
-      for (int g = 0; g < p.groups; ++g) kept |= (lanes >> (g * first_of) & 1u) << g;
-    }
+    whole_lane = p.lanes_per_group != 0;
+    kept = __ballot_sync(0xffffffffu, stays);
     if (!by_logit || by_sum) {
       const float least = from_ordered(__reduce_min_sync(0xffffffffu, stays ? ordered(mine) : 0xffffffffu));
       const float most = from_ordered(__reduce_max_sync(0xffffffffu, real && !stays ? ordered(mine) : ordered(-CUDART_INF_F)));
-      near = most > -CUDART_INF_F && too_near(least, most, tolerance);
+      const float size = real && mine > -CUDART_INF_F ? fabsf(a) + (b > -CUDART_INF_F ? fabsf(b) : 0.0f) : 0.0f;
+      near = most > -CUDART_INF_F && too_near(least, most, tolerance, __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(size))));
     }
   }
-  uint32_t key[VPL], largest = 0;
+  // Keys: the number, its lowest bits replaced by which of the lane's experts it is, the first one highest.  Sorted, so that a lane offers its
+  // largest and moves up once it is taken.
+  constexpr uint32_t WHICH = VPL - 1;
+  uint32_t key[VPL];
   {
-    int group = p.groups > 1 ? e0 / p.group_size : 0, left = p.groups > 1 ? (group + 1) * p.group_size - e0 : VPL;
+    const bool in = !whole_lane || p.groups == 1 || (kept >> lane & 1u);
+    int group = 0, left = VPL;
+    if (!whole_lane) {
+      group = e0 / p.group_size;
+      left = (group + 1) * p.group_size - e0;
+    }
 #pragma unroll
     for (int j = 0; j < VPL; ++j) {
-      if (left == 0) {
-        ++group;
-        left = p.group_size;
-      }
-      --left;
       const float by = by_logit ? l[j] : v[j];
-      key[j] = by > -CUDART_INF_F && (kept >> (group & 31) & 1u) ? ordered(by) : 0u;
-      largest = max(largest, key[j]);
+      bool can = in && by > -CUDART_INF_F;
+      if (!whole_lane) {
+        if (left == 0) {
+          ++group;
+          left = p.group_size;
+        }
+        --left;
+        can = can && (kept >> (group & 31) & 1u);
+      }
+      key[j] = can ? (ordered(by) & ~WHICH) | (WHICH - (uint32_t)j) : 0u;
     }
   }
-  // the k largest, one by one; with scores that may be off also the one behind them
+  sort_descending(key);
+  // The k largest, one by one, and where numbers may have lost what sets them apart the one behind them.  (The low bits of 16-bit logits
+  // are empty.)
+  const bool exact = by_logit && sizeof(T) == 2;
   int mine = -1;
   uint32_t before = 0;
-  const int rounds = by_logit ? p.k : p.k + 1;
-  for (int r = 0; r < rounds && !near; ++r) {
-    const uint32_t m = __reduce_max_sync(0xffffffffu, largest);
+  const int rounds = exact ? p.k : p.k + 1;
+  for (int r = 0; r < rounds; ++r) {
+    const uint32_t head = key[0] & ~WHICH;
+    const uint32_t m = __reduce_max_sync(0xffffffffu, head);
     if (m == 0) break;
-    if (!by_logit && r > 0) near = too_near(from_ordered(before), from_ordered(m), tolerance);
-    before = m;
-    const int from = __ffs(__ballot_sync(0xffffffffu, largest == m)) - 1;
-    int j_of = 0;
-    if (lane == from) {
-      largest = 0;
-      bool done = false;
-#pragma unroll
-      for (int j = 0; j < VPL; ++j) {
-        if (!done && key[j] == m) {
-          done = true;
-          j_of = j;
-          key[j] = 0;
-        }
-        largest = max(largest, key[j]);
-      }
+    if (!exact && r > 0) {
+      const float a = from_ordered(before), b = from_ordered(m);
+      near |= by_logit ? m == before : too_near(a, b, tolerance, fmaxf(fabsf(a), fabsf(b)));
+      if (near) break;
     }
-    j_of = __shfl_sync(0xffffffffu, j_of, from);
-    if (lane == r && r < p.k) mine = from * VPL + j_of;
+    before = m;
+    const int from = __ffs(__ballot_sync(0xffffffffu, head == m)) - 1;
+    const uint32_t taken = __shfl_sync(0xffffffffu, key[0], from);
+    if (lane == r && r < p.k) mine = from * VPL + (int)(WHICH - (taken & WHICH));
+    if (lane == from) {
+#pragma unroll
+      for (int j = 0; j + 1 < VPL; ++j) key[j] = key[j + 1];
+      key[VPL - 1] = 0;
+    }
   }
   if (near) {
 #pragma unroll
@@ -353,7 +389,7 @@ int launch_route(const void* logits, RouteParams p, cudaStream_t st) {
 // A stable counting sort of the pairs by expert.  Every block takes a run of pairs; the first kernel counts them by expert, the
 // second adds up the blocks in front and ranks its own.  Within a block each warp takes a run of its own, 32 pairs at a
 // time; equal experts among the 32 are ranked by a match.
-constexpr int PLAN_THREADS = 512, PLAN_WARPS = PLAN_THREADS / 32;
+constexpr int PLAN_THREADS = 512, PLAN_WARPS = PLAN_THREADS / 32, PLAN_KEEP = 8;
 
 struct PlanParams {
   const int32_t* ids;
@@ -417,9 +453,18 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_place_kernel(const PlanPara
       }
     }
   }
-  for (int64_t i = w_begin + lane; i < w_end; i += 32) {
-    const int e = expert_of(p, i, w_end);
-    if (e >= 0) atomicAdd(&next[e], 1);
+  // the experts of the warp's pairs, PLAN_KEEP at a time in registers; a run that is no longer stays there
+  int mine[PLAN_KEEP];
+  const bool all_kept = per_warp <= 32 * PLAN_KEEP;
+  auto load = [&](int64_t i0) {
+#pragma unroll
+    for (int i = 0; i < PLAN_KEEP; ++i) mine[i] = expert_of(p, i0 + i * 32 + lane, w_end);
+  };
+  for (int64_t i0 = w_begin; i0 < w_end; i0 += 32 * PLAN_KEEP) {
+    load(i0);
+#pragma unroll
+    for (int i = 0; i < PLAN_KEEP; ++i)
+      if (mine[i] >= 0) atomicAdd(&next[mine[i]], 1);
   }
   __syncthreads();
   // experts in slices of PLAN_THREADS: pairs of all experts in front, of this one in the blocks in front, of this block's warps in front
@@ -461,22 +506,27 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_place_kernel(const PlanPara
     if (blockIdx.x == 0) p.offsets[p.E] = in_front;
   }
   __syncthreads();
-  for (int64_t i0 = w_begin; i0 < w_end; i0 += 32) {
-    const int64_t i = i0 + lane;
-    const int e = expert_of(p, i, w_end);
-    const unsigned same = __match_any_sync(0xffffffffu, e);
-    const int rank = __popc(same & ((1u << lane) - 1u));
-    int at = -1;
-    if (e >= 0) at = next[e] + rank;
-    __syncwarp();
-    if (e >= 0) {
-      if (rank == 0) next[e] = at + __popc(same);
-      p.order[at] = (int32_t)i;
-    }
-    __syncwarp();
-    if (i < w_end) {
-      p.place[i] = at;
-      if (i >= all_pairs) p.order[i] = -1;   // behind the last pair
+  for (int64_t i0 = w_begin; i0 < w_end; i0 += 32 * PLAN_KEEP) {
+    if (!all_kept) load(i0);
+#pragma unroll
+    for (int b = 0; b < PLAN_KEEP; ++b) {
+      const int64_t i = i0 + b * 32 + lane;
+      if (i - lane >= w_end) break;
+      const int e = mine[b];
+      const unsigned same = __match_any_sync(0xffffffffu, e);
+      const int rank = __popc(same & ((1u << lane) - 1u));
+      int at = -1;
+      if (e >= 0) at = next[e] + rank;
+      __syncwarp();
+      if (e >= 0) {
+        if (rank == 0) next[e] = at + __popc(same);
+        p.order[at] = (int32_t)i;
+      }
+      __syncwarp();
+      if (i < w_end) {
+        p.place[i] = at;
+        if (i >= all_pairs) p.order[i] = -1;   // behind the last pair
+      }
     }
   }
 }
