@@ -30,7 +30,8 @@ struct RouteParams {
   int lanes_per_group;    // lanes that hold a group, 0 where lanes and groups do not match
 };
 
-__device__ __forceinline__ float finite_logit(float l) { return l != l ? -CUDART_INF_F : fminf(l, 3.402823466e38f); }
+// NaN is -inf, +inf the largest number
+__device__ __forceinline__ float finite_logit(float l) { return fminf(fmaxf(l, -CUDART_INF_F), 3.402823466e38f); }
 
 template <typename F>
 __device__ __forceinline__ F warp_sum(F v) {
@@ -127,8 +128,8 @@ __device__ int choose(const RouteParams& p, const float* row, double* value, int
 
 // fp32 numbers as unsigned integers of the same order; 0 stands for an expert that cannot be chosen
 __device__ __forceinline__ uint32_t ordered(float v) {
-  const uint32_t b = __float_as_uint(v);
-  return b & 0x80000000u ? ~b : b | 0x80000000u;
+  const int b = __float_as_int(v);
+  return (uint32_t)(b ^ ((b >> 31) | (int)0x80000000));
 }
 __device__ __forceinline__ float from_ordered(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7FFFFFFFu : ~k); }
 
@@ -168,197 +169,213 @@ __device__ __forceinline__ void sort_descending(uint32_t (&k)[N]) {
           }
 }
 
-// VPL experts per lane: VPL lane .. VPL lane + VPL - 1
+// VPL experts per lane: VPL lane .. VPL lane + VPL - 1.  A warp takes every so many tokens; its next token's logits are on their way while it
+// chooses.  Instructions bound it: about 700 a token at 256 experts, 8 groups and a choice of 8.
+constexpr int route_blocks(int vpl) { return vpl <= 4 ? 5 : vpl <= 8 ? 3 : vpl <= 16 ? 2 : 1; }   // per SM
+
 template <int DT, int VPL>
-__global__ void __launch_bounds__(ROUTE_WARPS * 32) route_kernel(const void* __restrict__ logits, const RouteParams p) {
+__global__ void __launch_bounds__(ROUTE_WARPS * 32, route_blocks(VPL)) route_kernel(const void* __restrict__ logits, const RouteParams p) {
   using T = typename StorageOf<DT>::type;
+  constexpr int WORD = VPL * sizeof(T) >= 16 ? 16 / sizeof(T) : 1;     // values per load
+  struct alignas(WORD * sizeof(T)) Word { T v[WORD]; };
   extern __shared__ double route_smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   double* value = route_smem + (size_t)warp * p.E;
   float* row = reinterpret_cast<float*>(route_smem + (size_t)ROUTE_WARPS * p.E) + (size_t)warp * p.E;
-  const int64_t t = (int64_t)blockIdx.x * ROUTE_WARPS + warp;
-  chain_wait();
-  chain_release();
-  if (t >= p.T) return;
-  const T* src = static_cast<const T*>(logits) + t * p.ld;
   const int e0 = lane * VPL;
-  float l[VPL];
-  constexpr int WORD = VPL * sizeof(T) >= 16 ? 16 / sizeof(T) : 1;     // values per load
-  if (WORD > 1 && p.vec) {
-#pragma unroll
-    for (int j = 0; j < VPL; j += WORD) {
-      struct alignas(WORD * sizeof(T)) Word { T v[WORD]; } w;
-      if (e0 + j < p.E) {     // E is a multiple of WORD
-        w = *reinterpret_cast<const Word*>(src + e0 + j);
-#pragma unroll
-        for (int i = 0; i < WORD; ++i) l[j + i] = finite_logit(to_float(w.v[i]));
-      } else {
-#pragma unroll
-        for (int i = 0; i < WORD; ++i) l[j + i] = -CUDART_INF_F;
-      }
-    }
-  } else {
-#pragma unroll
-    for (int j = 0; j < VPL; ++j) l[j] = e0 + j < p.E ? finite_logit(to_float(src[e0 + j])) : -CUDART_INF_F;
-  }
-
   const bool by_logit = p.bias == nullptr;   // sigmoid and softmax are increasing
   const bool by_sum = p.groups > 1 && p.top2;
+  const bool by_score = !by_logit || by_sum;
   const float tolerance = !p.sigmoid ? 2e-5f : VPL <= 8 ? 4e-6f : 1e-5f;
-  // softmax: its largest logit and sum, where scores are needed
-  float top = 0.0f, total = 1.0f;
-  if (!p.sigmoid && (!by_logit || by_sum || !p.renormalise)) {
-    top = l[0];
+  const int64_t stride = (int64_t)gridDim.x * ROUTE_WARPS;
+  chain_wait();
+  chain_release();
+
+  Word raw[VPL / WORD];
+  auto load = [&](int64_t t) {
+    const T* src = static_cast<const T*>(logits) + t * p.ld + e0;
 #pragma unroll
-    for (int j = 1; j < VPL; ++j) top = fmaxf(top, l[j]);
-    top = warp_max(top);
-    total = 0.0f;
+    for (int j = 0; j < VPL / WORD; ++j) {
+      if (WORD == 1 || p.vec) {     // (then E is a multiple of WORD)
+        if (e0 + j * WORD < p.E) raw[j] = *reinterpret_cast<const Word*>(src + j * WORD);
+      } else {
 #pragma unroll
-    for (int j = 0; j < VPL; ++j) total += l[j] > -CUDART_INF_F ? expf(l[j] - top) : 0.0f;
-    total = warp_sum(total);
-  }
-  // v: what groups and, with a bias, experts are compared by
-  float v[VPL];
-  if (by_logit && !by_sum) {
-#pragma unroll
-    for (int j = 0; j < VPL; ++j) v[j] = l[j];
-  } else {
-    const float inv = __fdividef(1.0f, total);
-#pragma unroll
-    for (int j = 0; j < VPL; ++j) {
-      v[j] = p.sigmoid ? quick_sigmoid(l[j]) : quick_exp(l[j] - top) * inv;
-      if (!by_logit && e0 + j < p.E) v[j] += __ldg(p.bias + e0 + j);
-      if (!(l[j] > -CUDART_INF_F) || v[j] != v[j]) v[j] = -CUDART_INF_F;
+        for (int i = 0; i < WORD; ++i)
+          if (e0 + j * WORD + i < p.E) raw[j].v[i] = src[j * WORD + i];
+      }
     }
-  }
-  bool near = false;
-  bool whole_lane = true;           // groups keep or drop all of a lane's experts
-  unsigned kept = 0xffffffffu;      // otherwise: bit per group
-  if (p.groups > 1) {
-    float a = -CUDART_INF_F, b = -CUDART_INF_F;     // the two largest of group `group`
-    int group, first_of = 1;                        // group g is held by lane g * first_of
-    if (p.lanes_per_group) {                        // whole lanes, 2^n of them, to a group
-      first_of = p.lanes_per_group;
-      group = lane / first_of;
+  };
+  float bias[VPL];
+#pragma unroll
+  for (int j = 0; j < VPL; ++j) bias[j] = by_logit || e0 + j >= p.E ? 0.0f : fmaxf(p.bias[e0 + j], -CUDART_INF_F);   // NaN is -inf
+
+  int64_t t = (int64_t)blockIdx.x * ROUTE_WARPS + warp;
+  if (t < p.T) load(t);
+  for (; t < p.T; t += stride) {
+    float l[VPL];
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) l[j] = e0 + j < p.E ? finite_logit(to_float(raw[j / WORD].v[j % WORD])) : -CUDART_INF_F;
+    if (t + stride < p.T) load(t + stride);
+
+    // softmax: its largest logit and sum, where scores are needed
+    float top = 0.0f, total = 1.0f;
+    if (!p.sigmoid && (by_score || !p.renormalise)) {
+      top = l[0];
+#pragma unroll
+      for (int j = 1; j < VPL; ++j) top = fmaxf(top, l[j]);
+      top = warp_max(top);
+      total = 0.0f;
+#pragma unroll
+      for (int j = 0; j < VPL; ++j) total += l[j] > -CUDART_INF_F ? expf(l[j] - top) : 0.0f;
+      total = warp_sum(total);
+    }
+    // v: what groups and, with a bias, experts are compared by
+    float v[VPL];
+    if (!by_score) {
+#pragma unroll
+      for (int j = 0; j < VPL; ++j) v[j] = l[j];
+    } else {
+      const float inv = __fdividef(1.0f, total);
 #pragma unroll
       for (int j = 0; j < VPL; ++j) {
-        b = fmaxf(b, fminf(a, v[j]));
-        a = fmaxf(a, v[j]);
+        const float s = p.sigmoid ? quick_sigmoid(l[j]) : quick_exp(l[j] - top) * inv;
+        v[j] = l[j] > -CUDART_INF_F ? s + bias[j] : -CUDART_INF_F;
       }
-      for (int o = 1; o < first_of; o <<= 1) {
-        const float a2 = __shfl_xor_sync(0xffffffffu, a, o), b2 = __shfl_xor_sync(0xffffffffu, b, o);
-        b = fmaxf(fminf(a, a2), fmaxf(b, b2));
-        a = fmaxf(a, a2);
-      }
-    } else {
-      group = lane;
+    }
+    bool near = false;
+    bool whole_lane = true;           // groups keep or drop all of a lane's experts
+    unsigned kept = 0xffffffffu;      // bit per lane, or per group
+    if (p.groups > 1) {
+      float a = -CUDART_INF_F, b = -CUDART_INF_F;     // the two largest of group `group`
+      int group, first_of = 1;                        // group g is held by lane g * first_of
+      if (p.lanes_per_group) {                        // whole lanes, 2^n of them, to a group
+        first_of = p.lanes_per_group;
+        group = lane / first_of;
 #pragma unroll
-      for (int j = 0; j < VPL; ++j)
-        if (e0 + j < p.E) row[e0 + j] = v[j];
-      __syncwarp();
-      if (lane < p.groups) {
-        for (int i = 0; i < p.group_size; ++i) {
-          const float u = row[lane * p.group_size + i];
-          b = fmaxf(b, fminf(a, u));
-          a = fmaxf(a, u);
+        for (int j = 0; j < VPL; ++j) {
+          b = fmaxf(b, fminf(a, v[j]));
+          a = fmaxf(a, v[j]);
         }
+        for (int o = 1; o < first_of; o <<= 1) {
+          const float a2 = __shfl_xor_sync(0xffffffffu, a, o), b2 = __shfl_xor_sync(0xffffffffu, b, o);
+          b = fmaxf(fminf(a, a2), fmaxf(b, b2));
+          a = fmaxf(a, a2);
+        }
+      } else {
+        group = lane;
+#pragma unroll
+        for (int j = 0; j < VPL; ++j)
+          if (e0 + j < p.E) row[e0 + j] = v[j];
+        __syncwarp();
+        if (lane < p.groups) {
+          for (int i = 0; i < p.group_size; ++i) {
+            const float u = row[lane * p.group_size + i];
+            b = fmaxf(b, fminf(a, u));
+            a = fmaxf(a, u);
+          }
+        }
+        __syncwarp();
       }
-      __syncwarp();
+      const float mine = by_sum && b > -CUDART_INF_F ? a + b : a;
+      int better = 0;
+      for (int g = 0; g < p.groups; ++g) {
+        const float u = __shfl_sync(0xffffffffu, mine, g * first_of);
+        better += u > mine || (u == mine && g < group);
+      }
+      const bool real = group < p.groups, stays = real && better < p.keep;
+      whole_lane = p.lanes_per_group != 0;
+      kept = __ballot_sync(0xffffffffu, stays);
+      if (by_score) {
+        const float least = from_ordered(__reduce_min_sync(0xffffffffu, stays ? ordered(mine) : 0xffffffffu));
+        const float most = from_ordered(__reduce_max_sync(0xffffffffu, real && !stays ? ordered(mine) : ordered(-CUDART_INF_F)));
+        const float size = real && mine > -CUDART_INF_F ? fabsf(a) + (b > -CUDART_INF_F ? fabsf(b) : 0.0f) : 0.0f;
+        near = most > -CUDART_INF_F && too_near(least, most, tolerance, __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(size))));
+      }
     }
-    const float mine = by_sum && b > -CUDART_INF_F ? a + b : a;
-    int better = 0;
-    for (int g = 0; g < p.groups; ++g) {
-      const float u = __shfl_sync(0xffffffffu, mine, g * first_of);
-      better += u > mine || (u == mine && g < group);
-    }
-    const bool real = group < p.groups, stays = real && better < p.keep;
-    whole_lane = p.lanes_per_group != 0;
-    kept = __ballot_sync(0xffffffffu, stays);
-    if (!by_logit || by_sum) {
-      const float least = from_ordered(__reduce_min_sync(0xffffffffu, stays ? ordered(mine) : 0xffffffffu));
-      const float most = from_ordered(__reduce_max_sync(0xffffffffu, real && !stays ? ordered(mine) : ordered(-CUDART_INF_F)));
-      const float size = real && mine > -CUDART_INF_F ? fabsf(a) + (b > -CUDART_INF_F ? fabsf(b) : 0.0f) : 0.0f;
-      near = most > -CUDART_INF_F && too_near(least, most, tolerance, __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(size))));
-    }
-  }
-  // Keys: the number, its lowest bits replaced by which of the lane's experts it is, the first one highest.  Sorted, so that a lane offers its
-  // largest and moves up once it is taken.
-  constexpr uint32_t WHICH = VPL - 1;
-  uint32_t key[VPL];
-  {
-    const bool in = !whole_lane || p.groups == 1 || (kept >> lane & 1u);
-    int group = 0, left = VPL;
-    if (!whole_lane) {
-      group = e0 / p.group_size;
-      left = (group + 1) * p.group_size - e0;
-    }
+    // Keys: the number, its lowest bits replaced by which of the lane's experts it is, the first one highest.  Sorted, so that a lane offers its
+    // largest and moves up once it is taken.
+    constexpr uint32_t WHICH = VPL - 1;
+    uint32_t key[VPL];
 #pragma unroll
     for (int j = 0; j < VPL; ++j) {
       const float by = by_logit ? l[j] : v[j];
-      bool can = in && by > -CUDART_INF_F;
-      if (!whole_lane) {
+      key[j] = by > -CUDART_INF_F ? (ordered(by) & ~WHICH) | (WHICH - (uint32_t)j) : 0u;
+    }
+    if (whole_lane) {
+      if (!(kept >> lane & 1u))
+#pragma unroll
+        for (int j = 0; j < VPL; ++j) key[j] = 0;
+    } else {
+      int group = e0 / p.group_size, left = (group + 1) * p.group_size - e0;
+#pragma unroll
+      for (int j = 0; j < VPL; ++j) {
         if (left == 0) {
           ++group;
           left = p.group_size;
         }
         --left;
-        can = can && (kept >> (group & 31) & 1u);
+        if (!(kept >> (group & 31) & 1u)) key[j] = 0;
       }
-      key[j] = can ? (ordered(by) & ~WHICH) | (WHICH - (uint32_t)j) : 0u;
     }
-  }
-  sort_descending(key);
-  // The k largest, one by one, and where numbers may have lost what sets them apart the one behind them.  (The low bits of 16-bit logits
-  // are empty.)
-  const bool exact = by_logit && sizeof(T) == 2;
-  int mine = -1;
-  uint32_t before = 0;
-  const int rounds = exact ? p.k : p.k + 1;
-  for (int r = 0; r < rounds; ++r) {
-    const uint32_t head = key[0] & ~WHICH;
-    const uint32_t m = __reduce_max_sync(0xffffffffu, head);
-    if (m == 0) break;
-    if (!exact && r > 0) {
-      const float a = from_ordered(before), b = from_ordered(m);
-      near |= by_logit ? m == before : too_near(a, b, tolerance, fmaxf(fabsf(a), fabsf(b)));
-      if (near) break;
-    }
-    before = m;
-    const int from = __ffs(__ballot_sync(0xffffffffu, head == m)) - 1;
-    const uint32_t taken = __shfl_sync(0xffffffffu, key[0], from);
-    if (lane == r && r < p.k) mine = from * VPL + (int)(WHICH - (taken & WHICH));
-    if (lane == from) {
+    sort_descending(key);
+    // The k largest, one by one, and where numbers may have lost what sets them apart the one behind them.  (The low bits of 16-bit logits
+    // are empty.)  Lane r keeps the r-th.
+    const bool exact = by_logit && sizeof(T) == 2;
+    const int rounds = exact ? p.k : p.k + 1;
+    uint32_t my_key = 0, behind = 0;     // `behind`: the one that comes (k + 1)-th, of which lane 32 would have to know
+    int mine = -1;
+    for (int r = 0; r < rounds; ++r) {
+      const uint32_t head = key[0] & ~WHICH;
+      const uint32_t m = __reduce_max_sync(0xffffffffu, head);
+      const int from = __ffs(__ballot_sync(0xffffffffu, head == m)) - 1;
+      const uint32_t taken = __shfl_sync(0xffffffffu, key[0], from);
+      if (lane == r) {
+        my_key = m;
+        mine = from * VPL + (int)(WHICH - (taken & WHICH));
+      }
+      behind = m;
+      if (lane == from) {
 #pragma unroll
-      for (int j = 0; j + 1 < VPL; ++j) key[j] = key[j + 1];
-      key[VPL - 1] = 0;
+        for (int j = 0; j + 1 < VPL; ++j) key[j] = key[j + 1];
+        key[VPL - 1] = 0;
+      }
     }
-  }
-  if (near) {
+    if (my_key == 0 || lane >= p.k) mine = -1;
+    if (!exact) {
+      uint32_t next = __shfl_down_sync(0xffffffffu, my_key, 1);
+      if (lane == p.k - 1) next = behind;
+      const float a = from_ordered(my_key), b = from_ordered(next);
+      const bool mine_near = lane < p.k && next != 0 && (by_logit ? my_key == next : too_near(a, b, tolerance, fmaxf(fabsf(a), fabsf(b))));
+      near |= __any_sync(0xffffffffu, mine_near);
+    }
+    if (near) {
 #pragma unroll
-    for (int j = 0; j < VPL; ++j)
-      if (e0 + j < p.E) row[e0 + j] = l[j];
-    __syncwarp();
-    mine = choose(p, row, value, lane);
-  }
-  // the weights, lane j the j-th: softmax over all experts, or without its common factor where the sum divides it out; sigmoid
-  // times e^-m for m = min(0, largest chosen logit), which cannot underflow as a whole
-  const float chosen = mine >= 0 ? finite_logit(to_float(src[mine])) : -CUDART_INF_F;
-  float w = 0.0f;
-  if (p.sigmoid) {
-    const float m = p.renormalise ? fminf(0.0f, warp_max(chosen)) : 0.0f;
-    if (mine >= 0) w = 1.0f / (expf(m) + expf(m - chosen));
-  } else {
-    if (p.renormalise) top = warp_max(chosen);
-    if (mine >= 0) w = expf(chosen - top);
-    if (!p.renormalise && mine >= 0) w /= total;
-  }
-  if (p.renormalise) {
-    const float sum = warp_sum(w);
-    if (mine >= 0) w /= sum;
-  }
-  if (lane < p.k) {
-    p.ids[t * p.k + lane] = mine;
-    p.weights[t * p.k + lane] = w * p.scale;
+      for (int j = 0; j < VPL; ++j)
+        if (e0 + j < p.E) row[e0 + j] = l[j];
+      __syncwarp();
+      mine = choose(p, row, value, lane);
+      __syncwarp();
+    }
+    // the weights, lane j the j-th: softmax over all experts, or without its common factor where the sum divides it out; sigmoid
+    // times e^-m for m = min(0, largest chosen logit), which cannot underflow as a whole
+    const float chosen = mine >= 0 ? finite_logit(to_float(static_cast<const T*>(logits)[t * p.ld + mine])) : -CUDART_INF_F;
+    float w = 0.0f;
+    if (p.sigmoid) {
+      const float m = p.renormalise ? fminf(0.0f, warp_max(chosen)) : 0.0f;
+      if (mine >= 0) w = 1.0f / (expf(m) + expf(m - chosen));
+    } else {
+      if (p.renormalise) top = warp_max(chosen);
+      if (mine >= 0) w = expf(chosen - top);
+      if (!p.renormalise && mine >= 0) w /= total;
+    }
+    if (p.renormalise) {
+      const float sum = warp_sum(w);
+      if (mine >= 0) w /= sum;
+    }
+    if (lane < p.k) {
+      p.ids[t * p.k + lane] = mine;
+      p.weights[t * p.k + lane] = w * p.scale;
+    }
   }
 }
 
@@ -372,7 +389,8 @@ int launch_route(const void* logits, RouteParams p, cudaStream_t st) {
     const int lanes = p.group_size / VPL;                                                                                 \
     p.lanes_per_group = p.group_size % VPL == 0 && (lanes & (lanes - 1)) == 0 && lanes * p.groups <= 32 ? lanes : 0;      \
     if (smem > 48 * 1024) MQ_CUDA(cudaFuncSetAttribute(route_kernel<DT, VPL>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)); \
-    MQ_CUDA(launch_chained(true, route_kernel<DT, VPL>, dim3((unsigned)ceil_div(p.T, ROUTE_WARPS)), dim3(ROUTE_WARPS * 32), smem, st, logits, p)); \
+    const int64_t blocks = ceil_div(p.T, ROUTE_WARPS), most = 148 * route_blocks(VPL);                                    \
+    MQ_CUDA(launch_chained(true, route_kernel<DT, VPL>, dim3((unsigned)(blocks < most ? blocks : most)), dim3(ROUTE_WARPS * 32), smem, st, logits, p)); \
   } while (0)
   if (p.E <= 32) MQ_ROUTE(1);
   else if (p.E <= 64) MQ_ROUTE(2);
