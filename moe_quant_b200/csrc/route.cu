@@ -16,7 +16,7 @@
 namespace mq {
 namespace {
 
-constexpr int ROUTE_WARPS = 8;
+constexpr int ROUTE_WARPS = 8, EXTRA = 4;
 
 struct RouteParams {
   int64_t T, ld;
@@ -43,85 +43,107 @@ __device__ __forceinline__ F warp_max(F v) {
   for (int o = 16; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
   return v;
 }
-// the larger value, the lower index of equals; all lanes get it
-__device__ __forceinline__ void warp_argmax(double& v, int& i) {
-  for (int o = 16; o > 0; o >>= 1) {
-    const double u = __shfl_xor_sync(0xffffffffu, v, o);
-    const int j = __shfl_xor_sync(0xffffffffu, i, o);
-    if (u > v || (u == v && j < i)) {
-      v = u;
-      i = j;
-    }
-  }
+__device__ __forceinline__ uint64_t ordered64(double v) {
+  const int64_t b = __double_as_longlong(v);
+  return (uint64_t)(b ^ ((b >> 63) | (int64_t)0x8000000000000000ull));
 }
 
-// The choice in 64 bits.  `row` holds the token's logits (finite_logit), `value` is scratch of E doubles, both of this warp.
-// Lane j < k gets the j-th expert, or -1.
-__device__ int choose(const RouteParams& p, const float* row, double* value, int lane) {
+// The choice in 64 bits, for one token.  `row` holds its logits (finite_logit), `value` is scratch of E doubles, both of this warp.
+// Lane j < k gets the j-th expert, or -1.  Out of line: few tokens come here.
+template <int VPL>
+__device__ __noinline__ int choose(const RouteParams& p, const float* row, double* value, int lane) {
   const bool by_logit = p.bias == nullptr;   // sigmoid and softmax are increasing
-  double top = -CUDART_INF, total = 0.0;
   const bool by_score = !by_logit || (p.groups > 1 && p.top2);
-  if (!p.sigmoid && by_score) {
-    for (int e = lane; e < p.E; e += 32) top = max(top, (double)row[e]);
-    top = warp_max(top);
-    for (int e = lane; e < p.E; e += 32)
-      if (row[e] > -CUDART_INF_F) total += exp((double)row[e] - top);
-    total = warp_sum(total);
-  }
-  for (int e = lane; e < p.E; e += 32) {
-    const double l = row[e];
-    double v = -CUDART_INF;
-    if (row[e] > -CUDART_INF_F) {
-      if (!by_score) v = l;
-      else v = p.sigmoid ? 1.0 / (1.0 + exp(-l)) : exp(l - top) / total;
-      if (!by_logit) v += (double)p.bias[e];
-      if (v != v) v = -CUDART_INF;
+  const int e0 = lane * VPL;
+  double v[VPL];
+#pragma unroll
+  for (int j = 0; j < VPL; ++j) v[j] = e0 + j < p.E ? (double)row[e0 + j] : -CUDART_INF;
+  if (by_score) {
+    double top = 0.0, total = 1.0;
+    if (!p.sigmoid) {
+      top = v[0];
+#pragma unroll
+      for (int j = 1; j < VPL; ++j) top = max(top, v[j]);
+      top = warp_max(top);
+      total = 0.0;
+#pragma unroll 1
+      for (int j = 0; j < VPL; ++j) total += e0 + j < p.E && row[e0 + j] > -CUDART_INF_F ? exp((double)row[e0 + j] - top) : 0.0;
+      total = warp_sum(total);
     }
-    value[e] = v;
+#pragma unroll 4
+    for (int j = 0; j < VPL; ++j) {
+      const double e = exp(p.sigmoid ? -v[j] : v[j] - top);
+      double s = p.sigmoid ? 1.0 / (1.0 + e) : e / total;
+      if (!by_logit && e0 + j < p.E) s += (double)p.bias[e0 + j];
+      v[j] = v[j] > -CUDART_INF && s == s ? s : -CUDART_INF;
+    }
   }
-  __syncwarp();
   if (p.groups > 1) {
-    double of_group = -CUDART_INF;   // of group `lane`
-    if (lane < p.groups) {
-      double second = -CUDART_INF;
-      for (int i = 0; i < p.group_size; ++i) {
-        const double v = value[lane * p.group_size + i];
-        if (v > of_group) {
-          second = of_group;
-          of_group = v;
-        } else if (v > second) {
-          second = v;
-        }
+    __syncwarp();
+#pragma unroll
+    for (int j = 0; j < VPL; ++j)
+      if (e0 + j < p.E) value[e0 + j] = v[j];
+    __syncwarp();
+    // as many lanes as there are to a group, a power of two of them
+    int share = 1;
+    while (2 * share * p.groups <= 32) share *= 2;
+    const int group = lane / share;
+    double a = -CUDART_INF, b = -CUDART_INF;
+    if (group < p.groups)
+      for (int i = lane % share; i < p.group_size; i += share) {
+        const double u = value[group * p.group_size + i];
+        b = max(b, min(a, u));
+        a = max(a, u);
       }
-      if (p.top2 && second > -CUDART_INF) of_group += second;
+    for (int o = 1; o < share; o <<= 1) {
+      const double a2 = __shfl_xor_sync(0xffffffffu, a, o), b2 = __shfl_xor_sync(0xffffffffu, b, o);
+      b = max(min(a, a2), max(b, b2));
+      a = max(a, a2);
     }
+    const double mine = p.top2 && b > -CUDART_INF ? a + b : a;
     int better = 0;
     for (int g = 0; g < p.groups; ++g) {
-      const double u = __shfl_sync(0xffffffffu, of_group, g);
-      better += u > of_group || (u == of_group && g < lane);
+      const double u = __shfl_sync(0xffffffffu, mine, g * share);
+      better += u > mine || (u == mine && g < group);
     }
-    const unsigned kept = __ballot_sync(0xffffffffu, lane < p.groups && better < p.keep);
-    __syncwarp();
-    for (int e = lane; e < p.E; e += 32) {
-      if (!(kept >> (e / p.group_size) & 1u)) value[e] = -CUDART_INF;
-      else if (by_logit) value[e] = row[e];
+    const unsigned lanes = __ballot_sync(0xffffffffu, group < p.groups && better < p.keep);
+#pragma unroll
+    for (int j = 0; j < VPL; ++j) {
+      if (e0 + j >= p.E) continue;
+      if (!(lanes >> ((e0 + j) / p.group_size * share) & 1u)) v[j] = -CUDART_INF;
+      else if (by_logit) v[j] = row[e0 + j];
     }
-    __syncwarp();
+  }
+  uint64_t key[VPL], largest = 0;
+#pragma unroll
+  for (int j = 0; j < VPL; ++j) {
+    key[j] = v[j] > -CUDART_INF ? ordered64(v[j]) : 0ull;
+    largest = max(largest, key[j]);
   }
   int mine = -1;
   for (int r = 0; r < p.k; ++r) {
-    double v = -CUDART_INF;
-    int at = p.E;
-    for (int e = lane; e < p.E; e += 32)
-      if (value[e] > v) {
-        v = value[e];
-        at = e;
+    const uint32_t high = __reduce_max_sync(0xffffffffu, (uint32_t)(largest >> 32));
+    const bool with_high = (uint32_t)(largest >> 32) == high;
+    const uint32_t low = __reduce_max_sync(0xffffffffu, with_high ? (uint32_t)largest : 0u);
+    if ((high | low) == 0) break;
+    const int from = __ffs(__ballot_sync(0xffffffffu, with_high && (uint32_t)largest == low)) - 1;
+    int j_of = 0;
+    if (lane == from) {
+      const uint64_t taken = largest;
+      bool done = false;
+      largest = 0;
+#pragma unroll
+      for (int j = 0; j < VPL; ++j) {
+        if (!done && key[j] == taken) {
+          done = true;
+          j_of = j;
+          key[j] = 0;
+        }
+        largest = max(largest, key[j]);
       }
-    warp_argmax(v, at);
-    if (!(v > -CUDART_INF)) break;
-    if (lane == r) mine = at;
-    if (lane == 0) value[at] = -CUDART_INF;
-    __syncwarp();
+    }
+    j_of = __shfl_sync(0xffffffffu, j_of, from);
+    if (lane == r) mine = from * VPL + j_of;
   }
   return mine;
 }
@@ -171,7 +193,7 @@ __device__ __forceinline__ void sort_descending(uint32_t (&k)[N]) {
 
 // VPL experts per lane: VPL lane .. VPL lane + VPL - 1.  A warp takes every so many tokens; its next token's logits are on their way while it
 // chooses.  Instructions bound it: about 700 a token at 256 experts, 8 groups and a choice of 8.
-constexpr int route_blocks(int vpl) { return vpl <= 4 ? 5 : vpl <= 8 ? 3 : vpl <= 16 ? 2 : 1; }   // per SM
+constexpr int route_blocks(int vpl) { return vpl <= 4 ? 5 : vpl <= 8 ? 4 : vpl <= 16 ? 2 : 1; }   // per SM
 
 template <int DT, int VPL>
 __global__ void __launch_bounds__(ROUTE_WARPS * 32, route_blocks(VPL)) route_kernel(const void* __restrict__ logits, const RouteParams p) {
@@ -187,7 +209,12 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32, route_blocks(VPL)) route_ker
   const bool by_sum = p.groups > 1 && p.top2;
   const bool by_score = !by_logit || by_sum;
   const float tolerance = !p.sigmoid ? 2e-5f : VPL <= 8 ? 4e-6f : 1e-5f;
-  const int64_t stride = (int64_t)gridDim.x * ROUTE_WARPS;
+  // a block's tokens go to whichever of its warps is free: one that is in doubt about a token takes several times as long
+  const int64_t begin = p.T / gridDim.x * blockIdx.x + min((int64_t)blockIdx.x, p.T % gridDim.x);
+  const int64_t end = begin + p.T / gridDim.x + (blockIdx.x < p.T % gridDim.x);
+  __shared__ int handed_out;
+  if (threadIdx.x == 0) handed_out = ROUTE_WARPS;
+  __syncthreads();
   chain_wait();
   chain_release();
 
@@ -209,13 +236,16 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32, route_blocks(VPL)) route_ker
 #pragma unroll
   for (int j = 0; j < VPL; ++j) bias[j] = by_logit || e0 + j >= p.E ? 0.0f : fmaxf(p.bias[e0 + j], -CUDART_INF_F);   // NaN is -inf
 
-  int64_t t = (int64_t)blockIdx.x * ROUTE_WARPS + warp;
-  if (t < p.T) load(t);
-  for (; t < p.T; t += stride) {
+  int64_t t = begin + warp, t_next = 0;
+  if (t < end) load(t);
+  for (; t < end; t = t_next) {
+    int number = 0;
+    if (lane == 0) number = atomicAdd(&handed_out, 1);
+    t_next = begin + __shfl_sync(0xffffffffu, number, 0);
     float l[VPL];
 #pragma unroll
     for (int j = 0; j < VPL; ++j) l[j] = e0 + j < p.E ? finite_logit(to_float(raw[j / WORD].v[j % WORD])) : -CUDART_INF_F;
-    if (t + stride < p.T) load(t + stride);
+    if (t_next < end) load(t_next);
 
     // softmax: its largest logit and sum, where scores are needed
     float top = 0.0f, total = 1.0f;
@@ -321,41 +351,78 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32, route_blocks(VPL)) route_ker
     // The k largest, one by one, and where numbers may have lost what sets them apart the one behind them.  (The low bits of 16-bit logits
     // are empty.)  Lane r keeps the r-th.
     const bool exact = by_logit && sizeof(T) == 2;
-    const int rounds = exact ? p.k : p.k + 1;
-    uint32_t my_key = 0, behind = 0;     // `behind`: the one that comes (k + 1)-th, of which lane 32 would have to know
+    uint32_t my_key = 0, last = 0;     // `last`: of the last round
     int mine = -1;
-    for (int r = 0; r < rounds; ++r) {
+    auto take = [&](int r) {
       const uint32_t head = key[0] & ~WHICH;
       const uint32_t m = __reduce_max_sync(0xffffffffu, head);
       const int from = __ffs(__ballot_sync(0xffffffffu, head == m)) - 1;
       const uint32_t taken = __shfl_sync(0xffffffffu, key[0], from);
       if (lane == r) {
         my_key = m;
-        mine = from * VPL + (int)(WHICH - (taken & WHICH));
+        mine = m ? from * VPL + (int)(WHICH - (taken & WHICH)) : -1;
       }
-      behind = m;
+      last = m;
       if (lane == from) {
 #pragma unroll
         for (int j = 0; j + 1 < VPL; ++j) key[j] = key[j + 1];
         key[VPL - 1] = 0;
       }
-    }
-    if (my_key == 0 || lane >= p.k) mine = -1;
+    };
+    auto apart = [&](uint32_t ka, uint32_t kb) {     // whether ka is larger for sure
+      if (by_logit) return ka != kb;
+      const float a = from_ordered(ka), b = from_ordered(kb);
+      return !too_near(a, b, tolerance, fmaxf(fabsf(a), fabsf(b)));
+    };
+#pragma unroll 4
+    for (int r = 0; r < p.k + (exact ? 0 : 1); ++r) take(r);
     if (!exact) {
       uint32_t next = __shfl_down_sync(0xffffffffu, my_key, 1);
-      if (lane == p.k - 1) next = behind;
-      const float a = from_ordered(my_key), b = from_ordered(next);
-      const bool mine_near = lane < p.k && next != 0 && (by_logit ? my_key == next : too_near(a, b, tolerance, fmaxf(fabsf(a), fabsf(b))));
-      near |= __any_sync(0xffffffffu, mine_near);
-    }
-    if (near) {
+      if (lane == p.k - 1) next = last;     // (lane 32 of k = 32)
+      const bool in_doubt = __any_sync(0xffffffffu, lane < p.k && next != 0 && !apart(my_key, next));
+      if (near || in_doubt) {
+        // A few more, as far as these have surely left the k-th behind: then the choice is among them, and a lane each finds their values in
+        // 64 bits.  Otherwise (or where a group or a softmax's sum is in doubt) all of the token's values are formed anew.
+        const int n = p.k + EXTRA;
+        bool among = !near && (by_logit || p.sigmoid) && n <= 32;
+        if (among) {
+#pragma unroll 1
+          for (int r = p.k + 1; r < n; ++r) take(r);
+          among = last == 0 || apart(__shfl_sync(0xffffffffu, my_key, p.k - 1), last);
+        }
+        if (among) {
+          double d = -CUDART_INF;
+          if (mine >= 0) {
+            d = finite_logit(to_float(static_cast<const T*>(logits)[t * p.ld + mine]));
+            if (!by_logit) d = 1.0 / (1.0 + exp(-d)) + (double)p.bias[mine];
+          }
+          int rank = 0;
+#pragma unroll 1
+          for (int c = 0; c < n; ++c) {
+            const double u = __shfl_sync(0xffffffffu, d, c);
+            const int i = __shfl_sync(0xffffffffu, mine, c);
+            rank += u > d || (u == d && i < mine);
+          }
+          if (mine < 0) rank = 32;
+          const int found = mine;
+          mine = -1;
+#pragma unroll 1
+          for (int c = 0; c < p.k; ++c) {
+            const unsigned who = __ballot_sync(0xffffffffu, rank == c);
+            const int i = __shfl_sync(0xffffffffu, found, who ? __ffs(who) - 1 : 0);
+            if (lane == c && who) mine = i;
+          }
+        } else {
 #pragma unroll
-      for (int j = 0; j < VPL; ++j)
-        if (e0 + j < p.E) row[e0 + j] = l[j];
-      __syncwarp();
-      mine = choose(p, row, value, lane);
-      __syncwarp();
+          for (int j = 0; j < VPL; ++j)
+            if (e0 + j < p.E) row[e0 + j] = l[j];
+          __syncwarp();
+          mine = choose<VPL>(p, row, value, lane);
+          __syncwarp();
+        }
+      }
     }
+    if (lane >= p.k) mine = -1;
     // the weights, lane j the j-th: softmax over all experts, or without its common factor where the sum divides it out; sigmoid
     // times e^-m for m = min(0, largest chosen logit), which cannot underflow as a whole
     const float chosen = mine >= 0 ? finite_logit(to_float(static_cast<const T*>(logits)[t * p.ld + mine])) : -CUDART_INF_F;
@@ -407,7 +474,7 @@ int launch_route(const void* logits, RouteParams p, cudaStream_t st) {
 // A stable counting sort of the pairs by expert.  Every block takes a run of pairs; the first kernel counts them by expert, the
 // second adds up the blocks in front and ranks its own.  Within a block each warp takes a run of its own, 32 pairs at a
 // time; equal experts among the 32 are ranked by a match.
-constexpr int PLAN_THREADS = 512, PLAN_WARPS = PLAN_THREADS / 32, PLAN_KEEP = 8;
+constexpr int PLAN_THREADS = 512, PLAN_WARPS = PLAN_THREADS / 32, PLAN_KEEP = 8, PLAN_BLOCKS = 148;
 
 struct PlanParams {
   const int32_t* ids;
@@ -431,9 +498,13 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_count_kernel(const PlanPara
   chain_wait();
   chain_release();
   const int64_t begin = (int64_t)blockIdx.x * p.run, end = min(begin + p.run, p.pairs);
-  for (int64_t i = begin + threadIdx.x; i < end; i += PLAN_THREADS) {
-    const int e = expert_of(p, i, end);
-    if (e >= 0) atomicAdd(&plan_smem[e], 1);
+  for (int64_t i0 = begin + threadIdx.x; i0 < end; i0 += PLAN_THREADS * PLAN_KEEP) {
+    int e[PLAN_KEEP];
+#pragma unroll
+    for (int i = 0; i < PLAN_KEEP; ++i) e[i] = expert_of(p, i0 + i * PLAN_THREADS, end);
+#pragma unroll
+    for (int i = 0; i < PLAN_KEEP; ++i)
+      if (e[i] >= 0) atomicAdd(&plan_smem[e[i]], 1);
   }
   __syncthreads();
   for (int e = threadIdx.x; e < p.E; e += PLAN_THREADS) p.counts[(int64_t)blockIdx.x * p.E + e] = plan_smem[e];
@@ -460,11 +531,17 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_place_kernel(const PlanPara
       const int e = e0 + lane;
       int total = 0, before = 0;
       if (e < p.E) {
-#pragma unroll 10
-        for (int b = warp; b < (int)gridDim.x; b += PLAN_WARPS) {
-          const int c = __ldcg(p.counts + (int64_t)b * p.E + e);
-          total += c;
-          before += b < (int)blockIdx.x ? c : 0;
+        constexpr int SHARE = (PLAN_BLOCKS + PLAN_WARPS - 1) / PLAN_WARPS;
+        int c[SHARE];
+#pragma unroll
+        for (int i = 0; i < SHARE; ++i) {
+          const int b = warp + i * PLAN_WARPS;
+          c[i] = b < (int)gridDim.x ? __ldcg(p.counts + (int64_t)b * p.E + e) : 0;
+        }
+#pragma unroll
+        for (int i = 0; i < SHARE; ++i) {
+          total += c[i];
+          before += warp + i * PLAN_WARPS < (int)blockIdx.x ? c[i] : 0;
         }
         atomicAdd(&totals[e], total);
         atomicAdd(&befores[e], before);
@@ -552,7 +629,7 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_place_kernel(const PlanPara
 int plan_blocks(int64_t pairs) {
   const int64_t run = 32 * PLAN_WARPS;
   const int64_t b = ceil_div(pairs, 4 * run);
-  return (int)(b < 1 ? 1 : b > 148 ? 148 : b);
+  return (int)(b < 1 ? 1 : b > PLAN_BLOCKS ? PLAN_BLOCKS : b);
 }
 
 }  // namespace
