@@ -232,10 +232,21 @@ extern "C" int mq_quantize_tokens(const void* x, int dtype, int64_t T, int64_t K
   return quantize_rows(dtype, RowsParams{x, ldx, T, nullptr, nullptr, 0, (int)K, codes, ldc, scale}, static_cast<cudaStream_t>(stream));
 }
 
+namespace mq {
+namespace {
+Int8Product dense_product(int64_t T, int64_t N, int64_t K) {
+  Int8Product p = {};
+  p.E = 1; p.rows = (int)N; p.K = (int)K; p.T = T;
+  p.x_rows = T;
+  return p;
+}
+}  // namespace
+}  // namespace mq
+
 extern "C" size_t mq_int8_matmul_workspace_bytes(int x_dtype, int64_t T, int64_t N, int64_t K) {
-  (void)N;
-  if (x_dtype == MQ_I8 || int8_few_fits(T, K)) return 0;
-  return align_up((size_t)T * (size_t)pitch_of(K), 256) + align_up((size_t)T * 4, 256);
+  if (T <= 0 || N <= 0 || K <= 0 || K > INT8_MAX_K || T >= (1ll << 31) - 256 || N >= (1ll << 31) - 256 || int8_few_fits(T, K)) return 0;
+  const size_t codes = x_dtype == MQ_I8 ? 0 : align_up((size_t)T * (size_t)pitch_of(K), 256) + align_up((size_t)T * 4, 256);
+  return codes + align_up(int8_umma_scratch_bytes(dense_product(T, N, K), INT8_Y), 256);
 }
 
 extern "C" int mq_int8_matmul(const void* x, int x_dtype, const float* x_scale, int64_t T, int64_t K, int64_t ldx, const int8_t* w, int64_t N,
@@ -257,18 +268,18 @@ extern "C" int mq_int8_matmul(const void* x, int x_dtype, const float* x_scale, 
   const size_t need = mq_int8_matmul_workspace_bytes(x_dtype, T, N, K);
   MQ_REQUIRE(need == 0 || (workspace && aligned(workspace, 16) && workspace_bytes >= need), MQ_ERR_WORKSPACE,
              "mq_int8_matmul: the workspace has %zu bytes and needs %zu", workspace_bytes, need);
-  Int8Product p = {};
+  Int8Product p = dense_product(T, N, K);
   p.x_scale = x_scale;
-  p.w = w; p.ldw = ldw; p.w_expert = 0; p.w_scale = w_scale;
-  p.E = 1; p.rows = (int)N; p.K = (int)K; p.T = T;
-  p.x_rows = T;
+  p.w = w; p.ldw = ldw; p.w_scale = w_scale;
   const Int8Out o = {INT8_Y, out_dtype, y, ldy, bias, nullptr};
   if (int8_few_fits(T, K)) return int8_few(x, x_dtype, ldx, p, o, st);
+  Workspace ws(workspace, workspace_bytes);
+  const size_t n_sums = int8_umma_scratch_bytes(p, INT8_Y);
+  char* sums = n_sums ? ws.take<char>(n_sums) : nullptr;
   if (x_dtype == MQ_I8) {
     p.x = static_cast<const int8_t*>(x);
     p.ldx = ldx;
   } else {
-    Workspace ws(workspace, workspace_bytes);
     int8_t* codes = ws.take<int8_t>((size_t)T * pitch_of(K));
     float* scale = ws.take<float>((size_t)T);
     MQ_TRY(quantize_rows(x_dtype, RowsParams{x, ldx, T, nullptr, nullptr, 0, (int)K, codes, pitch_of(K), scale}, st));
@@ -276,7 +287,7 @@ extern "C" int mq_int8_matmul(const void* x, int x_dtype, const float* x_scale, 
     p.ldx = pitch_of(K);
     p.x_scale = scale;
   }
-  return int8_product_umma(p, o, st);
+  return int8_product_umma(p, o, sums, st);
 }
 
 namespace mq {
@@ -365,10 +376,10 @@ extern "C" int mq_int8_experts(const void* x, int dtype, int64_t T, int64_t K, i
   // the tokens' codes, once for each of their pairs, where the plan has them
   MQ_TRY(quantize_rows(dtype, RowsParams{x, ldx, T, nullptr, b.place, top_k, (int)K, b.x_codes, pitch_of(K), b.x_scale}, st));
   up.x = b.x_codes; up.ldx = pitch_of(K); up.x_rows = P; up.x_scale = b.x_scale; up.offsets = b.offsets;
-  MQ_TRY(int8_product_umma(up, Int8Out{INT8_GATED, MQ_F32, b.h, pitch_of(I), nullptr, nullptr}, st));
+  MQ_TRY(int8_product_umma(up, Int8Out{INT8_GATED, MQ_F32, b.h, pitch_of(I), nullptr, nullptr}, nullptr, st));
   MQ_TRY(quantize_rows(MQ_F32, RowsParams{b.h, pitch_of(I), P, b.offsets + E, nullptr, 0, (int)I, b.h_codes, pitch_of(I), b.h_scale}, st));
   dn.x = b.h_codes; dn.ldx = pitch_of(I); dn.x_rows = P; dn.x_scale = b.h_scale; dn.offsets = b.offsets;
-  MQ_TRY(int8_product_umma(dn, Int8Out{INT8_PAIRS, MQ_F16, b.pairs, pitch_of(K), nullptr, b.power}, st));
+  MQ_TRY(int8_product_umma(dn, Int8Out{INT8_PAIRS, MQ_F16, b.pairs, pitch_of(K), nullptr, b.power}, nullptr, st));
   const CombineParams c = {b.pairs, pitch_of(K), b.power, b.h_scale, weights, b.place, ids, (int)first, top_k, (int)K, (int)ceil_div(K, 32), T, y, ldy};
   return dtype == MQ_BF16 ? launch_combine<MQ_BF16>(c, st) : launch_combine<MQ_F16>(c, st);
 }

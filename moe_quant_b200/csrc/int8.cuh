@@ -32,6 +32,7 @@ enum Int8Result {
   // is off by 2^-25 of the power.  Half the bytes of fp32; the sum over a token's pairs and the result's own rounding
   // (2^-8, 2^-11) come after it.
   INT8_PAIRS = 2,
+  INT8_SUMS = 3,   // the sums themselves, of a share of k (within int8_umma.cu)
 };
 
 struct Int8Out {
@@ -42,7 +43,10 @@ struct Int8Out {
   float* power;    // INT8_PAIRS: (E, ceil(rows / 32)), written by the product
 };
 
-int int8_product_umma(const Int8Product& p, const Int8Out& o, cudaStream_t st);   // on the tensor cores (int8_umma.cu)
+// On the tensor cores (int8_umma.cu).  `scratch`: int8_umma_scratch_bytes bytes on a 16-byte boundary, or NULL (then no tile's k is shared
+// among CTAs).
+size_t int8_umma_scratch_bytes(const Int8Product& p, int kind);
+int int8_product_umma(const Int8Product& p, const Int8Out& o, void* scratch, cudaStream_t st);
 
 // A few tokens (int8_few.cu): x of any type, codes made on the way (p.x is not read; p.x_scale for MQ_I8 alone).
 constexpr int64_t INT8_FEW_TOKENS = 4;

@@ -9,6 +9,9 @@
 //   warps 4 .. 11        : epilogue, a quarter of the CTA's weight rows each, chunks of 32 tokens by turns
 // Persistent: a pair of CTAs takes every 74th tile.  Eight tiles of weight rows at a time go with all tiles of tokens, so that the
 // SMs that run side by side share rows of either in the L2.
+// Where there are fewer tiles than pairs of CTAs, several take a share of k each (`splits`) and store their sums as integers; a second kernel
+// on all SMs adds these up and does what the epilogue does.  (Adding them up in place by atomics, with the last CTA to arrive
+// doing the epilogue, took 39 us for 512 tokens through 2048 x 7168, where unshared tiles take 27.)
 #include "int8.cuh"
 #include "profile.cuh"
 #include "umma_pair.cuh"
@@ -28,6 +31,9 @@ struct PairArgs {
   int max_width, m_tiles;
   int sum_shift;   // INT8_PAIRS: 2^sum_shift brings the largest sum down to 2^15
   int packed;      // two neighbouring results of a token are stored together
+  int splits;      // CTA pairs that share a tile's k
+  int* sums;       // INT8_SUMS: (splits, T, ld_sums)
+  int64_t ld_sums;
   int* fault;
 };
 
@@ -68,11 +74,22 @@ __device__ __forceinline__ void tmem_ld32_int(uint32_t taddr, int (&r)[32]) {
 __host__ __device__ __forceinline__ int token_tiles(int64_t count, int max_width) { return (int)((count + max_width - 1) / max_width); }
 __host__ __device__ __forceinline__ int tile_width(int64_t count, int tiles) { return (int)((((count + tiles - 1) / tiles) + 31) / 32 * 32); }
 
-// The tile that comes `unit`-th: which expert, which weight rows, which of its tokens.
+// The tile that comes `unit`-th: which expert, which weight rows, which of its tokens, which share of k.
 struct Unit {
   int e, m, width;
+  int share, slab0, slab1;
   int t0, t_end;     // rows of the result
   __device__ __forceinline__ bool seek(int64_t unit, const PairArgs& a, const int* offsets, const int* tiles_before) {
+    const int slabs = (a.p.K + I8_K - 1) / I8_K;
+    share = 0;
+    slab0 = 0;
+    slab1 = slabs;
+    if (a.splits > 1) {
+      share = (int)(unit % a.splits);
+      unit /= a.splits;
+      slab0 = slabs * share / a.splits;
+      slab1 = slabs * (share + 1) / a.splits;
+    }
     if (unit >= (int64_t)tiles_before[a.p.E] * a.m_tiles) return false;
     int lo = 0, hi = a.p.E;      // the last expert whose tiles begin at or in front of this one
     while (hi - lo > 1) {
@@ -102,7 +119,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
   constexpr int TILE_ROWS = 256 / SETS;            // result columns of a tile
   const Int8Product& p = a.p;
   const int rank = (int)(blockIdx.x & 1), pair = (int)(blockIdx.x >> 1), n_pairs = (int)(gridDim.x >> 1);
-  const int slabs = (p.K + I8_K - 1) / I8_K;
 
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
@@ -166,7 +182,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
       const int b_row = u.t0 + rank * half;
       const int n_boxes = (half + 31) / 32;
       const uint32_t bytes = 2 * (I8_TILE_BYTES + (uint32_t)n_boxes * 32 * I8_K);
-      for (int s = 0; s < slabs; ++s, ++it) {
+      for (int s = u.slab0; s < u.slab1; ++s, ++it) {
         const int st = it % I8_STAGES;
         if (it >= I8_STAGES && !mbar_wait(empty0 + 8 * st, ((it / I8_STAGES) - 1) & 1, a.fault, 91)) { ok = false; break; }
         const uint32_t dst = smem_base + (uint32_t)st * I8_STAGE_BYTES, bar = full_leader + 8 * st;
@@ -202,7 +218,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
         const uint32_t acc = tmem_acc + (uint32_t)(b * I8_MAX_WIDTH);
         if (n >= 2) ok = mbar_wait(acc_empty + 8 * b, ((n >> 1) - 1) & 1, a.fault, 93);
         tc_fence_after();
-        for (int s = 0; s < slabs && ok; ++s) {
+        for (int s = u.slab0; s < u.slab1 && ok; ++s) {
           const int st = it % I8_STAGES;
           ok = mbar_wait(full0 + 8 * st, (it / I8_STAGES) & 1, a.fault, 92);
           if (!ok) break;
@@ -212,9 +228,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
             const uint64_t a0 = kmajor_sw128_desc(a_tile), b0 = kmajor_sw128_desc(a_tile + I8_TILE_BYTES);
 #pragma unroll
             for (int kk = 0; kk < I8_K / 32; ++kk)
-              umma_i8_pair(acc, a0 + (uint64_t)((kk * 32) >> 4), b0 + (uint64_t)((kk * 32) >> 4), idesc, (s | kk) > 0 ? 1u : 0u);
+              umma_i8_pair(acc, a0 + (uint64_t)((kk * 32) >> 4), b0 + (uint64_t)((kk * 32) >> 4), idesc, s > u.slab0 || kk > 0 ? 1u : 0u);
             umma_commit_pair(empty0 + 8 * st);
-            if (s == slabs - 1) umma_commit_pair(acc_full + 8 * b);
+            if (s == u.slab1 - 1) umma_commit_pair(acc_full + 8 * b);
           }
           __syncwarp();
           ++it;
@@ -256,7 +272,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
       for (int i = 0; i < 4; ++i) {
         const int t = u.t0 + (2 * i + h) * 32 + lane;
         xs[i] = 0.0f;
-        if (2 * i + h < chunks && t < u.t_end) xs[i] = KIND == INT8_PAIRS ? 1.0f : __ldcg(p.x_scale + t);
+        if (2 * i + h < chunks && t < u.t_end) xs[i] = KIND == INT8_PAIRS || KIND == INT8_SUMS ? 1.0f : __ldcg(p.x_scale + t);
       }
       ok = mbar_wait(acc_full + 8 * b, (n >> 1) & 1, a.fault, 94);
       if (!ok) break;
@@ -267,10 +283,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
         if (c >= chunks) break;
         int r[32];
         tmem_ld32_int(t_lane + (uint32_t)(b * I8_MAX_WIDTH + c * 32), r);
+        const int t = u.t0 + c * 32, left = u.t_end - t;     // tokens of this chunk that exist
+        if constexpr (KIND == INT8_SUMS) {
+          int* out = a.sums + ((int64_t)u.share * p.T + t) * a.ld_sums + col;
+#pragma unroll
+          for (int j = 0; j < 32; ++j)
+            if (col_in && j < left) out[j * a.ld_sums] = r[j];
+          continue;
+        }
         __syncwarp();
         my_scale[lane] = xs[i];
         __syncwarp();
-        const int t = u.t0 + c * 32, left = u.t_end - t;     // tokens of this chunk that exist
         float v[32];
 #pragma unroll
         for (int j = 0; j < 32; j += 4) {
@@ -348,6 +371,38 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
   }
 }
 
+// y from the sums of `splits` shares of k: four results of a token a thread
+__global__ void __launch_bounds__(256) finish_kernel(const PairArgs a) {
+  const Int8Product& p = a.p;
+  chain_wait();
+  chain_release();
+  const int words = (int)(a.ld_sums >> 2);
+  const int64_t all = p.T * words;
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < all; i += (int64_t)gridDim.x * 256) {
+    const int64_t t = i / words;
+    const int n = (int)(i - t * words) * 4;
+    const int4* src = reinterpret_cast<const int4*>(a.sums + t * a.ld_sums + n);
+    int4 sum = make_int4(0, 0, 0, 0);
+#pragma unroll 4
+    for (int s = 0; s < a.splits; ++s) {
+      const int4 v = __ldcg(src + s * (p.T * words));
+      sum.x += v.x; sum.y += v.y; sum.z += v.z; sum.w += v.w;
+    }
+    const float xs = __ldcg(p.x_scale + t);
+    const int r[4] = {sum.x, sum.y, sum.z, sum.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (n + j >= p.rows) break;
+      float v = (float)r[j] * xs * __ldg(p.w_scale + n + j);
+      if (a.o.bias) v += __ldg(a.o.bias + n + j);
+      const int64_t at = t * a.o.ldy + n + j;
+      if (a.o.dtype == MQ_F32) static_cast<float*>(a.o.y)[at] = v;
+      else if (a.o.dtype == MQ_BF16) static_cast<__nv_bfloat16*>(a.o.y)[at] = __float2bfloat16_rn(v);
+      else static_cast<__half*>(a.o.y)[at] = __float2half_rn(v);
+    }
+  }
+}
+
 int encode(EncodeTiledFn enc, CUtensorMap* map, int rank, const void* base, const cuuint64_t* dims, const cuuint64_t* strides, const cuuint32_t* box) {
   const cuuint32_t ones[4] = {1, 1, 1, 1};
   const CUresult r = enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, (cuuint32_t)rank, const_cast<void*>(base), dims, strides, box, ones,
@@ -373,7 +428,46 @@ int launch(const CUtensorMap& map_w, const CUtensorMap& map_x, const PairArgs& a
 
 }  // namespace
 
-int int8_product_umma(const Int8Product& p, const Int8Out& o, cudaStream_t st) {
+namespace {
+// How wide a tile of tokens is at most and how many pairs of CTAs share its k, from what a tile costs (measured, us): a slab of 128 of k
+// 0.40 at 256 columns where the MMA bounds it, and 0.20 + 0.0008 a column where its 16 KB + 64 bytes a column bound it; about 4 beside
+// the slabs and 0.01 a column for the last epilogue; where k is shared, the second kernel and the sums' way through the L2.
+struct Shape {
+  int width, splits;
+};
+constexpr int I8_MOST_SPLITS = 16;
+Shape best_shape(int64_t rows_of_tiles, int64_t T, int slabs, bool shared) {
+  Shape best = {I8_MAX_WIDTH, 1};
+  double best_us = 1e30;
+  for (int width = I8_MAX_WIDTH; width >= 32; width -= 32) {
+    const int64_t n_tiles = token_tiles(T, width), tiles = rows_of_tiles * n_tiles;
+    const int w = tile_width(T, (int)n_tiles);
+    const double slab_us = 0.0016 * w > 0.2 + 0.0008 * w ? 0.0016 * w : 0.2 + 0.0008 * w;
+    const int fit = shared && tiles < I8_PAIRS ? (int)(I8_PAIRS / tiles) : 1;
+    for (int splits = 1; splits <= fit && splits <= I8_MOST_SPLITS && splits * 2 <= slabs; ++splits) {
+      const double us = (double)ceil_div(tiles * splits, I8_PAIRS) * (double)ceil_div(slabs, splits) * slab_us + 4.0 + 0.01 * w +
+                        (splits > 1 ? 2.5 + 8.0 * splits * (double)T * (double)rows_of_tiles * 256 / 4e6 : 0.0);
+      if (us < best_us * 0.98) {
+        best_us = us;
+        best = {width, splits};
+      }
+    }
+  }
+  return best;
+}
+int64_t row_tiles(const Int8Product& p, int kind) { return ceil_div(p.rows, kind == INT8_GATED ? 128 : 256); }
+Shape shape_of(const Int8Product& p, int kind, bool shared) {
+  if (p.offsets || kind != INT8_Y) return Shape{I8_MAX_WIDTH, 1};   // several experts, whose rows the host does not know
+  return best_shape(row_tiles(p, kind), p.T, (int)ceil_div(p.K, I8_K), shared);
+}
+}  // namespace
+
+size_t int8_umma_scratch_bytes(const Int8Product& p, int kind) {
+  const Shape s = shape_of(p, kind, true);
+  return s.splits == 1 ? 0 : (size_t)s.splits * (size_t)p.T * (size_t)align_up(p.rows, 4) * 4;
+}
+
+int int8_product_umma(const Int8Product& p, const Int8Out& o, void* scratch, cudaStream_t st) {
   EncodeTiledFn enc;
   MQ_TRY(get_encoder(&enc));
   PairArgs a = {};
@@ -395,10 +489,21 @@ int int8_product_umma(const Int8Product& p, const Int8Out& o, cudaStream_t st) {
     const cuuint32_t box[2] = {I8_K, 32};
     MQ_TRY(encode(enc, &map_x, 2, p.x, dims, strides, box));
   }
-  a.m_tiles = (int)ceil_div(p.rows, 256 / sets);
-  a.max_width = I8_MAX_WIDTH;
-  const int64_t most = (int64_t)a.m_tiles * (p.offsets ? ceil_div(p.T, a.max_width) + p.E : token_tiles(p.T, a.max_width));
+  a.m_tiles = (int)row_tiles(p, o.kind);
+  const Shape shape = shape_of(p, o.kind, scratch != nullptr);
+  a.max_width = shape.width;
+  a.splits = shape.splits;
+  a.sums = static_cast<int*>(scratch);
+  a.ld_sums = (int64_t)align_up(p.rows, 4);
+  const int64_t most = a.m_tiles * (ceil_div(p.T, a.max_width) + (p.offsets ? p.E : 0)) * a.splits;
   const int pairs = (int)(most < I8_PAIRS ? most : I8_PAIRS);
+  if (a.splits > 1) {
+    MQ_TRY(launch<INT8_SUMS>(map_w, map_x, a, pairs, st));
+    const int64_t blocks = ceil_div(p.T * (a.ld_sums >> 2), 256);
+    MQ_CUDA(launch_chained(true, finish_kernel, dim3((unsigned)(blocks < 148 * 8 ? blocks : 148 * 8)), dim3(256), 0, st, a));
+    MQ_LAUNCH_CHECK();
+    return MQ_OK;
+  }
   const size_t size = dtype_size(o.dtype);
   while ((int64_t)p.K > (2ll << a.sum_shift)) ++a.sum_shift;   // 127 * 128 * K / 2^shift < 2^14 K / 2^shift <= 2^15
   a.packed = p.rows % 2 == 0 && o.ldy % 2 == 0 && aligned(o.y, 2 * size);
