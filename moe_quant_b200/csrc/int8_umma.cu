@@ -4,7 +4,9 @@
 // The weights are the operand of 128 rows per CTA, the tokens the one of up to 256 columns, so a tile can be as narrow as the tokens
 // that there are (32 and up in steps of 32) while weights fill the tensor core.  Two CTAs of a cluster share a tile of 256 weight
 // rows (cta_group::2): each keeps 128 of them and half of the tokens, 32 KB per 128 of k instead of 48.
-//   warp 0 of either CTA : TMA, six stages of 32 KB; the bytes of both CTAs count on the leader's barrier
+//   warp 0 of either CTA : TMA, 192 KB of stages (six where tiles are 256 tokens wide, nine of 20 KB where they are up to 64: a load takes
+//                          about two microseconds from the wait for its stage to the end of its MMAs, and that many bytes must be under
+//                          way meanwhile); the bytes of both CTAs count on the leader's barrier
 //   warp 1 of the leader : tcgen05.mma for both SMs, two accumulators of 256 columns by turns
 //   warps 4 .. 11        : epilogue, a quarter of the CTA's weight rows each, chunks of 32 tokens by turns
 // Persistent: a pair of CTAs takes every 74th tile.  Eight tiles of weight rows at a time go with all tiles of tokens, so that the
@@ -19,17 +21,18 @@
 namespace mq {
 namespace {
 
-constexpr int I8_STAGES = 6, I8_THREADS = 384, I8_K = 128, I8_TILE_BYTES = 128 * I8_K, I8_MAX_WIDTH = 256, I8_ROW_GROUP = 8;
+constexpr int I8_MAX_STAGES = 9, I8_THREADS = 384, I8_K = 128, I8_TILE_BYTES = 128 * I8_K, I8_MAX_WIDTH = 256, I8_ROW_GROUP = 8;
 constexpr int I8_PAIRS = 74;
-constexpr uint32_t I8_STAGE_BYTES = 2 * I8_TILE_BYTES;
+constexpr int I8_RING_BYTES = 192 * 1024;
 constexpr int I8_MAX_EXPERTS = 1024;
-constexpr size_t kInt8Smem = (size_t)I8_STAGES * I8_STAGE_BYTES + 1024;
+constexpr size_t kInt8Smem = (size_t)I8_RING_BYTES + 1024;
 
 struct PairArgs {
   Int8Product p;
   Int8Out o;
   int max_width, m_tiles;
   int sum_shift;   // INT8_PAIRS: 2^sum_shift brings the largest sum down to 2^15
+  int stages, stage_bytes;
   int packed;      // two neighbouring results of a token are stored together
   int splits;      // CTA pairs that share a tile's k
   int* sums;       // INT8_SUMS: (splits, T, ld_sums)
@@ -122,16 +125,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
 
   extern __shared__ uint8_t smem_raw[];
   const uint32_t smem_base = (smem_u32(smem_raw) + 1023u) & ~1023u;
-  __shared__ __align__(8) uint64_t bars[2 * I8_STAGES + 4];
+  __shared__ __align__(8) uint64_t bars[2 * I8_MAX_STAGES + 4];
   __shared__ uint32_t tmem_slot;
   __shared__ PairEnd end;
   __shared__ int offsets[I8_MAX_EXPERTS + 1], tiles_before[I8_MAX_EXPERTS + 1];
   __shared__ __align__(16) float token_scale[8][32];
-  const uint32_t full0 = smem_u32(&bars[0]), empty0 = smem_u32(&bars[I8_STAGES]);
-  const uint32_t acc_full = smem_u32(&bars[2 * I8_STAGES]), acc_empty = smem_u32(&bars[2 * I8_STAGES + 2]);
+  const uint32_t full0 = smem_u32(&bars[0]), empty0 = smem_u32(&bars[I8_MAX_STAGES]);
+  const uint32_t acc_full = smem_u32(&bars[2 * I8_MAX_STAGES]), acc_empty = smem_u32(&bars[2 * I8_MAX_STAGES + 2]);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < I8_STAGES; ++s) {
+    for (int s = 0; s < a.stages; ++s) {
       mbar_init(full0 + 8 * s, 1);    // the leader's: its producer's arrival, then the bytes of both CTAs
       mbar_init(empty0 + 8 * s, 1);
     }
@@ -174,7 +177,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
 
   if (warp == 0) {
     const uint32_t full_leader = leader_addr(full0);
-    int it = 0;
+    int it = 0, st = 0;
+    uint32_t round = 0;
     bool ok = true;
     Unit u;
     for (int64_t unit = pair; ok && u.seek(unit, a, offsets, tiles_before); unit += n_pairs) {
@@ -183,9 +187,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
       const int n_boxes = (half + 31) / 32;
       const uint32_t bytes = 2 * (I8_TILE_BYTES + (uint32_t)n_boxes * 32 * I8_K);
       for (int s = u.slab0; s < u.slab1; ++s, ++it) {
-        const int st = it % I8_STAGES;
-        if (it >= I8_STAGES && !mbar_wait(empty0 + 8 * st, ((it / I8_STAGES) - 1) & 1, a.fault, 91)) { ok = false; break; }
-        const uint32_t dst = smem_base + (uint32_t)st * I8_STAGE_BYTES, bar = full_leader + 8 * st;
+        if (it >= a.stages && !mbar_wait(empty0 + 8 * st, (round - 1) & 1, a.fault, 91)) { ok = false; break; }
+        const uint32_t dst = smem_base + (uint32_t)(st * a.stage_bytes), bar = full_leader + 8 * st;
         if (lane == 0) {
           if (rank == 0) mbar_expect_tx(full0 + 8 * st, bytes);
           if constexpr (KIND == INT8_GATED) {
@@ -199,16 +202,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
           for (int j = 0; j < n_boxes; ++j) load_tokens_pair(dst + I8_TILE_BYTES + j * 32 * I8_K, &map_x, bar, s * I8_K, b_row + 32 * j);
         }
         __syncwarp();
+        if (++st == a.stages) {
+          st = 0;
+          ++round;
+        }
       }
     }
-    ok = PairEnd::await_stages<I8_STAGES>(empty0, it, ok, a.fault, 95);
+    ok = PairEnd::await_stages(a.stages, empty0, it, ok, a.fault, 95);
     if (lane == 0) {
       end.copied_by(rank, it);
       if (!ok) end.give_up();
     }
   } else if (warp == 1) {
     if (rank == 0) {
-      int it = 0, n = 0;
+      int it = 0, n = 0, st = 0;
+      uint32_t round = 0;
       bool ok = true;
       Unit u;
       for (int64_t unit = pair; ok && u.seek(unit, a, offsets, tiles_before); unit += n_pairs, ++n) {
@@ -219,12 +227,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
         if (n >= 2) ok = mbar_wait(acc_empty + 8 * b, ((n >> 1) - 1) & 1, a.fault, 93);
         tc_fence_after();
         for (int s = u.slab0; s < u.slab1 && ok; ++s) {
-          const int st = it % I8_STAGES;
-          ok = mbar_wait(full0 + 8 * st, (it / I8_STAGES) & 1, a.fault, 92);
+          ok = mbar_wait(full0 + 8 * st, round & 1, a.fault, 92);
           if (!ok) break;
           tc_fence_after();
           if (lane == 0) {
-            const uint32_t a_tile = smem_base + (uint32_t)st * I8_STAGE_BYTES;
+            const uint32_t a_tile = smem_base + (uint32_t)(st * a.stage_bytes);
             const uint64_t a0 = kmajor_sw128_desc(a_tile), b0 = kmajor_sw128_desc(a_tile + I8_TILE_BYTES);
 #pragma unroll
             for (int kk = 0; kk < I8_K / 32; ++kk)
@@ -234,6 +241,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
           }
           __syncwarp();
           ++it;
+          if (++st == a.stages) {
+            st = 0;
+            ++round;
+          }
         }
         if (!ok) break;
       }
@@ -361,7 +372,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
   __syncthreads();
   cluster_sync();   // neither CTA issues a copy, an MMA or an arrival any more
   if (end.given_up) {   // the same in both CTAs
-    if (warp == 0) end.drain<I8_STAGES>(rank, full0, empty0, acc_full);
+    if (warp == 0) end.drain(a.stages, rank, full0, empty0, acc_full);
     __syncthreads();
     cluster_sync();   // the other CTA's copies signal the leader's barriers
   }
@@ -442,7 +453,7 @@ Shape best_shape(int64_t rows_of_tiles, int64_t T, int slabs, bool shared) {
   for (int width = I8_MAX_WIDTH; width >= 32; width -= 32) {
     const int64_t n_tiles = token_tiles(T, width), tiles = rows_of_tiles * n_tiles;
     const int w = tile_width(T, (int)n_tiles);
-    const double slab_us = 0.0016 * w > 0.2 + 0.0008 * w ? 0.0016 * w : 0.2 + 0.0008 * w;
+    const double slab_us = 0.0016 * w > 0.17 + 0.0008 * w ? 0.0016 * w : 0.17 + 0.0008 * w;
     const int fit = shared && tiles < I8_PAIRS ? (int)(I8_PAIRS / tiles) : 1;
     for (int splits = 1; splits <= fit && splits <= I8_MOST_SPLITS && splits * 2 <= slabs; ++splits) {
       const double us = (double)ceil_div(tiles * splits, I8_PAIRS) * (double)ceil_div(slabs, splits) * slab_us + 4.0 + 0.01 * w +
@@ -457,7 +468,8 @@ Shape best_shape(int64_t rows_of_tiles, int64_t T, int slabs, bool shared) {
 }
 int64_t row_tiles(const Int8Product& p, int kind) { return ceil_div(p.rows, kind == INT8_GATED ? 128 : 256); }
 Shape shape_of(const Int8Product& p, int kind, bool shared) {
-  if (p.offsets || kind != INT8_Y) return Shape{I8_MAX_WIDTH, 1};   // several experts, whose rows the host does not know
+  // several experts, whose rows the host does not know: a tile need not be wider than there are rows
+  if (p.offsets || kind != INT8_Y) return Shape{p.T < I8_MAX_WIDTH ? tile_width(p.T, 1) : I8_MAX_WIDTH, 1};
   return best_shape(row_tiles(p, kind), p.T, (int)ceil_div(p.K, I8_K), shared);
 }
 }  // namespace
@@ -493,6 +505,8 @@ int int8_product_umma(const Int8Product& p, const Int8Out& o, void* scratch, cud
   const Shape shape = shape_of(p, o.kind, scratch != nullptr);
   a.max_width = shape.width;
   a.splits = shape.splits;
+  a.stage_bytes = I8_TILE_BYTES + (a.max_width / 2 + 31) / 32 * 32 * I8_K;
+  a.stages = I8_RING_BYTES / a.stage_bytes < I8_MAX_STAGES ? I8_RING_BYTES / a.stage_bytes : I8_MAX_STAGES;
   a.sums = static_cast<int*>(scratch);
   a.ld_sums = (int64_t)align_up(p.rows, 4);
   const int64_t most = a.m_tiles * (ceil_div(p.T, a.max_width) + (p.offsets ? p.E : 0)) * a.splits;

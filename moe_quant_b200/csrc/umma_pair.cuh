@@ -90,18 +90,24 @@ struct PairEnd {
   }
   __device__ __forceinline__ void copied_by(int rank, int slabs) { set_in_cta(&n_copied[rank], 0, slabs); }
   // by the producers' warps: the last use of every stage has been read (so its copies had landed) and its commit has arrived in this CTA
-  template <int NST>
-  static __device__ __forceinline__ bool await_stages(uint32_t empty0, int slabs, bool ok, int* fault, int code) {
-    for (int j = slabs > NST ? slabs - NST : 0; j < slabs && ok; ++j) ok = mbar_wait(empty0 + 8 * (j % NST), (j / NST) & 1, fault, code);
+  static __device__ __forceinline__ bool await_stages(int stages, uint32_t empty0, int slabs, bool ok, int* fault, int code) {
+    for (int j = slabs > stages ? slabs - stages : 0; j < slabs && ok; ++j) ok = mbar_wait(empty0 + 8 * (j % stages), (j / stages) & 1, fault, code);
     return ok;
   }
-  template <int NST>
-  __device__ __forceinline__ void drain(int rank, uint32_t full0, uint32_t empty0, uint32_t acc_full) const {
-    for (int j = n_multiplied > NST ? n_multiplied - NST : 0; j < n_multiplied; ++j) mbar_drain(empty0 + 8 * (j % NST), (j / NST) & 1);
+  __device__ __forceinline__ void drain(int stages, int rank, uint32_t full0, uint32_t empty0, uint32_t acc_full) const {
+    for (int j = n_multiplied > stages ? n_multiplied - stages : 0; j < n_multiplied; ++j) mbar_drain(empty0 + 8 * (j % stages), (j / stages) & 1);
     for (int j = n_accs > 2 ? n_accs - 2 : 0; j < n_accs; ++j) mbar_drain(acc_full + 8 * (j & 1), (j >> 1) & 1);
     if (rank != 0) return;
     const int c = n_copied[0] > n_copied[1] ? n_copied[0] : n_copied[1];
-    for (int j = c > NST ? c - NST : 0; j < c; ++j) mbar_drain(full0 + 8 * (j % NST), (j / NST) & 1);
+    for (int j = c > stages ? c - stages : 0; j < c; ++j) mbar_drain(full0 + 8 * (j % stages), (j / stages) & 1);
+  }
+  template <int NST>
+  static __device__ __forceinline__ bool await_stages(uint32_t empty0, int slabs, bool ok, int* fault, int code) {
+    return await_stages(NST, empty0, slabs, ok, fault, code);
+  }
+  template <int NST>
+  __device__ __forceinline__ void drain(int rank, uint32_t full0, uint32_t empty0, uint32_t acc_full) const {
+    drain(NST, rank, full0, empty0, acc_full);
   }
 };
 
