@@ -175,21 +175,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
   tc_fence_after();
   const uint32_t tmem_acc = tmem_slot;
 
+  // Producer and MMA run in one thread each: with warps that wait and issue together a slab cost 680 cycles of issue, more than the MMAs of any
+  // width take (8192 tokens through 7168 x 7168: 382 us).
   if (warp == 0) {
-    const uint32_t full_leader = leader_addr(full0);
-    int it = 0, st = 0;
-    uint32_t round = 0;
-    bool ok = true;
-    Unit u;
-    for (int64_t unit = pair; ok && u.seek(unit, a, offsets, tiles_before); unit += n_pairs) {
-      const int half = u.width >> 1;
-      const int b_row = u.t0 + rank * half;
-      const int n_boxes = (half + 31) / 32;
-      const uint32_t bytes = 2 * (I8_TILE_BYTES + (uint32_t)n_boxes * 32 * I8_K);
-      for (int s = u.slab0; s < u.slab1; ++s, ++it) {
-        if (it >= a.stages && !mbar_wait(empty0 + 8 * st, (round - 1) & 1, a.fault, 91)) { ok = false; break; }
-        const uint32_t dst = smem_base + (uint32_t)(st * a.stage_bytes), bar = full_leader + 8 * st;
-        if (lane == 0) {
+    if (elect_one()) {
+      const uint32_t full_leader = leader_addr(full0);
+      int it = 0, st = 0;
+      uint32_t round = 0;
+      bool ok = true;
+      Unit u;
+      for (int64_t unit = pair; ok && u.seek(unit, a, offsets, tiles_before); unit += n_pairs) {
+        const int half = u.width >> 1;
+        const int b_row = u.t0 + rank * half;
+        const int n_boxes = (half + 31) / 32;
+        const uint32_t bytes = 2 * (I8_TILE_BYTES + (uint32_t)n_boxes * 32 * I8_K);
+        for (int s = u.slab0; s < u.slab1; ++s, ++it) {
+          if (it >= a.stages && !mbar_wait_lane(empty0 + 8 * st, (round - 1) & 1, a.fault, 91)) { ok = false; break; }
+          const uint32_t dst = smem_base + (uint32_t)(st * a.stage_bytes), bar = full_leader + 8 * st;
           if (rank == 0) mbar_expect_tx(full0 + 8 * st, bytes);
           if constexpr (KIND == INT8_GATED) {
             // sixteen gate rows, then the sixteen up rows of the same results, for each quarter of the CTA's rows
@@ -200,46 +202,42 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
             load_weights_pair(dst, &map_w, bar, s * I8_K, u.m * TILE_ROWS + rank * 128, 0, u.e);
           }
           for (int j = 0; j < n_boxes; ++j) load_tokens_pair(dst + I8_TILE_BYTES + j * 32 * I8_K, &map_x, bar, s * I8_K, b_row + 32 * j);
-        }
-        __syncwarp();
-        if (++st == a.stages) {
-          st = 0;
-          ++round;
+          if (++st == a.stages) {
+            st = 0;
+            ++round;
+          }
         }
       }
-    }
-    ok = PairEnd::await_stages(a.stages, empty0, it, ok, a.fault, 95);
-    if (lane == 0) {
+      // the last use of every stage has been read (so its copies had landed)
+      for (int j = it > a.stages ? it - a.stages : 0; j < it && ok; ++j) ok = mbar_wait_lane(empty0 + 8 * (j % a.stages), (j / a.stages) & 1, a.fault, 95);
       end.copied_by(rank, it);
       if (!ok) end.give_up();
     }
+    __syncwarp();
   } else if (warp == 1) {
-    if (rank == 0) {
+    if (rank == 0 && elect_one()) {
       int it = 0, n = 0, st = 0;
       uint32_t round = 0;
       bool ok = true;
       Unit u;
+      const uint64_t desc0 = kmajor_sw128_desc(smem_base);
       for (int64_t unit = pair; ok && u.seek(unit, a, offsets, tiles_before); unit += n_pairs, ++n) {
         const int b = n & 1;
         // sums of 32 bits, signed 8-bit operands, 256 rows, `width` columns
         const uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(u.width >> 3) << 17) | ((uint32_t)(256 >> 4) << 24);
         const uint32_t acc = tmem_acc + (uint32_t)(b * I8_MAX_WIDTH);
-        if (n >= 2) ok = mbar_wait(acc_empty + 8 * b, ((n >> 1) - 1) & 1, a.fault, 93);
+        if (n >= 2) ok = mbar_wait_lane(acc_empty + 8 * b, ((n >> 1) - 1) & 1, a.fault, 93);
         tc_fence_after();
         for (int s = u.slab0; s < u.slab1 && ok; ++s) {
-          ok = mbar_wait(full0 + 8 * st, round & 1, a.fault, 92);
+          ok = mbar_wait_lane(full0 + 8 * st, round & 1, a.fault, 92);
           if (!ok) break;
           tc_fence_after();
-          if (lane == 0) {
-            const uint32_t a_tile = smem_base + (uint32_t)(st * a.stage_bytes);
-            const uint64_t a0 = kmajor_sw128_desc(a_tile), b0 = kmajor_sw128_desc(a_tile + I8_TILE_BYTES);
+          const uint64_t a0 = desc0 + (uint64_t)((uint32_t)(st * a.stage_bytes) >> 4), b0 = a0 + (I8_TILE_BYTES >> 4);
 #pragma unroll
-            for (int kk = 0; kk < I8_K / 32; ++kk)
-              umma_i8_pair(acc, a0 + (uint64_t)((kk * 32) >> 4), b0 + (uint64_t)((kk * 32) >> 4), idesc, s > u.slab0 || kk > 0 ? 1u : 0u);
-            umma_commit_pair(empty0 + 8 * st);
-            if (s == u.slab1 - 1) umma_commit_pair(acc_full + 8 * b);
-          }
-          __syncwarp();
+          for (int kk = 0; kk < I8_K / 32; ++kk)
+            umma_i8_pair(acc, a0 + (uint64_t)((kk * 32) >> 4), b0 + (uint64_t)((kk * 32) >> 4), idesc, s > u.slab0 || kk > 0 ? 1u : 0u);
+          umma_commit_pair(empty0 + 8 * st);
+          if (s == u.slab1 - 1) umma_commit_pair(acc_full + 8 * b);
           ++it;
           if (++st == a.stages) {
             st = 0;
@@ -248,11 +246,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
         }
         if (!ok) break;
       }
-      if (lane == 0) {
-        end.multiplied(it, n);
-        if (!ok) end.give_up();
-      }
+      end.multiplied(it, n);
+      if (!ok) end.give_up();
     }
+    __syncwarp();
   } else if (warp >= 4) {
     const int h = (warp - 4) >> 2, q = warp & 3;   // which chunks of 32 tokens, TMEM lane quadrant
     const uint32_t empty_leader = leader_addr(acc_empty);
