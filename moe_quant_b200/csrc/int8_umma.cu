@@ -25,7 +25,8 @@ constexpr int I8_MAX_STAGES = 9, I8_THREADS = 384, I8_K = 128, I8_TILE_BYTES = 1
 constexpr int I8_PAIRS = 74;
 constexpr int I8_RING_BYTES = 192 * 1024;
 constexpr int I8_MAX_EXPERTS = 1024;
-constexpr size_t kInt8Smem = (size_t)I8_RING_BYTES + 1024;
+constexpr int I8_STAGING = 2048;   // of an epilogue warp
+constexpr size_t kInt8Smem = (size_t)I8_RING_BYTES + 8 * I8_STAGING + 1024;
 
 struct PairArgs {
   Int8Product p;
@@ -33,7 +34,7 @@ struct PairArgs {
   int max_width, m_tiles;
   int sum_shift;   // INT8_PAIRS: 2^sum_shift brings the largest sum down to 2^15
   int stages, stage_bytes;
-  int packed;      // two neighbouring results of a token are stored together
+  int packed;      // rows of results can be stored 16 bytes at a time
   int splits;      // CTA pairs that share a tile's k
   int* sums;       // INT8_SUMS: (splits, T, ld_sums)
   int64_t ld_sums;
@@ -113,9 +114,39 @@ struct Unit {
   }
 };
 
-__device__ __forceinline__ float gated(float g, float u) { return g / (1.0f + expf(-g)) * u; }
+// silu(g) u; the exponential is off by 2 + 1.2 |g| steps at most, the quotient by 2
+__device__ __forceinline__ float gated(float g, float u) { return __fdividef(g, 1.0f + __expf(-g)) * u; }
 
-template <int KIND>
+__device__ __forceinline__ uint16_t bits16(__nv_bfloat16 v) { return __bfloat16_as_ushort(v); }
+__device__ __forceinline__ uint16_t bits16(__half v) { return __half_as_ushort(v); }
+
+// Results of 32 columns (a lane each) for `TOKENS` tokens leave in 16-byte pieces of rows, through a tile in shared memory (2 KB, this
+// warp's).  Stored by the lanes as they come, in pieces of 64 bytes, an epilogue of 256 tokens took 6 us.
+template <int TOKENS, typename S, typename Of>
+__device__ __forceinline__ void store_rows(uint32_t tile, int lane, S* out, int64_t ld, int left, int cols, Of value) {
+  constexpr int PITCH = 32 * sizeof(S), PER = 16 / sizeof(S), LANES = 32 / PER;     // bytes of a row; values per piece; lanes per row
+  static_assert(TOKENS * PITCH == 2048, "the tile has 2 KB");
+#pragma unroll
+  for (int j = 0; j < TOKENS; ++j) {
+    if constexpr (sizeof(S) == 4) asm volatile("st.shared.f32 [%0], %1;" ::"r"(tile + j * PITCH + lane * 4), "f"(value(j)) : "memory");
+    else asm volatile("st.shared.u16 [%0], %1;" ::"r"(tile + j * PITCH + lane * 2), "h"(bits16(from_float<S>(value(j)))) : "memory");
+  }
+  __syncwarp();
+  const int row = lane / LANES, piece = lane % LANES;
+  S* to = out + (int64_t)row * ld + piece * PER;
+  const bool in = piece * PER < cols;
+#pragma unroll
+  for (int i = 0; i < TOKENS * LANES / 32; ++i) {
+    uint4 w;
+    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(tile + i * 512 + lane * 16) : "memory");
+    if (in && i * (32 / LANES) + row < left) *reinterpret_cast<uint4*>(to) = w;
+    to += (int64_t)(32 / LANES) * ld;
+  }
+  __syncwarp();
+}
+
+// DT: type of y (INT8_Y)
+template <int KIND, int DT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
     int8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const PairArgs a) {
   constexpr int SETS = KIND == INT8_GATED ? 2 : 1;
@@ -255,6 +286,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
     const uint32_t empty_leader = leader_addr(acc_empty);
     const uint32_t t_lane = tmem_acc + ((uint32_t)(q * 32) << 16);
     float* my_scale = token_scale[warp - 4];
+    const uint32_t tile = smem_base + (uint32_t)I8_RING_BYTES + (uint32_t)(warp - 4) * I8_STAGING;
     bool ok = true;
     int n = 0;
     Unit u;
@@ -299,17 +331,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
             if (col_in && j < left) out[j * a.ld_sums] = r[j];
           continue;
         }
-        __syncwarp();
-        my_scale[lane] = xs[i];
-        __syncwarp();
         float v[32];
+        if constexpr (KIND == INT8_PAIRS) {
 #pragma unroll
-        for (int j = 0; j < 32; j += 4) {
-          const float4 s4 = *reinterpret_cast<const float4*>(my_scale + j);
-          if (KIND == INT8_PAIRS) {
+          for (int j = 0; j < 32; ++j) v[j] = (float)r[j] * ws;
+        } else {
+          __syncwarp();
+          my_scale[lane] = xs[i];
+          __syncwarp();
 #pragma unroll
-            for (int i4 = 0; i4 < 4; ++i4) v[j + i4] = (float)r[j + i4] * ws;
-          } else {
+          for (int j = 0; j < 32; j += 4) {
+            const float4 s4 = *reinterpret_cast<const float4*>(my_scale + j);
             v[j] = (float)r[j] * s4.x * ws;
             v[j + 1] = (float)r[j + 1] * s4.y * ws;
             v[j + 2] = (float)r[j + 2] * s4.z * ws;
@@ -317,44 +349,48 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
           }
         }
         if constexpr (KIND == INT8_GATED) {
-          // lanes 0 .. 15 hold the gate, 16 .. 31 the up of the same results: the former take the even tokens, the latter the odd
+          // lanes 0 .. 15 hold the gate, 16 .. 31 the up of the same results: the former take the even tokens, the latter the odd; 32 tokens
+          // of 16 results lie in the tile as 16 rows of two tokens each
           const bool up = lane >= 16;
-          float* out = static_cast<float*>(a.o.y) + (int64_t)(t + up) * a.o.ldy + col;
+          float hv[16];
 #pragma unroll
           for (int j = 0; j < 32; j += 2) {
             const float other = __shfl_xor_sync(0xffffffffu, up ? v[j] : v[j + 1], 16);
-            const float hv = up ? gated(other, v[j + 1]) : gated(v[j], other);
-            if (col_in && j + up < left) out[(int64_t)j * a.o.ldy] = hv;
+            hv[j / 2] = up ? gated(other, v[j + 1]) : gated(v[j], other);
           }
+          float* out = static_cast<float*>(a.o.y) + (int64_t)t * a.o.ldy + (col - (lane & 15));
+          const int cols = p.rows - (col - (lane & 15));
+#pragma unroll
+          for (int j = 0; j < 16; ++j)
+            asm volatile("st.shared.f32 [%0], %1;" ::"r"(tile + j * 128 + lane * 4), "f"(hv[j]) : "memory");
+          __syncwarp();
+          const int token = lane >> 2, piece = lane & 3;
+          float* to = out + (int64_t)token * a.o.ldy + piece * 4;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            uint4 w;
+            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(tile + k * 512 + lane * 16) : "memory");
+            // (rows of h have room for a multiple of sixteen results)
+            if (piece * 4 < cols && k * 8 + token < left) *reinterpret_cast<uint4*>(to) = w;
+            to += 8 * a.o.ldy;
+          }
+          __syncwarp();
         } else {
+          using S = typename StorageOf<KIND == INT8_PAIRS ? MQ_F16 : DT>::type;
           if constexpr (KIND == INT8_Y) {
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] += bias;
           }
+          S* out = static_cast<S*>(a.o.y) + (int64_t)t * a.o.ldy + (col - lane);
           if (a.packed) {
-            // neighbouring lanes hold neighbouring results of a token: the even one takes both of the even tokens, the odd one of the odd
-            const bool odd = lane & 1;
-            const int64_t at = (int64_t)(t + odd) * a.o.ldy + (col & ~1);
-#pragma unroll
-            for (int j = 0; j < 32; j += 2) {
-              const float other = __shfl_xor_sync(0xffffffffu, odd ? v[j] : v[j + 1], 1);
-              const float lo = odd ? other : v[j], hi = odd ? v[j + 1] : other;
-              if (col_in && j + odd < left) {
-                if (a.o.dtype == MQ_BF16) *reinterpret_cast<__nv_bfloat162*>(static_cast<__nv_bfloat16*>(a.o.y) + at + (int64_t)j * a.o.ldy) = __floats2bfloat162_rn(lo, hi);
-                else if (a.o.dtype == MQ_F16) *reinterpret_cast<__half2*>(static_cast<__half*>(a.o.y) + at + (int64_t)j * a.o.ldy) = __floats2half2_rn(lo, hi);
-                else *reinterpret_cast<float2*>(static_cast<float*>(a.o.y) + at + (int64_t)j * a.o.ldy) = make_float2(lo, hi);
-              }
-            }
+            constexpr int TOKENS = 64 / sizeof(S);
+            store_rows<TOKENS>(tile, lane, out, a.o.ldy, left, p.rows - (col - lane), [&](int j) { return v[j]; });
+            if constexpr (TOKENS < 32)
+              store_rows<TOKENS>(tile, lane, out + (int64_t)TOKENS * a.o.ldy, a.o.ldy, left - TOKENS, p.rows - (col - lane), [&](int j) { return v[TOKENS + j]; });
           } else {
-            const int64_t at = (int64_t)t * a.o.ldy + col;
 #pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              if (col_in && j < left) {
-                if (a.o.dtype == MQ_F32) static_cast<float*>(a.o.y)[at + (int64_t)j * a.o.ldy] = v[j];
-                else if (a.o.dtype == MQ_BF16) static_cast<__nv_bfloat16*>(a.o.y)[at + (int64_t)j * a.o.ldy] = __float2bfloat16_rn(v[j]);
-                else static_cast<__half*>(a.o.y)[at + (int64_t)j * a.o.ldy] = __float2half_rn(v[j]);
-              }
-            }
+            for (int j = 0; j < 32; ++j)
+              if (col_in && j < left) out[(int64_t)j * a.o.ldy + lane] = from_float<S>(v[j]);
           }
         }
       }
@@ -420,16 +456,16 @@ int encode(EncodeTiledFn enc, CUtensorMap* map, int rank, const void* base, cons
   return MQ_OK;
 }
 
-template <int KIND>
+template <int KIND, int DT = MQ_F32>
 int launch(const CUtensorMap& map_w, const CUtensorMap& map_x, const PairArgs& a, int pairs, cudaStream_t st) {
   static bool ready[64] = {};
   int dev = 0;
   MQ_CUDA(cudaGetDevice(&dev));
   if (dev >= 64 || !ready[dev]) {
-    MQ_CUDA(cudaFuncSetAttribute(int8_pair_kernel<KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kInt8Smem));
+    MQ_CUDA(cudaFuncSetAttribute(int8_pair_kernel<KIND, DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kInt8Smem));
     if (dev < 64) ready[dev] = true;
   }
-  MQ_CUDA(launch_chained(true, int8_pair_kernel<KIND>, dim3((unsigned)(2 * pairs)), dim3(I8_THREADS), kInt8Smem, st, map_w, map_x, a));
+  MQ_CUDA(launch_chained(true, int8_pair_kernel<KIND, DT>, dim3((unsigned)(2 * pairs)), dim3(I8_THREADS), kInt8Smem, st, map_w, map_x, a));
   MQ_LAUNCH_CHECK();
   return MQ_OK;
 }
@@ -515,12 +551,14 @@ int int8_product_umma(const Int8Product& p, const Int8Out& o, void* scratch, cud
     MQ_LAUNCH_CHECK();
     return MQ_OK;
   }
-  const size_t size = dtype_size(o.dtype);
+  const int64_t piece = o.kind == INT8_GATED ? 4 : 16 / (int64_t)dtype_size(o.dtype);
   while ((int64_t)p.K > (2ll << a.sum_shift)) ++a.sum_shift;   // 127 * 128 * K / 2^shift < 2^14 K / 2^shift <= 2^15
-  a.packed = p.rows % 2 == 0 && o.ldy % 2 == 0 && aligned(o.y, 2 * size);
+  a.packed = p.rows % piece == 0 && o.ldy % piece == 0 && aligned(o.y, 16);
   if (o.kind == INT8_GATED) return launch<INT8_GATED>(map_w, map_x, a, pairs, st);
   if (o.kind == INT8_PAIRS) return launch<INT8_PAIRS>(map_w, map_x, a, pairs, st);
-  return launch<INT8_Y>(map_w, map_x, a, pairs, st);
+  if (o.dtype == MQ_F32) return launch<INT8_Y, MQ_F32>(map_w, map_x, a, pairs, st);
+  if (o.dtype == MQ_BF16) return launch<INT8_Y, MQ_BF16>(map_w, map_x, a, pairs, st);
+  return launch<INT8_Y, MQ_F16>(map_w, map_x, a, pairs, st);
 }
 
 }  // namespace mq
