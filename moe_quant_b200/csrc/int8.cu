@@ -29,24 +29,78 @@ struct RowsParams {
   int8_t* codes;
   int64_t ldc;
   float* scale;
+  // PLAN: the places are found on the way, and written with the offsets
+  const int32_t* ids;
+  int E, first;
+  int32_t *place_out, *offsets;
 };
+
+// Up to so many pairs every block finds the places of its tokens by itself, counting the pairs that come in front: a launch less (experts
+// of 64 tokens, 512 pairs: 9 us for the plan and the codes, 5 together).
+constexpr int PLAN_PAIRS = 2048;
 
 // G threads per row, CH * 8 values a thread at a time; a row of up to G * CH * 8 values stays in registers between the search for its
 // largest and the rounding, and the block's next row is on its way meanwhile; a longer one is read twice (the second time from the L2).
 // Blocks per SM: what a thread holds of a row, as values and as codes, beside what it needs anyway.
 constexpr int rows_blocks(int dt, int ch) { return dt == MQ_F32 ? (ch >= 8 ? 1 : ch >= 4 ? 3 : 4) : (ch >= 8 ? 3 : ch >= 4 ? 4 : 5); }
-template <int DT, int G, int CH, bool VEC>
+template <int DT, int G, int CH, bool VEC, bool PLAN>
 __global__ void __launch_bounds__(256, rows_blocks(DT, CH)) quantize_rows_kernel(const RowsParams p) {
   using S = typename StorageOf<DT>::type;
   __shared__ uint32_t part[2][8];
+  __shared__ int expert[PLAN ? PLAN_PAIRS : 1], count[PLAN ? 1024 : 1];
   chain_wait();
   chain_release();
+  const int n_pairs = PLAN ? (int)p.T * p.top_k : 0;
+  if constexpr (PLAN) {
+    for (int i = threadIdx.x; i < p.E; i += 256) count[i] = 0;
+    for (int i = threadIdx.x; i < n_pairs; i += 256) {
+      const int64_t e = (int64_t)p.ids[i] - p.first;
+      expert[i] = e >= 0 && e < p.E ? (int)e : -1;
+    }
+    __syncthreads();
+    if (blockIdx.x == 0) {
+      for (int i = threadIdx.x; i < n_pairs; i += 256)
+        if (expert[i] >= 0) atomicAdd(&count[expert[i]], 1);
+      __syncthreads();
+      if (threadIdx.x < 32) {
+        int before = 0;
+        for (int e0 = 0; e0 < p.E; e0 += 32) {
+          const int e = e0 + threadIdx.x, n = e < p.E ? count[e] : 0;
+          int sum = n;
+          for (int o = 1; o < 32; o <<= 1) {
+            const int u = __shfl_up_sync(0xffffffffu, sum, o);
+            if ((int)threadIdx.x >= o) sum += u;
+          }
+          if (e < p.E) p.offsets[e] = before + sum - n;
+          before += __shfl_sync(0xffffffffu, sum, 31);
+        }
+        if (threadIdx.x == 0) p.offsets[p.E] = before;
+      }
+      __syncwarp();
+    }
+  }
   const int lane = threadIdx.x % G, warp_lane = threadIdx.x & 31;
   const int64_t end = p.rows_end ? min(p.T, (int64_t)__ldcg(p.rows_end)) : p.T;
   const int64_t stride = (int64_t)gridDim.x * (256 / G);
   const bool once = p.K <= G * CH * 8;
   // lane s of a warp: where the token's s-th copy goes
-  auto places = [&](int64_t t) { return p.place ? (t < end && warp_lane < p.top_k ? p.place[t * p.top_k + warp_lane] : -1) : t < end ? 0 : -1; };
+  auto places = [&](int64_t t) {
+    if constexpr (PLAN) {
+      int to = -1;
+      for (int s = 0; s < p.top_k && t < end; ++s) {
+        const int i = (int)t * p.top_k + s, e = expert[i];
+        if (e < 0) continue;
+        int n = 0;
+        for (int j = warp_lane; j < n_pairs; j += 32) n += expert[j] >= 0 && (expert[j] < e || (expert[j] == e && j < i));
+        n = __reduce_add_sync(0xffffffffu, n);
+        if (warp_lane == s) to = n;
+      }
+      if (lane < p.top_k && t < end) p.place_out[t * p.top_k + lane] = to;
+      return to;
+    }
+    return p.place ? (t < end && warp_lane < p.top_k ? p.place[t * p.top_k + warp_lane] : -1) : t < end ? 0 : -1;
+  };
+  const bool placed = PLAN || p.place;
   Eight<S> raw[CH];
   auto load = [&](int64_t t, int k0) {
     const S* row = static_cast<const S*>(p.x) + t * p.ldx;
@@ -85,7 +139,7 @@ __global__ void __launch_bounds__(256, rows_blocks(DT, CH)) quantize_rows_kernel
         for (int c = 0; c < CH; ++c) word[c] = code.of(raw[c]);
         if (once && copies_next) load(t + stride, 0);
         for (unsigned left = copies; left; left &= left - 1) {
-          const int64_t row = p.place ? __shfl_sync(0xffffffffu, to, __ffs(left) - 1) : t;
+          const int64_t row = placed ? __shfl_sync(0xffffffffu, to, __ffs(left) - 1) : t;
 #pragma unroll
           for (int c = 0; c < CH; ++c) {
             const int k = k0 + (c * G + lane) * 8;
@@ -98,11 +152,11 @@ __global__ void __launch_bounds__(256, rows_blocks(DT, CH)) quantize_rows_kernel
                 if (k + j < p.K) out[j] = (int8_t)((j < 4 ? word[c].x : word[c].y) >> (8 * (j & 3)));
             }
           }
-          if (!p.place) break;
+          if (!placed) break;
         }
       }
       if (lane < 32) {
-        if (p.place) {
+        if (placed) {
           if (to >= 0) p.scale[to] = code.scale;
         } else if (lane == 0) {
           p.scale[t] = code.scale;
@@ -117,12 +171,12 @@ __global__ void __launch_bounds__(256, rows_blocks(DT, CH)) quantize_rows_kernel
   }
 }
 
-template <int DT>
+template <int DT, bool PLAN>
 int launch_rows(const RowsParams& p, bool vec, cudaStream_t st) {
 #define MQ_ROWS(G, CH)                                                                                                      \
   do {                                                                                                                      \
     const int64_t blocks = ceil_div(p.T, 256 / G), most = 148 * rows_blocks(DT, CH);                                        \
-    MQ_CUDA(launch_chained(true, vec ? quantize_rows_kernel<DT, G, CH, true> : quantize_rows_kernel<DT, G, CH, false>,      \
+    MQ_CUDA(launch_chained(true, vec ? quantize_rows_kernel<DT, G, CH, true, PLAN> : quantize_rows_kernel<DT, G, CH, false, PLAN>, \
                            dim3((unsigned)(blocks < most ? blocks : most)), dim3(256), 0, st, p));                          \
   } while (0)
   if (p.K <= 256) MQ_ROWS(32, 1);
@@ -140,9 +194,10 @@ int launch_rows(const RowsParams& p, bool vec, cudaStream_t st) {
 int quantize_rows(int dtype, RowsParams p, cudaStream_t st) {
   if (p.T == 0) return MQ_OK;
   const bool vec = p.K % 8 == 0 && aligned(p.x, 8 * dtype_size(dtype)) && p.ldx % 8 == 0 && aligned(p.codes, 8) && p.ldc % 8 == 0;
-  if (dtype == MQ_F32) return launch_rows<MQ_F32>(p, vec, st);
-  if (dtype == MQ_BF16) return launch_rows<MQ_BF16>(p, vec, st);
-  return launch_rows<MQ_F16>(p, vec, st);
+  if (p.ids) return dtype == MQ_BF16 ? launch_rows<MQ_BF16, true>(p, vec, st) : launch_rows<MQ_F16, true>(p, vec, st);
+  if (dtype == MQ_F32) return launch_rows<MQ_F32, false>(p, vec, st);
+  if (dtype == MQ_BF16) return launch_rows<MQ_BF16, false>(p, vec, st);
+  return launch_rows<MQ_F16, false>(p, vec, st);
 }
 
 // ---------------------------------------------------------------- products
@@ -372,9 +427,19 @@ extern "C" int mq_int8_experts(const void* x, int dtype, int64_t T, int64_t K, i
   dn.w = down; dn.ldw = ld_down; dn.w_expert = down_expert; dn.w_scale = down_scale;
   dn.E = (int)E; dn.rows = (int)K; dn.K = (int)I; dn.T = P;
   if (T == 1 && int8_one_token_fits(top_k, K, I)) return int8_one_token(x, dtype, ids, weights, top_k, (int)first, up, dn, b.h, y, st);
-  MQ_TRY(expert_plan(ids, P, (int)E, (int)first, b.offsets, b.order, b.place, b.plan, st));
   // the tokens' codes, once for each of their pairs, where the plan has them
-  MQ_TRY(quantize_rows(dtype, RowsParams{x, ldx, T, nullptr, b.place, top_k, (int)K, b.x_codes, pitch_of(K), b.x_scale}, st));
+  RowsParams rows = {x, ldx, T, nullptr, nullptr, top_k, (int)K, b.x_codes, pitch_of(K), b.x_scale};
+  if (P <= PLAN_PAIRS) {
+    rows.ids = ids;
+    rows.E = (int)E;
+    rows.first = (int)first;
+    rows.place_out = b.place;
+    rows.offsets = b.offsets;
+  } else {
+    MQ_TRY(expert_plan(ids, P, (int)E, (int)first, b.offsets, b.order, b.place, b.plan, st));
+    rows.place = b.place;
+  }
+  MQ_TRY(quantize_rows(dtype, rows, st));
   up.x = b.x_codes; up.ldx = pitch_of(K); up.x_rows = P; up.x_scale = b.x_scale; up.offsets = b.offsets;
   MQ_TRY(int8_product_umma(up, Int8Out{INT8_GATED, MQ_F32, b.h, pitch_of(I), nullptr, nullptr}, nullptr, st));
   MQ_TRY(quantize_rows(MQ_F32, RowsParams{b.h, pitch_of(I), P, b.offsets + E, nullptr, 0, (int)I, b.h_codes, pitch_of(I), b.h_scale}, st));

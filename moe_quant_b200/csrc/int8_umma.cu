@@ -473,9 +473,11 @@ int launch(const CUtensorMap& map_w, const CUtensorMap& map_x, const PairArgs& a
 }  // namespace
 
 namespace {
-// How wide a tile of tokens is at most and how many pairs of CTAs share its k, from what a tile costs (measured, us): a slab of 128 of k
-// 0.40 at 256 columns where the MMA bounds it, and 0.20 + 0.0008 a column where its 16 KB + 64 bytes a column bound it; about 4 beside
-// the slabs and 0.01 a column for the last epilogue; where k is shared, the second kernel and the sums' way through the L2.
+// How wide a tile of tokens is at most and how many pairs of CTAs share its k, from what a tile costs (us, measured over 2048 to 7168 rows of
+// 1024 to 16384): a slab of 128 of k 0.225 up to 64 columns and 0.20 + 0.00035 a column above, 4.9 + 0.008 a column beside the slabs; where k
+// is shared, 3.3 for the second kernel and 10 MB/us for the sums' way through the L2.  Picked / best of all shapes tried: 16 tokens
+// through 2048 x 7168 9.9 / 9.9 (not shared 17.1), 512 tokens 18.1 / 17.4, 2048 tokens 23.5 / 23.5 (128 wide 34.0), 1011 x 1008 x 1072 7.2 / 7.2 (256
+// wide 9.5).
 struct Shape {
   int width, splits;
 };
@@ -486,11 +488,11 @@ Shape best_shape(int64_t rows_of_tiles, int64_t T, int slabs, bool shared) {
   for (int width = I8_MAX_WIDTH; width >= 32; width -= 32) {
     const int64_t n_tiles = token_tiles(T, width), tiles = rows_of_tiles * n_tiles;
     const int w = tile_width(T, (int)n_tiles);
-    const double slab_us = 0.0016 * w > 0.17 + 0.0008 * w ? 0.0016 * w : 0.17 + 0.0008 * w;
+    const double slab_us = w <= 64 ? 0.225 : 0.20 + 0.00035 * w;
     const int fit = shared && tiles < I8_PAIRS ? (int)(I8_PAIRS / tiles) : 1;
     for (int splits = 1; splits <= fit && splits <= I8_MOST_SPLITS && splits * 2 <= slabs; ++splits) {
-      const double us = (double)ceil_div(tiles * splits, I8_PAIRS) * (double)ceil_div(slabs, splits) * slab_us + 4.0 + 0.01 * w +
-                        (splits > 1 ? 2.5 + 8.0 * splits * (double)T * (double)rows_of_tiles * 256 / 4e6 : 0.0);
+      const double us = (double)ceil_div(tiles * splits, I8_PAIRS) * (double)ceil_div(slabs, splits) * slab_us + 4.9 + 0.008 * w +
+                        (splits > 1 ? 3.3 + 8.0 * splits * (double)T * (double)rows_of_tiles * 256 / 1e7 : 0.0);
       if (us < best_us * 0.98) {
         best_us = us;
         best = {width, splits};

@@ -380,8 +380,17 @@ def pack_int4(codes: Tensor, zero_i8: Optional[Tensor] = None, group: int = 0) -
 # Forward only.  Scratch comes from the caching allocator with every call: a buffer kept per stream would be shared by two graphs captured
 # on one stream, whose replays may overlap.
 def _forward_only(what: str, *tensors: Optional[Tensor]) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise MoeQuantError(f"{what} has no backward pass: call it under torch.no_grad() or detach its inputs")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise MoeQuantError(f"{what} has no backward pass: call it under torch.no_grad() or detach its inputs")
+
+
+def _same_device(what: str, device: torch.device, *tensors: Optional[Tensor]) -> None:
+    for t in tensors:
+        if t is not None and t.device != device:
+            require_one_device(what, *[u for u in tensors if u is not None])
+            raise MoeQuantError(f"{what}: expected all tensors on {device}")
 
 
 def _rows(t: Tensor, what: str) -> Tensor:
@@ -475,7 +484,7 @@ def route_tokens(logits: Tensor, top_k: int, *, score: str = "softmax", bias: Op
         raise MoeQuantError("route_tokens: logits must be (..., E)")
     E, lead = logits.shape[-1], logits.shape[:-1]
     if bias is not None:
-        require_one_device("route_tokens", logits, bias)
+        _same_device("route_tokens", logits.device, bias)
         if bias.shape != (E,):
             raise MoeQuantError(f"route_tokens: bias of shape {tuple(bias.shape)} for {E} experts")
         bias = _fp32(bias)
@@ -543,7 +552,7 @@ def int8_matmul(x: Tensor, weight: Tensor, weight_scale: Tensor, bias: Optional[
     x_code, out_code = MQ_I8 if given else dtype_code(x.dtype), dtype_code(out_dtype)
     lead = x.shape[:-1]
     dev = x.device
-    require_one_device("int8_matmul", *(t for t in (x, weight, weight_scale, bias, x_scale) if t is not None))
+    _same_device("int8_matmul", dev, weight, weight_scale, bias, x_scale)
     weight_scale = _scales(weight_scale, (N,), "weight_scale")
     if bias is not None:
         bias = _scales(bias, (N,), "bias")
@@ -579,7 +588,7 @@ def int8_experts(x: Tensor, ids: Tensor, weights: Tensor, gate_up: Tensor, gate_
         raise MoeQuantError(f"int8_experts: x {tuple(x.shape)}, gate_up {tuple(gate_up.shape)} and down {tuple(down.shape)} do not match")
     if ids.dim() != x.dim() or ids.shape[:-1] != x.shape[:-1] or weights.shape != ids.shape:
         raise MoeQuantError(f"int8_experts: ids {tuple(ids.shape)} and weights {tuple(weights.shape)} do not match x {tuple(x.shape)}")
-    require_one_device("int8_experts", x, ids, weights, gate_up, gate_up_scale, down, down_scale)
+    _same_device("int8_experts", x.device, ids, weights, gate_up, gate_up_scale, down, down_scale)
     ids = _int32(ids, "ids")
     weights = _fp32(weights)
     gate_up_scale = _scales(gate_up_scale, (E, I2), "gate_up_scale")
