@@ -1,28 +1,30 @@
-// 8-bit integer products of a few tokens: the weights are read once, straight into registers, and bound the time.
+// 8-bit integer products of a few tokens: the weights are read once and bound the time.
 //
 // Every block holds the codes of all tokens in shared memory (it rounds them itself: they are few, and the first weights are on their way
-// meanwhile) and takes a run of weight rows, a row per warp.  A lane multiplies 16 weights at a time with the tokens' codes (dp4a);
-// the warp's sums come together in one reduction.  512 threads per block, one block per SM: sixteen warps with eight 16-byte loads per
-// lane under way are 64 KB per SM, which is what the memory's latency wants.
+// meanwhile) and takes a run of weight rows, a row per warp.  Rows come through a ring of four pieces of 2 KB that each warp keeps by
+// bulk copies: 128 KB per SM under way.  (Eight 16-byte loads per lane, 64 KB, gave 5.0 TB/s on the gate and up rows of one
+// token's eight experts, and fetching rows into the L2 ahead of them less still.)  A lane multiplies 16 weights at a time with the tokens'
+// codes (dp4a); the warp's sums come together in one reduction.
 #include <math_constants.h>
 
 #include "int8.cuh"
 #include "int8_codes.cuh"
+#include "mbarrier.cuh"
 #include "profile.cuh"
 
 namespace mq {
 namespace {
 
-constexpr int FEW_THREADS = 512, FEW_WARPS = FEW_THREADS / 32, FEW_BLOCKS = 148, FEW_LOADS = 8;
-constexpr int FEW_STEP = 512 * FEW_LOADS;   // bytes of a row that a warp loads at a time
-constexpr size_t FEW_SMEM = 200 * 1024;
+constexpr int FEW_THREADS = 512, FEW_WARPS = FEW_THREADS / 32, FEW_BLOCKS = 148;
+constexpr int FEW_PIECE = 2048, FEW_SLOTS = 4, FEW_RING = FEW_PIECE * FEW_SLOTS;
+constexpr size_t FEW_SMEM = 208 * 1024, FEW_CODES = FEW_SMEM - (size_t)FEW_WARPS * FEW_RING;   // in front of the rings: codes
 
-// bytes that a token's codes take: a whole number of steps, zeros behind the end
+// bytes that a token's codes take: a whole number of steps of a warp, zeros behind the end
 __host__ __device__ __forceinline__ int few_pitch(int K) { return (K + 511) / 512 * 512; }
 
-// 16 codes of a weight row from byte k on; zeros behind its end
-__device__ __forceinline__ int4 weights16(const int8_t* row, int k, int K) {
-  if (k + 16 <= K) return __ldcs(reinterpret_cast<const int4*>(row + k));
+// 16 codes of a row from byte k on; zeros behind its end
+__device__ __forceinline__ int4 codes16(const int8_t* row, int k, int K) {
+  if (k + 16 <= K) return *reinterpret_cast<const int4*>(row + k);
   int4 v = make_int4(0, 0, 0, 0);
   if (k < K) {
     uint32_t* p = reinterpret_cast<uint32_t*>(&v);
@@ -36,13 +38,83 @@ __device__ __forceinline__ int dot16(int4 a, int4 b, int sum) {
   return __dp4a(a.w, b.w, __dp4a(a.z, b.z, __dp4a(a.y, b.y, __dp4a(a.x, b.x, sum))));
 }
 
-// a step of a row into registers: only the loads that lie in the row
-__device__ __forceinline__ void load_step(int4 (&w)[FEW_LOADS], const int8_t* row, int k0, int K, int lane) {
-#pragma unroll
-  for (int i = 0; i < FEW_LOADS; ++i) {
-    const int k = k0 + i * 512 + lane * 16;
-    w[i] = k < K ? weights16(row, k, K) : make_int4(0, 0, 0, 0);
+// The weight rows of one warp, one after the other, through its ring.  Slots are refilled in the order in which they are emptied.
+struct RowStream {
+  uint32_t ring, bars;
+  int lane, n_rows, K, whole;          // `whole`: bytes of a row that are copied, a multiple of 16; up to 15 more are read directly
+  int next_row, next_at, next_slot;    // what is copied next, and where to
+  int slot;
+  uint32_t parity;
+  int under_way;
+  int* fault;
+  bool ok;
+  __device__ __forceinline__ RowStream(uint32_t ring_, uint32_t bars_, int lane_, int n_rows_, int K_, int* fault_)
+      : ring(ring_), bars(bars_), lane(lane_), n_rows(n_rows_), K(K_), whole(K_ & ~15), next_row(0), next_at(0), next_slot(0), slot(0), parity(0),
+        under_way(0), fault(fault_), ok(true) {}
+  template <typename RowOf>
+  __device__ __forceinline__ void copy_next(RowOf row_of) {
+    if (next_row >= n_rows || whole == 0) return;
+    const int bytes = min(FEW_PIECE, whole - next_at);
+    if (lane == 0) {
+      const uint32_t bar = bars + 8 * next_slot;
+      asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
+      asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                   ::"r"(ring + (uint32_t)(next_slot * FEW_PIECE)), "l"(row_of(next_row) + next_at), "r"(bytes), "r"(bar) : "memory");
+    }
+    ++under_way;
+    next_slot = next_slot + 1 == FEW_SLOTS ? 0 : next_slot + 1;
+    next_at += FEW_PIECE;
+    if (next_at >= whole) {
+      next_at = 0;
+      ++next_row;
+    }
   }
+  template <typename RowOf>
+  __device__ __forceinline__ void start(RowOf row_of) {
+    for (int i = 0; i < FEW_SLOTS; ++i) copy_next(row_of);
+  }
+  // use(k, 16 weights from byte k on) for this lane's share of row r, the r-th call
+  template <typename RowOf, typename Use>
+  __device__ __forceinline__ void row(int r, RowOf row_of, Use use) {
+    for (int at = 0; at < whole && ok; at += FEW_PIECE) {
+      ok = mbar_wait(bars + 8 * slot, parity, fault, 97);
+      if (!ok) return;
+      --under_way;
+      const uint32_t src = ring + (uint32_t)(slot * FEW_PIECE + lane * 16);
+#pragma unroll
+      for (int i = 0; i < FEW_PIECE / 512; ++i) {
+        const int k = at + i * 512 + lane * 16;
+        if (k < whole) {
+          int4 w;
+          asm volatile("ld.shared.v4.s32 {%0, %1, %2, %3}, [%4];" : "=r"(w.x), "=r"(w.y), "=r"(w.z), "=r"(w.w) : "r"(src + i * 512) : "memory");
+          use(k, w);
+        }
+      }
+      __syncwarp();      // all lanes have read the slot
+      slot = slot + 1 == FEW_SLOTS ? 0 : slot + 1;
+      if (slot == 0) parity ^= 1;
+      copy_next(row_of);
+    }
+    if (whole < K && lane == 0) use(whole, codes16(row_of(r), whole, K));
+  }
+  // after a wait that ran out: the copies that are still under way come to their end first
+  __device__ __forceinline__ void end() {
+    if (ok) return;
+    for (; under_way > 0; --under_way) {
+      const uint64_t t0 = global_ns();
+      while (!mbar_try(bars + 8 * slot, parity))
+        if (global_ns() - t0 > 100000000ull) break;
+      slot = slot + 1 == FEW_SLOTS ? 0 : slot + 1;
+      if (slot == 0) parity ^= 1;
+    }
+  }
+};
+
+// by one thread of the block, before any warp's stream starts
+__device__ __forceinline__ void init_bars(uint64_t (&bars)[FEW_WARPS][FEW_SLOTS]) {
+  for (int w = 0; w < FEW_WARPS; ++w)
+    for (int s = 0; s < FEW_SLOTS; ++s) mbar_init(smem_u32(&bars[w][s]), 1);
+  asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
 }
 
 // Rounds a row of numbers to codes in shared memory with `threads` threads (a multiple of 32, `id` of this one), whose warps leave their
@@ -73,6 +145,7 @@ struct FewParams {
   int out_dtype;
   void* y;
   int64_t ldy;
+  int* fault;
 };
 
 __device__ __forceinline__ void put(void* y, int dtype, int64_t at, float v) {
@@ -85,22 +158,27 @@ __device__ __forceinline__ void put(void* y, int dtype, int64_t at, float v) {
 template <int DT, int NT, bool VEC>
 __global__ void __launch_bounds__(FEW_THREADS, 1) int8_few_kernel(const FewParams p) {
   using S = typename StorageOf<DT == MQ_I8 ? MQ_F32 : DT>::type;
-  extern __shared__ __align__(16) int8_t few_codes[];
+  extern __shared__ __align__(128) int8_t few_codes[];
+  __shared__ uint64_t bars[FEW_WARPS][FEW_SLOTS];
   __shared__ uint32_t part[NT][FEW_WARPS];
   __shared__ float x_scale[NT];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, pitch = few_pitch(p.K);
   const int begin = (int)((int64_t)p.N * blockIdx.x / gridDim.x), end = (int)((int64_t)p.N * (blockIdx.x + 1) / gridDim.x);
+  if (threadIdx.x == 0) init_bars(bars);
+  __syncthreads();
   chain_wait();
   chain_release();
-  int4 w[FEW_LOADS];
-  int n = begin + warp;
-  if (n < end) load_step(w, p.w + (int64_t)n * p.ldw, 0, p.K, lane);
+  const int first = begin + warp;
+  auto row_of = [&](int r) { return p.w + (int64_t)(first + r * FEW_WARPS) * p.ldw; };
+  RowStream stream(smem_u32(few_codes) + (uint32_t)(NT * pitch + warp * FEW_RING), smem_u32(&bars[warp][0]), lane,
+                   first < end ? (end - first + FEW_WARPS - 1) / FEW_WARPS : 0, p.K, p.fault);
+  stream.start(row_of);
 #pragma unroll
   for (int t = 0; t < NT; ++t) {
     if constexpr (DT == MQ_I8) {
       const int8_t* row = static_cast<const int8_t*>(p.x) + t * p.ldx;
       for (int k = threadIdx.x * 16; k < pitch; k += FEW_THREADS * 16)
-        *reinterpret_cast<int4*>(few_codes + t * pitch + k) = t < p.T ? weights16(row, k, p.K) : make_int4(0, 0, 0, 0);
+        *reinterpret_cast<int4*>(few_codes + t * pitch + k) = t < p.T ? codes16(row, k, p.K) : make_int4(0, 0, 0, 0);
       if (threadIdx.x == 0 && t < p.T) x_scale[t] = p.x_scale[t];
     } else if (t < p.T) {
       const float s = round_row<VEC>(static_cast<const S*>(p.x) + t * p.ldx, p.K, few_codes + t * pitch, pitch, (int)threadIdx.x, FEW_THREADS, part[t], [] { __syncthreads(); });
@@ -110,35 +188,27 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) int8_few_kernel(const FewParam
     }
   }
   __syncthreads();
-  for (; n < end; n += FEW_WARPS) {
-    const int8_t* row = p.w + (int64_t)n * p.ldw;
+  for (int r = 0; r < stream.n_rows; ++r) {
     int sum[NT] = {};
-    for (int k0 = 0; k0 < p.K; k0 += FEW_STEP) {
-      int4 now[FEW_LOADS];
+    stream.row(r, row_of, [&](int k, int4 w) {
 #pragma unroll
-      for (int i = 0; i < FEW_LOADS; ++i) now[i] = w[i];
-      // the next step, of this row or the next one, is under way while this one is multiplied
-      if (k0 + FEW_STEP < p.K) load_step(w, row, k0 + FEW_STEP, p.K, lane);
-      else if (n + FEW_WARPS < end) load_step(w, row + (int64_t)FEW_WARPS * p.ldw, 0, p.K, lane);
-#pragma unroll
-      for (int i = 0; i < FEW_LOADS; ++i) {
-        const int k = k0 + i * 512;
-        if (k >= p.K) break;
-#pragma unroll
-        for (int t = 0; t < NT; ++t) sum[t] = dot16(now[i], *reinterpret_cast<const int4*>(few_codes + t * pitch + k + lane * 16), sum[t]);
-      }
-    }
+      for (int t = 0; t < NT; ++t) sum[t] = dot16(w, *reinterpret_cast<const int4*>(few_codes + t * pitch + k), sum[t]);
+    });
+    if (!stream.ok) break;
+    __syncwarp();
 #pragma unroll
     for (int t = 0; t < NT; ++t) sum[t] = __reduce_add_sync(0xffffffffu, sum[t]);
     int mine = sum[0];
 #pragma unroll
     for (int t = 1; t < NT; ++t) mine = lane == t ? sum[t] : mine;
     if (lane < p.T) {
+      const int n = first + r * FEW_WARPS;
       float v = (float)mine * x_scale[lane] * __ldg(p.w_scale + n);
       if (p.bias) v += __ldg(p.bias + n);
       put(p.y, p.out_dtype, lane * p.ldy + n, v);
     }
   }
+  stream.end();
 }
 
 // ---------------------------------------------------------------- the experts of one token
@@ -154,9 +224,15 @@ struct OneParams {
   const float *gate_up_scale, *down_scale;
   float* h;      // (top_k, I)
   void* y;
+  int* fault;
 };
 
 __device__ __forceinline__ float gated(float g, float u) { return g / (1.0f + expf(-g)) * u; }
+
+// bytes in front of the rings: codes of h and a product per row and pair
+__host__ __device__ __forceinline__ size_t one_token_down_codes(int top_k, int64_t K, int64_t I) {
+  return ((size_t)top_k * few_pitch((int)I) + (size_t)(K / FEW_BLOCKS + 1) * top_k * 4 + 127) / 128 * 128;
+}
 
 // the pairs of the token with experts here, in the order of its slots; a whole warp
 __device__ __forceinline__ int pairs_here(const OneParams& p, int lane, int* expert, int* slot) {
@@ -177,10 +253,12 @@ __device__ __forceinline__ int pairs_here(const OneParams& p, int lane, int* exp
 template <int DT, bool VEC>
 __global__ void __launch_bounds__(FEW_THREADS, 1) one_token_gated_kernel(const OneParams p) {
   using S = typename StorageOf<DT>::type;
-  extern __shared__ __align__(16) int8_t few_codes[];
+  extern __shared__ __align__(128) int8_t few_codes[];
+  __shared__ uint64_t bars[FEW_WARPS][FEW_SLOTS];
   __shared__ uint32_t part[FEW_WARPS];
   __shared__ int expert[32], slot[32], found;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, pitch = few_pitch(p.K);
+  if (threadIdx.x == 32) init_bars(bars);
   chain_wait();
   chain_release();
   if (warp == 0) {
@@ -190,53 +268,46 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) one_token_gated_kernel(const O
   __syncthreads();
   const int64_t all = (int64_t)found * p.I;     // 32 * INT8_MAX_K at most
   const int begin = (int)(all * blockIdx.x / gridDim.x), end = (int)(all * (blockIdx.x + 1) / gridDim.x);
-  // unit u: gate row and up row of result u % I of pair u / I
-  auto row_of = [&](int u, int set) {
-    const int pair = u / p.I, i = u % p.I;
-    return p.gate_up + (int64_t)expert[pair] * p.gate_up_expert + ((int64_t)set * p.I + i) * p.ld_gate_up;
+  // unit u: gate row and up row of result u % I of pair u / I; the warp's rows by turns
+  const int first = begin + warp, units = first < end ? (end - first + FEW_WARPS - 1) / FEW_WARPS : 0;
+  auto row_of = [&](int r) {
+    const int u = first + (r >> 1) * FEW_WARPS, pair = u / p.I, i = u - pair * p.I;
+    return p.gate_up + (int64_t)expert[pair] * p.gate_up_expert + ((int64_t)(r & 1) * p.I + i) * p.ld_gate_up;
   };
-  int4 w[FEW_LOADS];
-  int u = begin + warp;
-  if (u < end) load_step(w, row_of(u, 0), 0, p.K, lane);
+  RowStream stream(smem_u32(few_codes) + (uint32_t)(pitch + warp * FEW_RING), smem_u32(&bars[warp][0]), lane, 2 * units, p.K, p.fault);
+  stream.start(row_of);
   const float xs = round_row<VEC>(static_cast<const S*>(p.x), p.K, few_codes, pitch, (int)threadIdx.x, FEW_THREADS, part, [] { __syncthreads(); });
   __syncthreads();
-  for (; u < end; u += FEW_WARPS) {
-    int sum[2] = {0, 0};
+  for (int n = 0; n < units; ++n) {
+    int sum[2];
 #pragma unroll
     for (int set = 0; set < 2; ++set) {
-      const int8_t* row = row_of(u, set);
-      for (int k0 = 0; k0 < p.K; k0 += FEW_STEP) {
-        int4 now[FEW_LOADS];
-#pragma unroll
-        for (int i = 0; i < FEW_LOADS; ++i) now[i] = w[i];
-        if (k0 + FEW_STEP < p.K) load_step(w, row, k0 + FEW_STEP, p.K, lane);
-        else if (set == 0) load_step(w, row_of(u, 1), 0, p.K, lane);
-        else if (u + FEW_WARPS < end) load_step(w, row_of(u + FEW_WARPS, 0), 0, p.K, lane);
-#pragma unroll
-        for (int i = 0; i < FEW_LOADS; ++i) {
-          const int k = k0 + i * 512;
-          if (k >= p.K) break;
-          sum[set] = dot16(now[i], *reinterpret_cast<const int4*>(few_codes + k + lane * 16), sum[set]);
-        }
-      }
+      int s = 0;
+      stream.row(2 * n + set, row_of, [&](int k, int4 w) { s = dot16(w, *reinterpret_cast<const int4*>(few_codes + k), s); });
+      sum[set] = s;
     }
+    if (!stream.ok) break;
+    __syncwarp();
     const int g = __reduce_add_sync(0xffffffffu, sum[0]), up = __reduce_add_sync(0xffffffffu, sum[1]);
     if (lane == 0) {
-      const int pair = u / p.I, i = u % p.I;
+      const int u = first + n * FEW_WARPS, pair = u / p.I, i = u - pair * p.I;
       const float* sc = p.gate_up_scale + (int64_t)expert[pair] * 2 * p.I;
       p.h[(int64_t)pair * p.I + i] = gated((float)g * xs * __ldg(sc + i), (float)up * xs * __ldg(sc + p.I + i));
     }
   }
+  stream.end();
 }
 
 template <int DT>
 __global__ void __launch_bounds__(FEW_THREADS, 1) one_token_down_kernel(const OneParams p) {
-  extern __shared__ __align__(16) int8_t few_codes[];      // codes of h, then the products of the block's rows, (rows, pairs)
+  extern __shared__ __align__(128) int8_t few_codes[];      // codes of h, the products of the block's rows, (rows, pairs), and the rings
+  __shared__ uint64_t bars[FEW_WARPS][FEW_SLOTS];
   __shared__ int expert[32], slot[32], found;
   __shared__ float factor[32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, pitch = few_pitch(p.I);
   float* products = reinterpret_cast<float*>(few_codes + (size_t)p.top_k * pitch);
-  // (ids have been there since before the kernel in front began to write)
+  if (threadIdx.x == 32) init_bars(bars);
+  // (ids and weights have been there since before the kernel in front began)
   if (warp == 0) {
     const int n = pairs_here(p, lane, expert, slot);
     if (lane == 0) found = n;
@@ -246,10 +317,13 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) one_token_down_kernel(const On
   const int begin = (int)((int64_t)p.K * blockIdx.x / gridDim.x), end = (int)((int64_t)p.K * (blockIdx.x + 1) / gridDim.x);
   // unit u: row begin + u / n_pairs of the expert of pair u % n_pairs
   const int units = (end - begin) * n_pairs;
-  auto row_of = [&](int u) { return p.down + (int64_t)expert[u % n_pairs] * p.down_expert + (int64_t)(begin + u / n_pairs) * p.ld_down; };
-  int4 w[FEW_LOADS];
-  int u = warp;
-  if (u < units) load_step(w, row_of(u), 0, p.I, lane);
+  auto row_of = [&](int r) {
+    const int u = warp + r * FEW_WARPS;
+    return p.down + (int64_t)expert[u % n_pairs] * p.down_expert + (int64_t)(begin + u / n_pairs) * p.ld_down;
+  };
+  RowStream stream(smem_u32(few_codes) + (uint32_t)(one_token_down_codes(p.top_k, p.K, p.I) + warp * FEW_RING), smem_u32(&bars[warp][0]), lane,
+                   warp < units ? (units - warp + FEW_WARPS - 1) / FEW_WARPS : 0, p.I, p.fault);
+  stream.start(row_of);
   chain_wait();
   chain_release();
   for (int v = warp; v < n_pairs; v += FEW_WARPS) {
@@ -258,26 +332,16 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) one_token_down_kernel(const On
     if (lane == 0) factor[v] = s * p.weights[slot[v]];
   }
   __syncthreads();
-  for (; u < units; u += FEW_WARPS) {
-    const int v = u % n_pairs, n = begin + u / n_pairs;
-    const int8_t* row = row_of(u);
+  for (int r = 0; r < stream.n_rows; ++r) {
+    const int u = warp + r * FEW_WARPS, v = u % n_pairs, n = begin + u / n_pairs;
     int sum = 0;
-    for (int k0 = 0; k0 < p.I; k0 += FEW_STEP) {
-      int4 now[FEW_LOADS];
-#pragma unroll
-      for (int i = 0; i < FEW_LOADS; ++i) now[i] = w[i];
-      if (k0 + FEW_STEP < p.I) load_step(w, row, k0 + FEW_STEP, p.I, lane);
-      else if (u + FEW_WARPS < units) load_step(w, row_of(u + FEW_WARPS), 0, p.I, lane);
-#pragma unroll
-      for (int i = 0; i < FEW_LOADS; ++i) {
-        const int k = k0 + i * 512;
-        if (k >= p.I) break;
-        sum = dot16(now[i], *reinterpret_cast<const int4*>(few_codes + v * pitch + k + lane * 16), sum);
-      }
-    }
+    stream.row(r, row_of, [&](int k, int4 w) { sum = dot16(w, *reinterpret_cast<const int4*>(few_codes + v * pitch + k), sum); });
+    if (!stream.ok) break;
+    __syncwarp();
     sum = __reduce_add_sync(0xffffffffu, sum);
     if (lane == 0) products[u] = (float)sum * factor[v] * __ldg(p.down_scale + (int64_t)expert[v] * p.K + n);
   }
+  stream.end();
   __syncthreads();
   for (int r = threadIdx.x; r < end - begin; r += FEW_THREADS) {
     float sum = 0.0f;
@@ -288,7 +352,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) one_token_down_kernel(const On
 
 template <typename Params>
 int launch_few(void (*kernel)(Params), size_t smem, const Params& p, cudaStream_t st) {
-  if (smem > 48 * 1024) MQ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)FEW_SMEM));
+  MQ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)FEW_SMEM));
   MQ_CUDA(launch_chained(true, kernel, dim3(FEW_BLOCKS), dim3(FEW_THREADS), smem, st, p));
   MQ_LAUNCH_CHECK();
   return MQ_OK;
@@ -301,7 +365,7 @@ bool rows_of_eight(const void* x, int64_t ldx, int64_t K, int64_t T) {
 
 template <int DT, int NT>
 int few(const FewParams& p, cudaStream_t st) {
-  const size_t smem = (size_t)NT * few_pitch(p.K);
+  const size_t smem = (size_t)NT * few_pitch(p.K) + FEW_WARPS * FEW_RING;
   if constexpr (DT == MQ_I8) return launch_few(int8_few_kernel<DT, NT, true>, smem, p, st);
   else return rows_of_eight<DT>(p.x, p.ldx, p.K, p.T) ? launch_few(int8_few_kernel<DT, NT, true>, smem, p, st) : launch_few(int8_few_kernel<DT, NT, false>, smem, p, st);
 }
@@ -312,23 +376,20 @@ int few_of(const FewParams& p, cudaStream_t st) {
   return few<DT, 4>(p, st);
 }
 
-size_t one_token_down_smem(int top_k, int64_t K, int64_t I) {
-  return (size_t)top_k * few_pitch((int)I) + (size_t)(K / FEW_BLOCKS + 1) * top_k * 4;
-}
-
 template <int DT>
 int one_token(const OneParams& p, cudaStream_t st) {
-  const size_t smem = (size_t)few_pitch(p.K);
+  const size_t smem = (size_t)few_pitch(p.K) + FEW_WARPS * FEW_RING;
   MQ_TRY(rows_of_eight<DT>(p.x, 0, p.K, 1) ? launch_few(one_token_gated_kernel<DT, true>, smem, p, st) : launch_few(one_token_gated_kernel<DT, false>, smem, p, st));
-  return launch_few(one_token_down_kernel<DT>, one_token_down_smem(p.top_k, p.K, p.I), p, st);
+  return launch_few(one_token_down_kernel<DT>, one_token_down_codes(p.top_k, p.K, p.I) + FEW_WARPS * FEW_RING, p, st);
 }
 
 }  // namespace
 
-bool int8_few_fits(int64_t T, int64_t K) { return T <= INT8_FEW_TOKENS && (T <= 2 ? T : 4) * few_pitch((int)K) <= (int64_t)FEW_SMEM; }
+bool int8_few_fits(int64_t T, int64_t K) { return T <= INT8_FEW_TOKENS && (T <= 2 ? T : 4) * few_pitch((int)K) <= (int64_t)FEW_CODES; }
 
 int int8_few(const void* x, int dtype, int64_t ldx, const Int8Product& q, const Int8Out& o, cudaStream_t st) {
-  const FewParams p = {x, q.x_scale, ldx, (int)q.T, q.rows, q.K, q.w, q.ldw, q.w_scale, o.bias, o.dtype, o.y, o.ldy};
+  FewParams p = {x, q.x_scale, ldx, (int)q.T, q.rows, q.K, q.w, q.ldw, q.w_scale, o.bias, o.dtype, o.y, o.ldy, nullptr};
+  MQ_TRY(engine_fault_word(&p.fault));
   if (dtype == MQ_I8) return few_of<MQ_I8>(p, st);
   if (dtype == MQ_F32) return few_of<MQ_F32>(p, st);
   if (dtype == MQ_BF16) return few_of<MQ_BF16>(p, st);
@@ -336,13 +397,14 @@ int int8_few(const void* x, int dtype, int64_t ldx, const Int8Product& q, const 
 }
 
 bool int8_one_token_fits(int top_k, int64_t K, int64_t I) {
-  return (size_t)few_pitch((int)K) <= FEW_SMEM && one_token_down_smem(top_k, K, I) <= FEW_SMEM;
+  return (size_t)few_pitch((int)K) <= FEW_CODES && one_token_down_codes(top_k, K, I) <= FEW_CODES;
 }
 
 int int8_one_token(const void* x, int dtype, const int32_t* ids, const float* weights, int top_k, int first, const Int8Product& up, const Int8Product& down,
                    float* h, void* y, cudaStream_t st) {
-  const OneParams p = {x, up.K, up.rows, up.E, top_k, first, ids, weights, up.w, down.w, up.ldw, up.w_expert, down.ldw, down.w_expert,
-                       up.w_scale, down.w_scale, h, y};
+  OneParams p = {x, up.K, up.rows, up.E, top_k, first, ids, weights, up.w, down.w, up.ldw, up.w_expert, down.ldw, down.w_expert,
+                       up.w_scale, down.w_scale, h, y, nullptr};
+  MQ_TRY(engine_fault_word(&p.fault));
   return dtype == MQ_BF16 ? one_token<MQ_BF16>(p, st) : one_token<MQ_F16>(p, st);
 }
 
