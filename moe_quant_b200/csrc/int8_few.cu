@@ -1,7 +1,7 @@
 // 8-bit integer products of a few tokens: the weights are read once and bound the time.
 //
 // Every block holds the codes of all tokens in shared memory (it rounds them itself: they are few, and the first weights are on their way
-// meanwhile) and takes a run of weight rows, a row per warp.  Rows come through a ring of four pieces of 2 KB that each warp keeps by
+// meanwhile) and takes a run of weight rows, a row per warp.  Rows come through a ring of pieces of 2 KB that each warp keeps by
 // bulk copies: 128 KB per SM under way.  (Eight 16-byte loads per lane, 64 KB, gave 5.0 TB/s on the gate and up rows of one
 // token's eight experts, and fetching rows into the L2 ahead of them less still.)  A lane multiplies 16 weights at a time with the tokens'
 // codes (dp4a); the warp's sums come together in one reduction.
@@ -15,9 +15,13 @@
 namespace mq {
 namespace {
 
-constexpr int FEW_THREADS = 512, FEW_WARPS = FEW_THREADS / 32, FEW_BLOCKS = 148;
-constexpr int FEW_PIECE = 2048, FEW_SLOTS = 4, FEW_RING = FEW_PIECE * FEW_SLOTS;
-constexpr size_t FEW_SMEM = 208 * 1024, FEW_CODES = FEW_SMEM - (size_t)FEW_WARPS * FEW_RING;   // in front of the rings: codes
+// A layer's kernel has 16 warps of four slots each; the experts' kernels, which go through 20 times as many rows per SM, 32 of two: one
+// token through 2048 x 7168 takes 4.8 / 5.3 us with 16 / 32 warps, its eight experts 68.5 / 63.4.
+constexpr int FEW_THREADS = 512, FEW_WARPS = FEW_THREADS / 32, FEW_SLOTS = 4, FEW_BLOCKS = 148;
+constexpr int ONE_THREADS = 1024, ONE_WARPS = ONE_THREADS / 32, ONE_SLOTS = 2;
+constexpr int FEW_PIECE = 2048, FEW_RINGS = FEW_WARPS * FEW_SLOTS * FEW_PIECE;
+static_assert(FEW_RINGS == ONE_WARPS * ONE_SLOTS * FEW_PIECE, "the same bytes under way");
+constexpr size_t FEW_SMEM = 208 * 1024, FEW_CODES = FEW_SMEM - (size_t)FEW_RINGS;   // in front of the rings: codes
 
 // bytes that a token's codes take: a whole number of steps of a warp, zeros behind the end
 __host__ __device__ __forceinline__ int few_pitch(int K) { return (K + 511) / 512 * 512; }
@@ -39,30 +43,33 @@ __device__ __forceinline__ int dot16(int4 a, int4 b, int sum) {
 }
 
 // The weight rows of one warp, one after the other, through its ring.  Slots are refilled in the order in which they are emptied.
+template <int SLOTS>
 struct RowStream {
   uint32_t ring, bars;
   int lane, n_rows, K, whole;          // `whole`: bytes of a row that are copied, a multiple of 16; up to 15 more are read directly
   int next_row, next_at, next_slot;    // what is copied next, and where to
+  const int8_t* from;                  // the row that is being copied
   int slot;
   uint32_t parity;
   int under_way;
   int* fault;
   bool ok;
   __device__ __forceinline__ RowStream(uint32_t ring_, uint32_t bars_, int lane_, int n_rows_, int K_, int* fault_)
-      : ring(ring_), bars(bars_), lane(lane_), n_rows(n_rows_), K(K_), whole(K_ & ~15), next_row(0), next_at(0), next_slot(0), slot(0), parity(0),
+      : ring(ring_), bars(bars_), lane(lane_), n_rows(n_rows_), K(K_), whole(K_ & ~15), next_row(0), next_at(0), next_slot(0), from(nullptr), slot(0), parity(0),
         under_way(0), fault(fault_), ok(true) {}
   template <typename RowOf>
   __device__ __forceinline__ void copy_next(RowOf row_of) {
     if (next_row >= n_rows || whole == 0) return;
     const int bytes = min(FEW_PIECE, whole - next_at);
+    if (next_at == 0) from = row_of(next_row);
     if (lane == 0) {
       const uint32_t bar = bars + 8 * next_slot;
       asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
       asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-                   ::"r"(ring + (uint32_t)(next_slot * FEW_PIECE)), "l"(row_of(next_row) + next_at), "r"(bytes), "r"(bar) : "memory");
+                   ::"r"(ring + (uint32_t)(next_slot * FEW_PIECE)), "l"(from + next_at), "r"(bytes), "r"(bar) : "memory");
     }
     ++under_way;
-    next_slot = next_slot + 1 == FEW_SLOTS ? 0 : next_slot + 1;
+    next_slot = next_slot + 1 == SLOTS ? 0 : next_slot + 1;
     next_at += FEW_PIECE;
     if (next_at >= whole) {
       next_at = 0;
@@ -71,7 +78,7 @@ struct RowStream {
   }
   template <typename RowOf>
   __device__ __forceinline__ void start(RowOf row_of) {
-    for (int i = 0; i < FEW_SLOTS; ++i) copy_next(row_of);
+    for (int i = 0; i < SLOTS; ++i) copy_next(row_of);
   }
   // use(k, 16 weights from byte k on) for this lane's share of row r, the r-th call
   template <typename RowOf, typename Use>
@@ -91,7 +98,7 @@ struct RowStream {
         }
       }
       __syncwarp();      // all lanes have read the slot
-      slot = slot + 1 == FEW_SLOTS ? 0 : slot + 1;
+      slot = slot + 1 == SLOTS ? 0 : slot + 1;
       if (slot == 0) parity ^= 1;
       copy_next(row_of);
     }
@@ -104,16 +111,17 @@ struct RowStream {
       const uint64_t t0 = global_ns();
       while (!mbar_try(bars + 8 * slot, parity))
         if (global_ns() - t0 > 100000000ull) break;
-      slot = slot + 1 == FEW_SLOTS ? 0 : slot + 1;
+      slot = slot + 1 == SLOTS ? 0 : slot + 1;
       if (slot == 0) parity ^= 1;
     }
   }
 };
 
 // by one thread of the block, before any warp's stream starts
-__device__ __forceinline__ void init_bars(uint64_t (&bars)[FEW_WARPS][FEW_SLOTS]) {
-  for (int w = 0; w < FEW_WARPS; ++w)
-    for (int s = 0; s < FEW_SLOTS; ++s) mbar_init(smem_u32(&bars[w][s]), 1);
+template <int WARPS, int SLOTS>
+__device__ __forceinline__ void init_bars(uint64_t (&bars)[WARPS][SLOTS]) {
+  for (int w = 0; w < WARPS; ++w)
+    for (int s = 0; s < SLOTS; ++s) mbar_init(smem_u32(&bars[w][s]), 1);
   asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
 }
 
@@ -170,7 +178,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) int8_few_kernel(const FewParam
   chain_release();
   const int first = begin + warp;
   auto row_of = [&](int r) { return p.w + (int64_t)(first + r * FEW_WARPS) * p.ldw; };
-  RowStream stream(smem_u32(few_codes) + (uint32_t)(NT * pitch + warp * FEW_RING), smem_u32(&bars[warp][0]), lane,
+  RowStream<FEW_SLOTS> stream(smem_u32(few_codes) + (uint32_t)(NT * pitch + warp * FEW_SLOTS * FEW_PIECE), smem_u32(&bars[warp][0]), lane,
                    first < end ? (end - first + FEW_WARPS - 1) / FEW_WARPS : 0, p.K, p.fault);
   stream.start(row_of);
 #pragma unroll
@@ -251,11 +259,11 @@ __device__ __forceinline__ int pairs_here(const OneParams& p, int lane, int* exp
 }
 
 template <int DT, bool VEC>
-__global__ void __launch_bounds__(FEW_THREADS, 1) one_token_gated_kernel(const OneParams p) {
+__global__ void __launch_bounds__(ONE_THREADS, 1) one_token_gated_kernel(const OneParams p) {
   using S = typename StorageOf<DT>::type;
   extern __shared__ __align__(128) int8_t few_codes[];
-  __shared__ uint64_t bars[FEW_WARPS][FEW_SLOTS];
-  __shared__ uint32_t part[FEW_WARPS];
+  __shared__ uint64_t bars[ONE_WARPS][ONE_SLOTS];
+  __shared__ uint32_t part[ONE_WARPS];
   __shared__ int expert[32], slot[32], found;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, pitch = few_pitch(p.K);
   if (threadIdx.x == 32) init_bars(bars);
@@ -269,14 +277,14 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) one_token_gated_kernel(const O
   const int64_t all = (int64_t)found * p.I;     // 32 * INT8_MAX_K at most
   const int begin = (int)(all * blockIdx.x / gridDim.x), end = (int)(all * (blockIdx.x + 1) / gridDim.x);
   // unit u: gate row and up row of result u % I of pair u / I; the warp's rows by turns
-  const int first = begin + warp, units = first < end ? (end - first + FEW_WARPS - 1) / FEW_WARPS : 0;
+  const int first = begin + warp, units = first < end ? (end - first + ONE_WARPS - 1) / ONE_WARPS : 0;
   auto row_of = [&](int r) {
-    const int u = first + (r >> 1) * FEW_WARPS, pair = u / p.I, i = u - pair * p.I;
+    const int u = first + (r >> 1) * ONE_WARPS, pair = u / p.I, i = u - pair * p.I;
     return p.gate_up + (int64_t)expert[pair] * p.gate_up_expert + ((int64_t)(r & 1) * p.I + i) * p.ld_gate_up;
   };
-  RowStream stream(smem_u32(few_codes) + (uint32_t)(pitch + warp * FEW_RING), smem_u32(&bars[warp][0]), lane, 2 * units, p.K, p.fault);
+  RowStream<ONE_SLOTS> stream(smem_u32(few_codes) + (uint32_t)(pitch + warp * ONE_SLOTS * FEW_PIECE), smem_u32(&bars[warp][0]), lane, 2 * units, p.K, p.fault);
   stream.start(row_of);
-  const float xs = round_row<VEC>(static_cast<const S*>(p.x), p.K, few_codes, pitch, (int)threadIdx.x, FEW_THREADS, part, [] { __syncthreads(); });
+  const float xs = round_row<VEC>(static_cast<const S*>(p.x), p.K, few_codes, pitch, (int)threadIdx.x, ONE_THREADS, part, [] { __syncthreads(); });
   __syncthreads();
   for (int n = 0; n < units; ++n) {
     int sum[2];
@@ -290,7 +298,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) one_token_gated_kernel(const O
     __syncwarp();
     const int g = __reduce_add_sync(0xffffffffu, sum[0]), up = __reduce_add_sync(0xffffffffu, sum[1]);
     if (lane == 0) {
-      const int u = first + n * FEW_WARPS, pair = u / p.I, i = u - pair * p.I;
+      const int u = first + n * ONE_WARPS, pair = u / p.I, i = u - pair * p.I;
       const float* sc = p.gate_up_scale + (int64_t)expert[pair] * 2 * p.I;
       p.h[(int64_t)pair * p.I + i] = gated((float)g * xs * __ldg(sc + i), (float)up * xs * __ldg(sc + p.I + i));
     }
@@ -299,9 +307,9 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) one_token_gated_kernel(const O
 }
 
 template <int DT>
-__global__ void __launch_bounds__(FEW_THREADS, 1) one_token_down_kernel(const OneParams p) {
+__global__ void __launch_bounds__(ONE_THREADS, 1) one_token_down_kernel(const OneParams p) {
   extern __shared__ __align__(128) int8_t few_codes[];      // codes of h, the products of the block's rows, (rows, pairs), and the rings
-  __shared__ uint64_t bars[FEW_WARPS][FEW_SLOTS];
+  __shared__ uint64_t bars[ONE_WARPS][ONE_SLOTS];
   __shared__ int expert[32], slot[32], found;
   __shared__ float factor[32];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, pitch = few_pitch(p.I);
@@ -318,22 +326,22 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) one_token_down_kernel(const On
   // unit u: row begin + u / n_pairs of the expert of pair u % n_pairs
   const int units = (end - begin) * n_pairs;
   auto row_of = [&](int r) {
-    const int u = warp + r * FEW_WARPS;
+    const int u = warp + r * ONE_WARPS;
     return p.down + (int64_t)expert[u % n_pairs] * p.down_expert + (int64_t)(begin + u / n_pairs) * p.ld_down;
   };
-  RowStream stream(smem_u32(few_codes) + (uint32_t)(one_token_down_codes(p.top_k, p.K, p.I) + warp * FEW_RING), smem_u32(&bars[warp][0]), lane,
-                   warp < units ? (units - warp + FEW_WARPS - 1) / FEW_WARPS : 0, p.I, p.fault);
+  RowStream<ONE_SLOTS> stream(smem_u32(few_codes) + (uint32_t)(one_token_down_codes(p.top_k, p.K, p.I) + warp * ONE_SLOTS * FEW_PIECE), smem_u32(&bars[warp][0]), lane,
+                   warp < units ? (units - warp + ONE_WARPS - 1) / ONE_WARPS : 0, p.I, p.fault);
   stream.start(row_of);
   chain_wait();
   chain_release();
-  for (int v = warp; v < n_pairs; v += FEW_WARPS) {
+  for (int v = warp; v < n_pairs; v += ONE_WARPS) {
     const float s = p.I % 8 == 0 ? round_row<true>(p.h + (int64_t)v * p.I, p.I, few_codes + v * pitch, pitch, lane, 32, nullptr, [] {})
                                  : round_row<false>(p.h + (int64_t)v * p.I, p.I, few_codes + v * pitch, pitch, lane, 32, nullptr, [] {});
     if (lane == 0) factor[v] = s * p.weights[slot[v]];
   }
   __syncthreads();
   for (int r = 0; r < stream.n_rows; ++r) {
-    const int u = warp + r * FEW_WARPS, v = u % n_pairs, n = begin + u / n_pairs;
+    const int u = warp + r * ONE_WARPS, v = u % n_pairs, n = begin + u / n_pairs;
     int sum = 0;
     stream.row(r, row_of, [&](int k, int4 w) { sum = dot16(w, *reinterpret_cast<const int4*>(few_codes + v * pitch + k), sum); });
     if (!stream.ok) break;
@@ -343,7 +351,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) one_token_down_kernel(const On
   }
   stream.end();
   __syncthreads();
-  for (int r = threadIdx.x; r < end - begin; r += FEW_THREADS) {
+  for (int r = threadIdx.x; r < end - begin; r += ONE_THREADS) {
     float sum = 0.0f;
     for (int v = 0; v < n_pairs; ++v) sum += products[r * n_pairs + v];
     put(p.y, DT, begin + r, sum);
@@ -351,9 +359,9 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) one_token_down_kernel(const On
 }
 
 template <typename Params>
-int launch_few(void (*kernel)(Params), size_t smem, const Params& p, cudaStream_t st) {
+int launch_few(void (*kernel)(Params), int threads, size_t smem, const Params& p, cudaStream_t st) {
   MQ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)FEW_SMEM));
-  MQ_CUDA(launch_chained(true, kernel, dim3(FEW_BLOCKS), dim3(FEW_THREADS), smem, st, p));
+  MQ_CUDA(launch_chained(true, kernel, dim3(FEW_BLOCKS), dim3((unsigned)threads), smem, st, p));
   MQ_LAUNCH_CHECK();
   return MQ_OK;
 }
@@ -365,9 +373,9 @@ bool rows_of_eight(const void* x, int64_t ldx, int64_t K, int64_t T) {
 
 template <int DT, int NT>
 int few(const FewParams& p, cudaStream_t st) {
-  const size_t smem = (size_t)NT * few_pitch(p.K) + FEW_WARPS * FEW_RING;
-  if constexpr (DT == MQ_I8) return launch_few(int8_few_kernel<DT, NT, true>, smem, p, st);
-  else return rows_of_eight<DT>(p.x, p.ldx, p.K, p.T) ? launch_few(int8_few_kernel<DT, NT, true>, smem, p, st) : launch_few(int8_few_kernel<DT, NT, false>, smem, p, st);
+  const size_t smem = (size_t)NT * few_pitch(p.K) + FEW_RINGS;
+  if constexpr (DT == MQ_I8) return launch_few(int8_few_kernel<DT, NT, true>, FEW_THREADS, smem, p, st);
+  else return rows_of_eight<DT>(p.x, p.ldx, p.K, p.T) ? launch_few(int8_few_kernel<DT, NT, true>, FEW_THREADS, smem, p, st) : launch_few(int8_few_kernel<DT, NT, false>, FEW_THREADS, smem, p, st);
 }
 template <int DT>
 int few_of(const FewParams& p, cudaStream_t st) {
@@ -378,9 +386,9 @@ int few_of(const FewParams& p, cudaStream_t st) {
 
 template <int DT>
 int one_token(const OneParams& p, cudaStream_t st) {
-  const size_t smem = (size_t)few_pitch(p.K) + FEW_WARPS * FEW_RING;
-  MQ_TRY(rows_of_eight<DT>(p.x, 0, p.K, 1) ? launch_few(one_token_gated_kernel<DT, true>, smem, p, st) : launch_few(one_token_gated_kernel<DT, false>, smem, p, st));
-  return launch_few(one_token_down_kernel<DT>, one_token_down_codes(p.top_k, p.K, p.I) + FEW_WARPS * FEW_RING, p, st);
+  const size_t smem = (size_t)few_pitch(p.K) + FEW_RINGS;
+  MQ_TRY(rows_of_eight<DT>(p.x, 0, p.K, 1) ? launch_few(one_token_gated_kernel<DT, true>, ONE_THREADS, smem, p, st) : launch_few(one_token_gated_kernel<DT, false>, ONE_THREADS, smem, p, st));
+  return launch_few(one_token_down_kernel<DT>, ONE_THREADS, one_token_down_codes(p.top_k, p.K, p.I) + FEW_RINGS, p, st);
 }
 
 }  // namespace
