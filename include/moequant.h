@@ -322,7 +322,7 @@ int mq_int8_experts(const void* x, int dtype, int64_t T, int64_t K, int64_t ldx,
                     int64_t first, int64_t E, int64_t I, const int8_t* gate_up, int64_t ld_gate_up, int64_t gate_up_expert,
                     const float* gate_up_scale, const int8_t* down, int64_t ld_down, int64_t down_expert, const float* down_scale,
                     void* y, int64_t ldy, void* workspace, size_t workspace_bytes, void* stream);
-size_t mq_int8_experts_workspace_bytes(int64_t T, int top_k, int64_t E, int64_t K, int64_t I);
+size_t mq_int8_experts_workspace_bytes(int dtype, int64_t T, int top_k, int64_t E, int64_t K, int64_t I);
 
 #ifdef __cplusplus
 }

@@ -83,7 +83,7 @@ SIGNATURES = {
     "mq_int8_experts": (c_int, [c_void_p, c_int, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int, c_int64, c_int64, c_int64,
                                 c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64, c_int64, c_void_p, c_void_p, c_int64,
                                 c_void_p, c_size_t, c_void_p]),
-    "mq_int8_experts_workspace_bytes": (c_size_t, [c_int64, c_int, c_int64, c_int64, c_int64]),
+    "mq_int8_experts_workspace_bytes": (c_size_t, [c_int, c_int64, c_int, c_int64, c_int64, c_int64]),
     "mq_pack_int4": (c_int, [c_void_p, c_int64, c_int64, c_void_p, c_int64, c_void_p, c_void_p]),
 }
 
@@ -189,7 +189,7 @@ _NOTHING = _Nothing()
 def on_device(device: torch.device):
     """torch.cuda.device(device), or nothing where that device is the current one already: the calls of a small
     layer are bound by the host, and the guard alone cost a tenth of them."""
-    if device.index is None or device.index == torch.cuda.current_device():
+    if device.index is None or device.index == torch._C._cuda_getDevice():
         return _NOTHING
     return torch.cuda.device(device)
 

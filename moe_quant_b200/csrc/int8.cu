@@ -201,10 +201,11 @@ int quantize_rows(int dtype, RowsParams p, cudaStream_t st) {
 }
 
 // ---------------------------------------------------------------- products
-// y[t] = sum over the token's pairs, in the order of its slots, of weight * (the pair's down product).  The products are fp16, short of the
-// factor h_scale[pair] * power[expert, column / 32] (see INT8_PAIRS).  One block per token, eight columns a thread.
+// y[t] = sum over the token's pairs, in the order of its slots, of weight * (the pair's down product).  The products are short of the
+// factor h_scale[pair] (fp32), or h_scale[pair] * power[expert, column / 32] (fp16; see INT8_PAIRS).  One block per token, eight columns a
+// thread.
 struct CombineParams {
-  const __half* pairs;
+  const void* pairs;
   int64_t ldp;
   const float *power, *h_scale, *weights;
   const int32_t *place, *ids;
@@ -217,6 +218,8 @@ struct CombineParams {
 template <int DT, bool VEC>
 __global__ void __launch_bounds__(256) combine_kernel(const CombineParams p) {
   using S = typename StorageOf<DT>::type;
+  constexpr bool SCALED = DT == MQ_BF16;     // products in fp16
+  using P = typename StorageOf<SCALED ? MQ_F16 : MQ_F32>::type;
   __shared__ int row_of[2][32], power_of[2][32];
   __shared__ float factor_of[2][32];
   __shared__ int found[2];
@@ -231,8 +234,8 @@ __global__ void __launch_bounds__(256) combine_kernel(const CombineParams p) {
       if (at >= 0) {
         const int i = __popc(have & ((1u << s) - 1u));
         row_of[turn][i] = at;
-        power_of[turn][i] = (__ldcg(p.ids + t * p.top_k + s) - p.first) * p.powers;
-        factor_of[turn][i] = __ldcg(p.weights + t * p.top_k + s) * __ldcg(p.h_scale + at);
+        if (SCALED) power_of[turn][i] = (p.ids[t * p.top_k + s] - p.first) * p.powers;
+        factor_of[turn][i] = p.weights[t * p.top_k + s] * __ldcg(p.h_scale + at);
       }
       if (s == 0) found[turn] = __popc(have);
     }
@@ -240,18 +243,14 @@ __global__ void __launch_bounds__(256) combine_kernel(const CombineParams p) {
     const int n_pairs = found[turn];
     for (int n = threadIdx.x * 8; n < p.N; n += 256 * 8) {
       float sum[8] = {};
+#pragma unroll 2
       for (int i = 0; i < n_pairs; ++i) {
-        const __half* src = p.pairs + (int64_t)row_of[turn][i] * p.ldp + n;
-        const float f = factor_of[turn][i] * __ldcg(p.power + power_of[turn][i] + (n >> 5));
-        if (VEC) {
-          const Eight<__half> a = *reinterpret_cast<const Eight<__half>*>(src);
+        const P* src = static_cast<const P*>(p.pairs) + (int64_t)row_of[turn][i] * p.ldp + n;
+        const float f = factor_of[turn][i] * (SCALED ? __ldcg(p.power + power_of[turn][i] + (n >> 5)) : 1.0f);
+        // (rows of products have room for a multiple of sixteen)
+        const Eight<P> a = *reinterpret_cast<const Eight<P>*>(src);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) sum[j] = fmaf(f, __half2float(a.v[j]), sum[j]);
-        } else {
-#pragma unroll
-          for (int j = 0; j < 8; ++j)
-            if (n + j < p.N) sum[j] = fmaf(f, __half2float(src[j]), sum[j]);
-        }
+        for (int j = 0; j < 8; ++j) sum[j] = fmaf(f, to_float(a.v[j]), sum[j]);
       }
       S* out = static_cast<S*>(p.y) + t * p.ldy + n;
       if (VEC) {
@@ -352,11 +351,11 @@ struct ExpertsBuffers {
   void* plan;
   int8_t *x_codes, *h_codes;
   float *x_scale, *h_scale, *h, *power;
-  __half* pairs;
+  void* pairs;
 };
 // Carves the buffers out of ws, or adds up their bytes where there is none.  The products of the pairs take the place of the tokens'
 // codes and of the gated values, which have been read by then.
-size_t experts_buffers(int64_t T, int k, int E, int64_t K, int64_t I, Workspace* ws, ExpertsBuffers* b) {
+size_t experts_buffers(int dtype, int64_t T, int k, int E, int64_t K, int64_t I, Workspace* ws, ExpertsBuffers* b) {
   const size_t P = (size_t)T * k;
   size_t total = 0;
   auto take = [&](size_t bytes) -> char* {
@@ -373,11 +372,11 @@ size_t experts_buffers(int64_t T, int k, int E, int64_t K, int64_t I, Workspace*
   x.h_scale = reinterpret_cast<float*>(take(P * 4));
   x.power = reinterpret_cast<float*>(take((size_t)E * ceil_div(K, 32) * 4));
   x.h_codes = reinterpret_cast<int8_t*>(take(P * (size_t)pitch_of(I)));
-  const size_t codes = align_up(P * (size_t)pitch_of(K), 256), h = align_up(P * (size_t)pitch_of(I) * 4, 256), pairs = align_up(P * (size_t)pitch_of(K) * 2, 256);
+  const size_t codes = align_up(P * (size_t)pitch_of(K), 256), h = align_up(P * (size_t)pitch_of(I) * 4, 256), pairs = align_up(P * (size_t)pitch_of(K) * (dtype == MQ_BF16 ? 2 : 4), 256);
   char* shared = take(codes + h > pairs ? codes + h : pairs);
   x.x_codes = reinterpret_cast<int8_t*>(shared);
   x.h = reinterpret_cast<float*>(shared + codes);
-  x.pairs = reinterpret_cast<__half*>(shared);
+  x.pairs = shared;
   if (b) *b = x;
   return total;
 }
@@ -393,8 +392,8 @@ int launch_combine(const CombineParams& p, cudaStream_t st) {
 }  // namespace
 }  // namespace mq
 
-extern "C" size_t mq_int8_experts_workspace_bytes(int64_t T, int top_k, int64_t E, int64_t K, int64_t I) {
-  return experts_buffers(T, top_k, (int)E, K, I, nullptr, nullptr);
+extern "C" size_t mq_int8_experts_workspace_bytes(int dtype, int64_t T, int top_k, int64_t E, int64_t K, int64_t I) {
+  return experts_buffers(dtype, T, top_k, (int)E, K, I, nullptr, nullptr);
 }
 
 extern "C" int mq_int8_experts(const void* x, int dtype, int64_t T, int64_t K, int64_t ldx, const int32_t* ids, const float* weights, int top_k,
@@ -414,12 +413,12 @@ extern "C" int mq_int8_experts(const void* x, int dtype, int64_t T, int64_t K, i
   MQ_REQUIRE(x && ids && weights && gate_up && gate_up_scale && down && down_scale && y, MQ_ERR_ARGUMENT, "mq_int8_experts: null pointer");
   MQ_REQUIRE(aligned(gate_up, 16) && aligned(down, 16) && ld_gate_up % 16 == 0 && ld_down % 16 == 0 && gate_up_expert % 16 == 0 && down_expert % 16 == 0,
              MQ_ERR_ALIGNMENT, "mq_int8_experts: rows of 8-bit codes must start on 16-byte boundaries");
-  const size_t need = mq_int8_experts_workspace_bytes(T, top_k, E, K, I);
+  const size_t need = mq_int8_experts_workspace_bytes(dtype, T, top_k, E, K, I);
   MQ_REQUIRE(workspace && aligned(workspace, 16) && workspace_bytes >= need, MQ_ERR_WORKSPACE, "mq_int8_experts: the workspace has %zu bytes and needs %zu",
              workspace_bytes, need);
   Workspace ws(workspace, workspace_bytes);
   ExpertsBuffers b;
-  experts_buffers(T, top_k, (int)E, K, I, &ws, &b);
+  experts_buffers(dtype, T, top_k, (int)E, K, I, &ws, &b);
   const int64_t P = T * top_k;
   Int8Product up = {}, dn = {};
   up.w = gate_up; up.ldw = ld_gate_up; up.w_expert = gate_up_expert; up.w_scale = gate_up_scale;
@@ -444,7 +443,7 @@ extern "C" int mq_int8_experts(const void* x, int dtype, int64_t T, int64_t K, i
   MQ_TRY(int8_product_umma(up, Int8Out{INT8_GATED, MQ_F32, b.h, pitch_of(I), nullptr, nullptr}, nullptr, st));
   MQ_TRY(quantize_rows(MQ_F32, RowsParams{b.h, pitch_of(I), P, b.offsets + E, nullptr, 0, (int)I, b.h_codes, pitch_of(I), b.h_scale}, st));
   dn.x = b.h_codes; dn.ldx = pitch_of(I); dn.x_rows = P; dn.x_scale = b.h_scale; dn.offsets = b.offsets;
-  MQ_TRY(int8_product_umma(dn, Int8Out{INT8_PAIRS, MQ_F16, b.pairs, pitch_of(K), nullptr, b.power}, nullptr, st));
+  MQ_TRY(int8_product_umma(dn, Int8Out{INT8_PAIRS, dtype == MQ_BF16 ? MQ_F16 : MQ_F32, b.pairs, pitch_of(K), nullptr, b.power}, nullptr, st));
   const CombineParams c = {b.pairs, pitch_of(K), b.power, b.h_scale, weights, b.place, ids, (int)first, top_k, (int)K, (int)ceil_div(K, 32), T, y, ldy};
   return dtype == MQ_BF16 ? launch_combine<MQ_BF16>(c, st) : launch_combine<MQ_F16>(c, st);
 }

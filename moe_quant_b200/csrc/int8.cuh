@@ -2,6 +2,7 @@
 #pragma once
 
 #include "common.cuh"
+#include "mbarrier.cuh"
 
 namespace mq {
 
@@ -26,11 +27,11 @@ struct Int8Product {
 enum Int8Result {
   INT8_Y = 0,      // y = sum * x_scale * w_scale + bias, in the result's type
   INT8_GATED = 1,  // weights are gate rows and up rows, `rows` of either: h = silu(gate) * up, fp32
-  // The products of the pairs, short of x_scale and of a power of two per 32 columns, in fp16: sum * w_scale / power[e, n / 32] with
-  // power = 2^k p, p the power of two above the 32 scales and 2^k the one that brings any sum (at most 127 * 128 * K) to 2^15.  It cannot
-  // overflow, and keeps 11 bits down to a sum of 1 (for K up to 32768) times a scale of the column's neighbours; what is smaller
-  // is off by 2^-25 of the power.  Half the bytes of fp32; the sum over a token's pairs and the result's own rounding
-  // (2^-8, 2^-11) come after it.
+  // The products of the pairs, short of x_scale: sum * w_scale in fp32, or (for results of 8 significant bits) short of a power of two per
+  // 32 columns in fp16: sum * w_scale / power[e, n / 32] with power = 2^k p, p the power of two above the 32 scales and 2^k the one
+  // that brings any sum (at most 127 * 128 * K) to 2^15.  It cannot overflow, and keeps 11 bits down to a sum of 1 (for K up to 32768)
+  // times a scale of the column's neighbours; what is smaller is off by 2^-25 of the power.  Half the bytes, and against the 2^-8 of the
+  // results' own rounding nothing; for fp16 results it would raise the error by 1.4.
   INT8_PAIRS = 2,
   INT8_SUMS = 3,   // the sums themselves, of a share of k (within int8_umma.cu)
 };
@@ -40,7 +41,7 @@ struct Int8Out {
   void* y;
   int64_t ldy;
   const float* bias;
-  float* power;    // INT8_PAIRS: (E, ceil(rows / 32)), written by the product
+  float* power;    // INT8_PAIRS in fp16: (E, ceil(rows / 32)), written by the product
 };
 
 // On the tensor cores (int8_umma.cu).  `scratch`: int8_umma_scratch_bytes bytes on a 16-byte boundary, or NULL (then no tile's k is shared
@@ -56,5 +57,28 @@ int int8_few(const void* x, int dtype, int64_t ldx, const Int8Product& p, const 
 bool int8_one_token_fits(int top_k, int64_t K, int64_t I);
 int int8_one_token(const void* x, int dtype, const int32_t* ids, const float* weights, int top_k, int first, const Int8Product& up,
                    const Int8Product& down, float* h, void* y, cudaStream_t st);
+
+// Once per device: the word that waits record their codes in, and the shared memory that a kernel may take.  Looking them up in every
+// call cost 2 us of the 6 of a call.
+inline int fault_word(int** out) {
+  static int* word[64] = {};
+  int dev = 0;
+  MQ_CUDA(cudaGetDevice(&dev));
+  if (dev >= 64) return engine_fault_word(out);
+  if (!word[dev]) MQ_TRY(engine_fault_word(&word[dev]));
+  *out = word[dev];
+  return MQ_OK;
+}
+template <auto KERNEL>
+int allow_smem(size_t bytes) {
+  static bool ready[64] = {};
+  int dev = 0;
+  MQ_CUDA(cudaGetDevice(&dev));
+  if (dev >= 64 || !ready[dev]) {
+    MQ_CUDA(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    if (dev < 64) ready[dev] = true;
+  }
+  return MQ_OK;
+}
 
 }  // namespace mq

@@ -358,10 +358,10 @@ __global__ void __launch_bounds__(ONE_THREADS, 1) one_token_down_kernel(const On
   }
 }
 
-template <typename Params>
-int launch_few(void (*kernel)(Params), int threads, size_t smem, const Params& p, cudaStream_t st) {
-  MQ_CUDA(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)FEW_SMEM));
-  MQ_CUDA(launch_chained(true, kernel, dim3(FEW_BLOCKS), dim3((unsigned)threads), smem, st, p));
+template <auto KERNEL, typename Params>
+int launch_few(int threads, size_t smem, const Params& p, cudaStream_t st) {
+  MQ_TRY(allow_smem<KERNEL>(FEW_SMEM));
+  MQ_CUDA(launch_chained(true, KERNEL, dim3(FEW_BLOCKS), dim3((unsigned)threads), smem, st, p));
   MQ_LAUNCH_CHECK();
   return MQ_OK;
 }
@@ -374,8 +374,8 @@ bool rows_of_eight(const void* x, int64_t ldx, int64_t K, int64_t T) {
 template <int DT, int NT>
 int few(const FewParams& p, cudaStream_t st) {
   const size_t smem = (size_t)NT * few_pitch(p.K) + FEW_RINGS;
-  if constexpr (DT == MQ_I8) return launch_few(int8_few_kernel<DT, NT, true>, FEW_THREADS, smem, p, st);
-  else return rows_of_eight<DT>(p.x, p.ldx, p.K, p.T) ? launch_few(int8_few_kernel<DT, NT, true>, FEW_THREADS, smem, p, st) : launch_few(int8_few_kernel<DT, NT, false>, FEW_THREADS, smem, p, st);
+  if constexpr (DT == MQ_I8) return launch_few<int8_few_kernel<DT, NT, true>>(FEW_THREADS, smem, p, st);
+  else return rows_of_eight<DT>(p.x, p.ldx, p.K, p.T) ? launch_few<int8_few_kernel<DT, NT, true>>(FEW_THREADS, smem, p, st) : launch_few<int8_few_kernel<DT, NT, false>>(FEW_THREADS, smem, p, st);
 }
 template <int DT>
 int few_of(const FewParams& p, cudaStream_t st) {
@@ -387,8 +387,11 @@ int few_of(const FewParams& p, cudaStream_t st) {
 template <int DT>
 int one_token(const OneParams& p, cudaStream_t st) {
   const size_t smem = (size_t)few_pitch(p.K) + FEW_RINGS;
-  MQ_TRY(rows_of_eight<DT>(p.x, 0, p.K, 1) ? launch_few(one_token_gated_kernel<DT, true>, ONE_THREADS, smem, p, st) : launch_few(one_token_gated_kernel<DT, false>, ONE_THREADS, smem, p, st));
-  return launch_few(one_token_down_kernel<DT>, ONE_THREADS, one_token_down_codes(p.top_k, p.K, p.I) + FEW_RINGS, p, st);
+  int status;
+  if (rows_of_eight<DT>(p.x, 0, p.K, 1)) status = launch_few<one_token_gated_kernel<DT, true>>(ONE_THREADS, smem, p, st);
+  else status = launch_few<one_token_gated_kernel<DT, false>>(ONE_THREADS, smem, p, st);
+  MQ_TRY(status);
+  return launch_few<one_token_down_kernel<DT>>(ONE_THREADS, one_token_down_codes(p.top_k, p.K, p.I) + FEW_RINGS, p, st);
 }
 
 }  // namespace
@@ -397,7 +400,7 @@ bool int8_few_fits(int64_t T, int64_t K) { return T <= INT8_FEW_TOKENS && (T <= 
 
 int int8_few(const void* x, int dtype, int64_t ldx, const Int8Product& q, const Int8Out& o, cudaStream_t st) {
   FewParams p = {x, q.x_scale, ldx, (int)q.T, q.rows, q.K, q.w, q.ldw, q.w_scale, o.bias, o.dtype, o.y, o.ldy, nullptr};
-  MQ_TRY(engine_fault_word(&p.fault));
+  MQ_TRY(fault_word(&p.fault));
   if (dtype == MQ_I8) return few_of<MQ_I8>(p, st);
   if (dtype == MQ_F32) return few_of<MQ_F32>(p, st);
   if (dtype == MQ_BF16) return few_of<MQ_BF16>(p, st);
@@ -412,7 +415,7 @@ int int8_one_token(const void* x, int dtype, const int32_t* ids, const float* we
                    float* h, void* y, cudaStream_t st) {
   OneParams p = {x, up.K, up.rows, up.E, top_k, first, ids, weights, up.w, down.w, up.ldw, up.w_expert, down.ldw, down.w_expert,
                        up.w_scale, down.w_scale, h, y, nullptr};
-  MQ_TRY(engine_fault_word(&p.fault));
+  MQ_TRY(fault_word(&p.fault));
   return dtype == MQ_BF16 ? one_token<MQ_BF16>(p, st) : one_token<MQ_F16>(p, st);
 }
 

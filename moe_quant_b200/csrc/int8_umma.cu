@@ -145,7 +145,7 @@ __device__ __forceinline__ void store_rows(uint32_t tile, int lane, S* out, int6
   __syncwarp();
 }
 
-// DT: type of y (INT8_Y)
+// DT: type of what is stored (INT8_Y, INT8_PAIRS)
 template <int KIND, int DT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
     int8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_x, const PairArgs a) {
@@ -296,7 +296,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
       const bool col_in = col < p.rows;
       const int w_row = KIND == INT8_GATED ? (lane >> 4) * p.rows + col : col;
       float ws = col_in ? __ldg(p.w_scale + (int64_t)u.e * SETS * p.rows + w_row) : 0.0f;
-      if constexpr (KIND == INT8_PAIRS) {
+      if constexpr (KIND == INT8_PAIRS && DT == MQ_F16) {
         const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(ws) & 0x7FFFFFFFu);
         // the power of two above the 32 scales; nothing to take out of zeros, and nothing that helps infinities and NaN
         const int e2 = most == 0u || most >= 0x7F800000u ? 127 : min((int)(most >> 23) + 1, 253);
@@ -376,7 +376,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
           }
           __syncwarp();
         } else {
-          using S = typename StorageOf<KIND == INT8_PAIRS ? MQ_F16 : DT>::type;
+          using S = typename StorageOf<DT>::type;
           if constexpr (KIND == INT8_Y) {
 #pragma unroll
             for (int j = 0; j < 32; ++j) v[j] += bias;
@@ -458,13 +458,7 @@ int encode(EncodeTiledFn enc, CUtensorMap* map, int rank, const void* base, cons
 
 template <int KIND, int DT = MQ_F32>
 int launch(const CUtensorMap& map_w, const CUtensorMap& map_x, const PairArgs& a, int pairs, cudaStream_t st) {
-  static bool ready[64] = {};
-  int dev = 0;
-  MQ_CUDA(cudaGetDevice(&dev));
-  if (dev >= 64 || !ready[dev]) {
-    MQ_CUDA(cudaFuncSetAttribute(int8_pair_kernel<KIND, DT>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kInt8Smem));
-    if (dev < 64) ready[dev] = true;
-  }
+  MQ_TRY((allow_smem<int8_pair_kernel<KIND, DT>>(kInt8Smem)));
   MQ_CUDA(launch_chained(true, int8_pair_kernel<KIND, DT>, dim3((unsigned)(2 * pairs)), dim3(I8_THREADS), kInt8Smem, st, map_w, map_x, a));
   MQ_LAUNCH_CHECK();
   return MQ_OK;
@@ -520,7 +514,7 @@ int int8_product_umma(const Int8Product& p, const Int8Out& o, void* scratch, cud
   PairArgs a = {};
   a.p = p;
   a.o = o;
-  MQ_TRY(engine_fault_word(&a.fault));
+  MQ_TRY(fault_word(&a.fault));
   const int sets = o.kind == INT8_GATED ? 2 : 1;
   CUtensorMap map_w, map_x;
   {
@@ -557,7 +551,8 @@ int int8_product_umma(const Int8Product& p, const Int8Out& o, void* scratch, cud
   while ((int64_t)p.K > (2ll << a.sum_shift)) ++a.sum_shift;   // 127 * 128 * K / 2^shift < 2^14 K / 2^shift <= 2^15
   a.packed = p.rows % piece == 0 && o.ldy % piece == 0 && aligned(o.y, 16);
   if (o.kind == INT8_GATED) return launch<INT8_GATED>(map_w, map_x, a, pairs, st);
-  if (o.kind == INT8_PAIRS) return launch<INT8_PAIRS>(map_w, map_x, a, pairs, st);
+  if (o.kind == INT8_PAIRS && o.dtype == MQ_F32) return launch<INT8_PAIRS, MQ_F32>(map_w, map_x, a, pairs, st);
+  if (o.kind == INT8_PAIRS) return launch<INT8_PAIRS, MQ_F16>(map_w, map_x, a, pairs, st);
   if (o.dtype == MQ_F32) return launch<INT8_Y, MQ_F32>(map_w, map_x, a, pairs, st);
   if (o.dtype == MQ_BF16) return launch<INT8_Y, MQ_BF16>(map_w, map_x, a, pairs, st);
   return launch<INT8_Y, MQ_F16>(map_w, map_x, a, pairs, st);

@@ -598,10 +598,11 @@ def int8_experts(x: Tensor, ids: Tensor, weights: Tensor, gate_up: Tensor, gate_
     dev = x.device
     y = torch.empty(*x.shape[:-1], K, dtype=x.dtype, device=dev)
     L = lib()
-    nbytes = L.mq_int8_experts_workspace_bytes(T, k, E, K, I) if T and k and E else 0
+    code = dtype_code(x.dtype)
+    nbytes = L.mq_int8_experts_workspace_bytes(code, T, k, E, K, I) if T and k and E else 0
     ws = _scratch(dev, nbytes)
     with _lib.on_device(dev):
-        check(L.mq_int8_experts(ptr(rows), dtype_code(x.dtype), T, K, _pitch(rows), ptr(ids), ptr(weights), k, first, E, I, ptr(gate_up),
+        check(L.mq_int8_experts(ptr(rows), code, T, K, _pitch(rows), ptr(ids), ptr(weights), k, first, E, I, ptr(gate_up),
                                 _code_pitch(gate_up), gate_up.stride(0) if E > 1 else 0, ptr(gate_up_scale), ptr(down), _code_pitch(down),
                                 down.stride(0) if E > 1 else 0, ptr(down_scale), ptr(y), K, ptr(ws), nbytes, stream_ptr(dev)))
     return y
