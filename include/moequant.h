@@ -305,7 +305,7 @@ size_t mq_expert_plan_workspace_bytes(int64_t pairs, int64_t E);
 int mq_quantize_tokens(const void* x, int dtype, int64_t T, int64_t K, int64_t ldx, int8_t* codes, int64_t ldc, float* scale,
                        void* stream);
 
-/* y[t, n] = (sum over k of code[t, k] w[n, k]) x_scale[t] w_scale[n] + bias[n], the sum exact in 32-bit integers (K <= 131072).
+/* y[t, n] = (sum over k of code[t, k] w[n, k]) x_scale[t] w_scale[n] + bias[n], the sum exact in 32-bit integers (K <= 131072, for MQ_I8 one less).
  * x (T, K) of x_dtype gets its codes as mq_quantize_tokens gives them (x_scale is not read), or is codes already (MQ_I8) with
  * their scales.  w (N, K) int8; rows of codes start on 16-byte boundaries.  bias may be NULL.  y (T, N) of out_dtype.  */
 int mq_int8_matmul(const void* x, int x_dtype, const float* x_scale, int64_t T, int64_t K, int64_t ldx, const int8_t* w, int64_t N,

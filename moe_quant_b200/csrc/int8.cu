@@ -312,8 +312,10 @@ extern "C" int mq_int8_matmul(const void* x, int x_dtype, const float* x_scale, 
   MQ_REQUIRE(T >= 0 && N >= 0 && K >= 1 && ldx >= K && ldw >= K && ldy >= N, MQ_ERR_ARGUMENT,
              "mq_int8_matmul: bad sizes T=%lld N=%lld K=%lld ldx=%lld ldw=%lld ldy=%lld", (long long)T, (long long)N, (long long)K, (long long)ldx,
              (long long)ldw, (long long)ldy);
-  MQ_REQUIRE(K <= INT8_MAX_K, MQ_ERR_UNSUPPORTED, "mq_int8_matmul: K is at most %lld, so that a sum of products fits 32 bits (got %lld)",
-             (long long)INT8_MAX_K, (long long)K);
+  // (codes of the caller's may all be -128)
+  const int64_t most_k = x_dtype == MQ_I8 ? INT8_MAX_K - 1 : INT8_MAX_K;
+  MQ_REQUIRE(K <= most_k, MQ_ERR_UNSUPPORTED, "mq_int8_matmul: K is at most %lld, so that a sum of products fits 32 bits (got %lld)",
+             (long long)most_k, (long long)K);
   MQ_REQUIRE(T < (1ll << 31) - 256 && N < (1ll << 31) - 256, MQ_ERR_UNSUPPORTED, "mq_int8_matmul: too many tokens or rows");
   if (T == 0 || N == 0) return MQ_OK;
   MQ_REQUIRE(x && w && w_scale && y && (x_dtype != MQ_I8 || x_scale), MQ_ERR_ARGUMENT, "mq_int8_matmul: null pointer");

@@ -22,6 +22,29 @@ constexpr float NEAR_MIDDLE = 0.49999f;
 template <typename T>
 struct alignas(8 * sizeof(T)) Eight { T v[8]; };
 
+// the eight values as fp32, from whole words (taken one by one, halves of words cost several instructions each)
+__device__ __forceinline__ void to_floats(const Eight<float>& a, float (&x)[8]) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) x[j] = a.v[j];
+}
+__device__ __forceinline__ void to_floats(const Eight<__nv_bfloat16>& a, float (&x)[8]) {
+  const uint32_t* w = reinterpret_cast<const uint32_t*>(a.v);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    x[2 * j] = __uint_as_float(w[j] << 16);
+    x[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
+  }
+}
+__device__ __forceinline__ void to_floats(const Eight<__half>& a, float (&x)[8]) {
+  const __half2* w = reinterpret_cast<const __half2*>(a.v);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float2 f = __half22float2(w[j]);
+    x[2 * j] = f.x;
+    x[2 * j + 1] = f.y;
+  }
+}
+
 __device__ __forceinline__ float max3_abs_nan(float a, float b, float c) {   // NaN if one is
   float v;
   asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(v) : "f"(a), "f"(b), "f"(c));
@@ -91,19 +114,19 @@ struct RowCodes {
   }
   template <typename T>
   __device__ __forceinline__ uint2 of(const Eight<T>& a) const {
-    float r[8];
+    float r[8], x[8];
+    to_floats(a, x);
     if constexpr (sizeof(T) == 2) {
       if (careful_from < 0.0f) return careful_codes(a, top, inv, lift);
 #pragma unroll
       for (int j = 0; j < 8; ++j)
-        r[j] = __uint_as_float((__float_as_uint(to_float(a.v[j]) * inv) + 8u) & ~15u) + TO_INTEGER;
+        r[j] = __uint_as_float((__float_as_uint(x[j] * inv) + 8u) & ~15u) + TO_INTEGER;
     } else {
       float off[8];
 #pragma unroll
       for (int j = 0; j < 8; ++j) {
-        const float x = to_float(a.v[j]);
-        r[j] = __fmaf_rn(x, inv, TO_INTEGER);
-        off[j] = __fmaf_rn(x, inv, TO_INTEGER - r[j]);
+        r[j] = __fmaf_rn(x[j], inv, TO_INTEGER);
+        off[j] = __fmaf_rn(x[j], inv, TO_INTEGER - r[j]);
       }
       const float far = max3_abs_nan(max3_abs_nan(off[0], off[1], off[2]), max3_abs_nan(off[3], off[4], off[5]), max3_abs_nan(off[6], off[7], 0.0f));
       if (!(far <= careful_from)) return careful_codes(a, top, inv, lift);

@@ -74,7 +74,7 @@ def _whole(codes: Tensor) -> Tensor:
 def int8_block(block: nn.Module, results: Mapping[str, Tuple[Tensor, Tensor, Tensor]]):
     """Within the context the block's quantized layers run in 8-bit integers: `results` maps their names to what quantize(8)
     returned.  A module whose experts are all among them, and which has a place for it (`int8_experts`), runs them through
-    ops.int8_experts; every other layer becomes an Int8Linear."""
+    ops.int8_experts (in bf16 and fp16 blocks); every other layer becomes an Int8Linear."""
     undo = []
     left = dict(results)
     try:
@@ -86,6 +86,8 @@ def int8_block(block: nn.Module, results: Mapping[str, Tuple[Tensor, Tensor, Ten
             ids = sorted({int(m.group(1)) for m in (re.fullmatch(r"(\d+)\.(gate|up|down)_proj", n) for n in mine) if m})
             sides = [[left.get(f"{prefix}{i}.{side}_proj") for i in ids] for side in ("gate", "up", "down")]
             local = [i for i, e in enumerate(moe.experts) if e is not None]
+            if any(left[n][1].dtype == torch.float32 for n in mine.values()):
+                continue
             if not ids or ids != local or ids != list(range(ids[0], ids[-1] + 1)) or any(r is None for side in sides for r in side):
                 continue
             moe.int8_experts = Int8Experts(*sides, first=ids[0])

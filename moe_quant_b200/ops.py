@@ -419,7 +419,7 @@ def _int32(t: Tensor, what: str) -> Tensor:
         return t
     if t.dtype not in (torch.int32, torch.int64):
         raise MoeQuantError(f"{what} must be int32 or int64 (got {t.dtype})")
-    return t.to(torch.int32).contiguous()
+    return t.clamp(-1, 2 ** 31 - 1).to(torch.int32).contiguous()   # (what lies outside is no expert's number, and must not become one)
 
 
 def _fp32(t: Tensor) -> Tensor:
@@ -480,8 +480,8 @@ def route_tokens(logits: Tensor, top_k: int, *, score: str = "softmax", bias: Op
     if score not in ("softmax", "sigmoid") or group_score not in ("max", "top2"):
         raise MoeQuantError(f"route_tokens: unknown score {score!r} or group_score {group_score!r}")
     _forward_only("route_tokens", logits, bias)
-    if logits.dim() < 1:
-        raise MoeQuantError("route_tokens: logits must be (..., E)")
+    if logits.dim() < 1 or top_k < 1:
+        raise MoeQuantError("route_tokens: logits must be (..., E) and top_k at least 1")
     E, lead = logits.shape[-1], logits.shape[:-1]
     if bias is not None:
         _same_device("route_tokens", logits.device, bias)

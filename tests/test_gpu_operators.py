@@ -285,6 +285,35 @@ def test_int8_matmul_of_the_largest_sums(cuda):
         assert torch.all((y.cpu().double() - want).abs() <= 5 * 2.0 ** -24 * want.abs())
 
 
+def test_int8_matmul_of_the_lowest_codes(cuda):
+    """-128 on both sides over the longest row that is allowed."""
+    K = 131071
+    w = torch.full((2, K + 1), -128, dtype=torch.int8, device=cuda)[:, :K]
+    for T in (1, 20):
+        q = torch.full((T, K + 1), -128, dtype=torch.int8, device=cuda)[:, :K]
+        y = ops.int8_matmul(q, w, torch.ones(2, device=cuda), x_scale=torch.ones(T, device=cuda), out_dtype=FP32)
+        assert torch.all((y.double() - 16384.0 * K).abs() <= 3 * 2.0 ** -24 * 16384.0 * K)
+
+
+def test_offsets_beyond_32_bits(cuda):
+    """More than 2^31 values in, and out: the last rows are as in a call of their own."""
+    T, K = 300007, 7168
+    x = torch.empty(T, K, dtype=BF16, device=cuda)
+    x[:64] = 0.0
+    x[64:].copy_(torch.randn(1, K, device=cuda).to(BF16).expand(T - 64, K))
+    x[-64:] = torch.randn(64, K, device=cuda).to(BF16)
+    codes, scale = ops.quantize_tokens(x)
+    tail, tail_scale = ops.quantize_tokens(x[-64:].clone())
+    assert torch.equal(codes[-64:], tail) and torch.equal(scale[-64:], tail_scale) and not torch.any(codes[:64])
+    assert torch.equal(codes[T // 2], codes[64])
+    del codes
+    w = torch.randint(-128, 128, (8200, K), dtype=torch.int8, device=cuda)
+    y = ops.int8_matmul(x, w, torch.ones(8200, device=cuda))
+    assert y.numel() > 2 ** 31
+    assert torch.equal(y[-64:], ops.int8_matmul(x[-64:].clone(), w, torch.ones(8200, device=cuda)))
+    assert torch.equal(y[T // 2], y[64]) and not torch.any(y[:64])
+
+
 @pytest.mark.parametrize("T", [2, 30, 200])
 def test_int8_matmul_broken_and_zero_tokens(cuda, T):
     x = _tokens(T, 320, BF16, 1)
@@ -377,6 +406,28 @@ def test_int8_experts_without_pairs_and_with_crowded_ones(cuda, T):
     _check_experts(ops.int8_experts(**_on(c, cuda)), c)
     c["ids"][T // 2:] = 7                                        # an expert of another rank
     _check_experts(ops.int8_experts(**_on(c, cuda)), c)
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+def test_int8_experts_of_the_largest_sums(cuda, dtype):
+    """Every product of the down projection at its limit: h codes of 127 against weights of -128 and 127, scales that differ by 2^20."""
+    T, K, I = 40, 64, 4096
+    x = torch.ones(T, 16, dtype=dtype)
+    gu, gus = torch.full((1, 2 * I, 16), 127, dtype=torch.int8), torch.full((1, 2 * I), 1.0 / 127 / 16)
+    d = torch.full((1, 16, I), -128, dtype=torch.int8)
+    d[0, 1::2] = 127
+    ds = torch.full((1, 16), 1e-4)
+    ds[0, 3], ds[0, 4] = 1e-4 * 2.0 ** -20, 3.9e-4
+    c = dict(x=x, ids=torch.zeros(T, 1, dtype=torch.int32), weights=torch.ones(T, 1), gate_up=gu, gate_up_scale=gus, down=d, down_scale=ds, first=0)
+    y = ops.int8_experts(**_on(c, cuda))
+    assert torch.all(torch.isfinite(y))
+    _check_experts(y, c)
+
+
+def test_ids_outside_32_bits_are_no_expert(cuda):
+    ids = torch.tensor([[2 ** 32 + 1, 1], [-2 ** 40, 0]], device=cuda)
+    p = ops.expert_plan(ids, 2)
+    assert p.offsets.tolist() == [0, 1, 2] and p.place.tolist() == [[-1, 1], [-1, 0]]
 
 
 @pytest.mark.parametrize("T", [1, 5, 100])
@@ -492,7 +543,7 @@ def test_wrapper_refusals(cuda):
            lambda: ops.int8_matmul(x, w, s, bias=s[:4]), lambda: ops.int8_matmul(x, w.t()[:, :32].t(), s, out_dtype=torch.float64),
            lambda: ops.int8_matmul(x[:, 8:24], w[:, 8:24], s), lambda: ops.int8_matmul(x[:, :16], w.reshape(16, 16)[:8].t().contiguous().t(), s),
            lambda: ops.int8_matmul(x, w, s.cpu()), lambda: ops.int8_matmul(x[:, :20], torch.zeros(8, 20, dtype=torch.int8, device=cuda), s),
-           lambda: ops.route_tokens(x, 0), lambda: ops.route_tokens(x, 33), lambda: ops.route_tokens(x, 2, score="tanh"), lambda: ops.route_tokens(x, 2, groups=5),
+           lambda: ops.route_tokens(x, 0), lambda: ops.route_tokens(x, -1), lambda: ops.route_tokens(x, 33), lambda: ops.route_tokens(x, 2, score="tanh"), lambda: ops.route_tokens(x, 2, groups=5),
            lambda: ops.route_tokens(x, 2, bias=s), lambda: ops.route_tokens(x.to(torch.int8), 2), lambda: ops.route_tokens(x, 2, groups=4, keep_groups=5),
            lambda: ops.expert_plan(weights, 4), lambda: ops.expert_plan(ids, 0), lambda: ops.expert_plan(ids, 2000), lambda: ops.expert_plan(ids, 4, first=-1),
            lambda: ops.int8_experts(x, ids, weights, gu, gus, d, ds), lambda: ops.int8_experts(h, ids[:3], weights[:3], gu, gus, d, ds),
@@ -569,6 +620,16 @@ def test_block_driver_gives_the_outputs_of_the_served_block(cuda):
     for a, b, x in zip(got["outputs"], want["outputs"], inputs):
         assert a.shape == b.shape and bool(torch.isfinite(a).all())
         assert float((a - b).float().norm() / (b - x).float().norm()) < 0.1
+
+
+def test_block_driver_of_an_fp32_block(cuda):
+    block = SyntheticMoEBlock(hidden=64, inter=32, n_experts=4, top_k=2, q_rank=32, kv_rank=32, n_heads=2, nope_dim=16, rope_dim=16, v_dim=32, seed=1).to(cuda)
+    x = _tokens(80, 64, FP32, 3).to(cuda)[None]
+    plain = copy.deepcopy(block)
+    a = quantize_block(block, [x], bits=8, group_size=None, int8_outputs=True)["outputs"][0]
+    b = quantize_block(plain, [x], bits=8, group_size=None)["outputs"][0]
+    assert a.dtype == FP32 and bool(torch.isfinite(a).all())
+    assert float((a - b).norm() / (b - x).norm()) < 0.1
 
 
 def test_block_runs_its_experts_by_the_operators(cuda):

@@ -60,7 +60,7 @@ def test_quantize_refusals(change, status):
     ({"x_dtype": 4}, 1), ({"out_dtype": 3}, 1), ({"T": -1}, 1), ({"N": -1}, 1), ({"K": 0}, 1), ({"ldx": 60}, 1), ({"ldw": 60}, 1), ({"ldy": 7}, 1),
     ({"K": 131088, "ldx": 131088, "ldw": 131088}, 3), ({"T": 2 ** 31}, 3), ({"N": 2 ** 31, "ldy": 2 ** 31}, 3), ({"x": None}, 1), ({"w": None}, 1),
     ({"w_scale": None}, 1), ({"y": None}, 1), ({"x_dtype": 3}, 1), ({"w": P + 8}, 2), ({"ldw": 72}, 2), ({"x_dtype": 3, "x_scale": P, "x": P + 8}, 2),
-    ({"x_dtype": 3, "x_scale": P, "ldx": 72}, 2), ({"ws": None}, 4), ({"bytes": 16}, 4), ({"ws": P + 8}, 4)])
+    ({"x_dtype": 3, "x_scale": P, "ldx": 72}, 2), ({"x_dtype": 3, "x_scale": P, "K": 131072, "ldx": 131072, "ldw": 131072}, 3), ({"ws": None}, 4), ({"bytes": 16}, 4), ({"ws": P + 8}, 4)])
 def test_matmul_refusals(change, status):
     a = {"x": P, "x_dtype": 1, "x_scale": None, "T": 40, "K": 64, "ldx": 64, "w": P, "N": 8, "ldw": 64, "w_scale": P, "bias": None, "out_dtype": 1,
          "y": P, "ldy": 8, "ws": P, "bytes": 1 << 30, **change}
@@ -125,7 +125,7 @@ def test_int8_experts_stacks_gate_rows_before_up_rows():
 
 
 def _results(block):
-    return {n: (torch.randint(0, 256, l.weight.shape, dtype=torch.uint8), torch.ones(l.weight.shape[0], 1), torch.full((l.weight.shape[0], 1), 128.0))
+    return {n: (torch.randint(0, 256, l.weight.shape, dtype=torch.uint8), torch.ones(l.weight.shape[0], 1, dtype=torch.bfloat16), torch.full((l.weight.shape[0], 1), 128.0))
             for n, l in block.named_modules() if isinstance(l, nn.Linear)}
 
 
@@ -146,6 +146,13 @@ def test_int8_block_swaps_layers_and_puts_them_back():
         assert block.mlp.int8_experts is None and isinstance(block.mlp.experts[0].gate_proj, Int8Linear)
         assert isinstance(block.mlp.experts[2].up_proj, nn.Linear)
     assert dict(block.named_modules()) == before
+
+
+def test_int8_block_of_fp32_layers_goes_layer_by_layer():
+    block = SyntheticMoEBlock(hidden=32, inter=16, n_experts=2, top_k=1, q_rank=16, kv_rank=16, n_heads=2, nope_dim=8, rope_dim=8, v_dim=8)
+    results = {n: (q, s.float(), z) for n, (q, s, z) in _results(block).items()}
+    with int8_block(block, results):
+        assert block.mlp.int8_experts is None and isinstance(block.mlp.experts[1].down_proj, Int8Linear)
 
 
 def test_int8_block_puts_layers_back_after_an_error():
