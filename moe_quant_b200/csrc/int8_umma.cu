@@ -221,7 +221,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
         const int n_boxes = (half + 31) / 32;
         const uint32_t bytes = 2 * (I8_TILE_BYTES + (uint32_t)n_boxes * 32 * I8_K);
         for (int s = u.slab0; s < u.slab1; ++s, ++it) {
-          if (it >= a.stages && !mbar_wait_lane(empty0 + 8 * st, (round - 1) & 1, a.fault, 91)) { ok = false; break; }
+          if (it >= a.stages && !mbar_wait_elected(empty0 + 8 * st, (round - 1) & 1, a.fault, 91)) { ok = false; break; }
           const uint32_t dst = smem_base + (uint32_t)(st * a.stage_bytes), bar = full_leader + 8 * st;
           if (rank == 0) mbar_expect_tx(full0 + 8 * st, bytes);
           if constexpr (KIND == INT8_GATED) {
@@ -240,7 +240,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
         }
       }
       // the last use of every stage has been read (so its copies had landed)
-      for (int j = it > a.stages ? it - a.stages : 0; j < it && ok; ++j) ok = mbar_wait_lane(empty0 + 8 * (j % a.stages), (j / a.stages) & 1, a.fault, 95);
+      for (int j = it > a.stages ? it - a.stages : 0; j < it && ok; ++j) ok = mbar_wait_elected(empty0 + 8 * (j % a.stages), (j / a.stages) & 1, a.fault, 95);
       end.copied_by(rank, it);
       if (!ok) end.give_up();
     }
@@ -257,10 +257,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
         // sums of 32 bits, signed 8-bit operands, 256 rows, `width` columns
         const uint32_t idesc = (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)(u.width >> 3) << 17) | ((uint32_t)(256 >> 4) << 24);
         const uint32_t acc = tmem_acc + (uint32_t)(b * I8_MAX_WIDTH);
-        if (n >= 2) ok = mbar_wait_lane(acc_empty + 8 * b, ((n >> 1) - 1) & 1, a.fault, 93);
+        if (n >= 2) ok = mbar_wait_elected(acc_empty + 8 * b, ((n >> 1) - 1) & 1, a.fault, 93);
         tc_fence_after();
         for (int s = u.slab0; s < u.slab1 && ok; ++s) {
-          ok = mbar_wait_lane(full0 + 8 * st, round & 1, a.fault, 92);
+          ok = mbar_wait_elected(full0 + 8 * st, round & 1, a.fault, 92);
           if (!ok) break;
           tc_fence_after();
           const uint64_t a0 = desc0 + (uint64_t)((uint32_t)(st * a.stage_bytes) >> 4), b0 = a0 + (I8_TILE_BYTES >> 4);

@@ -57,6 +57,8 @@ __device__ __forceinline__ bool mbar_wait_lane(uint32_t bar, uint32_t parity, in
     if ((it & 255u) == 255u && limit.expired(fault, code)) return false;
   }
 }
+// By a thread that issues copies or MMAs alone, elected once for the whole loop: the other lanes of its warp are past it and wait for its end.
+__device__ __forceinline__ bool mbar_wait_elected(uint32_t bar, uint32_t parity, int* fault, int code) { return mbar_wait_lane(bar, parity, fault, code); }
 // By a whole warp.  Its lanes poll one by one, and a barrier may complete between the poll of one that gives up and that of the next:
 // they agree, so that what follows (shuffles, tensor memory loads) is entered by all of them or by none.
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, int* fault, int code) {

@@ -1,5 +1,7 @@
 """Operators of the quantized layers: what needs no device.  Refusals are decided on the host, before any launch."""
 import math
+import os
+import re
 
 import pytest
 import torch
@@ -169,6 +171,16 @@ def test_int8_outputs_need_eight_bits_per_channel():
     for bits, group in ((4, None), (8, 128)):
         with pytest.raises(MoeQuantError, match="bits=8"):
             quantize_block(block, [], bits=bits, group_size=group, int8_outputs=True)
+
+
+def test_only_elected_threads_wait_alone():
+    """Waits of a single thread stand between its election and the point where its warp comes together again."""
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "moe_quant_b200", "csrc")
+    for name in sorted(n for n in os.listdir(csrc) if n.endswith((".cu", ".cuh")) and n != "mbarrier.cuh"):
+        body = open(os.path.join(csrc, name)).read()
+        for at in (m.start() for m in re.finditer(r"mbar_wait_elected\(", body)):
+            elected, joined = body.rfind("elect_one())", 0, at), body.find("__syncwarp();", at)
+            assert elected >= 0 and "__syncwarp" not in body[elected:at] and "_sync(" not in body[elected:joined], name
 
 
 # ------------------------------------------------------------------ the reference itself
