@@ -5,6 +5,10 @@
 //   product           y[t, n] = (sum_k code[t, k] w[n, k]) scale[t] w_scale[n] + bias[n], the sum in 32-bit integers: exact
 //   experts           h = silu(gate product) * up product per pair of token and expert, codes of h as above, and
 //                     y[t] = sum over the token's pairs of weight * down product
+//
+// Here: the codes (bound by memory and by instructions: 16384 x 2048 fp32 5.9 TB/s, 32768 x 2048 bf16 4.8, 16384 x 7168 bf16 4.5), the sum over a
+// token's pairs (5.1 TB/s), and the calls.  The products are in int8_umma.cu (tensor cores, bound by them) and int8_few.cu (up to four tokens,
+// and the experts of one: bound by the weights' bytes).
 #include <math_constants.h>
 
 #include "int8.cuh"

@@ -7,7 +7,7 @@
 //
 // One warp per token, a run of experts per lane.  Which experts come first is decided on fp32 scores wherever these lie further apart than
 // they can be off, and in 64 bits in the rows where some do not (without a bias the logits themselves order the experts: exactly).
-// 65536 tokens, 256 experts in 8 groups with a bias: 192 us with every row in 64 bits.
+// 65536 tokens, 256 experts in 8 groups with a bias: 88 us (0.76 TB/s of logits), 192 with every row in 64 bits.
 #include <math_constants.h>
 
 #include "common.cuh"
@@ -17,6 +17,7 @@ namespace mq {
 namespace {
 
 constexpr int ROUTE_WARPS = 8, EXTRA = 4;
+constexpr size_t SMEM_AS_IS = 47 * 1024;   // of the 48 KB that need no permission, beside what a kernel has of its own
 
 struct RouteParams {
   int64_t T, ld;
@@ -167,11 +168,14 @@ __device__ __forceinline__ float quick_sigmoid(float l) {
   return y;
 }
 
-// Whether a value that came out as `a` may in truth not lie above one that came out as `b` <= a; `size` bounds what the values were summed
-// from.  quick_sigmoid is off by 4e-7 at most (the exponential by 2^-22 and by 9e-8 |l|, times s (1 - s); sum and reciprocal by
-// 2^-23 each), the sum with the bias by 2^-24 |v|, a softmax score by 3.2e-6 (its sum over up to 1024 experts, 32 in a lane and five levels of
-// lanes, and the exponentials), and the low bits that give way to an index by 2^-23 VPL |v|.  Two values, or two sums of two.
-__device__ __forceinline__ bool too_near(float a, float b, float tolerance, float size) { return !(a - b > tolerance * (1.0f + size)); }
+// How far a value may be off.  quick_sigmoid by 4e-7 at most (the exponential by 2^-22 and by 9e-8 |l|, times s (1 - s); sum and reciprocal by
+// 2^-23 each), a softmax score by 3.2e-6 (its sum over up to 1024 experts, 32 in a lane and five levels of lanes, and the exponentials); the sum
+// with the bias adds 2^-24 |v|.  So of two values the larger is certain where they are apart by 8e-7 (6.4e-6) + 1.2e-7 |v|, and by
+// 2^-23 VPL |v| more where low bits have given way to an index; of two sums of two values by 1.6e-6 (1.3e-5) + 2.4e-7 of what was summed.
+struct Margin {
+  float fixed, per_size;
+  __device__ __forceinline__ bool certain(float a, float b, float size) const { return a - b > fixed + per_size * size; }   // no for NaN
+};
 
 // Descending, by a network of compare-exchanges (odd-even merges).
 template <int N>
@@ -191,8 +195,9 @@ __device__ __forceinline__ void sort_descending(uint32_t (&k)[N]) {
           }
 }
 
-// VPL experts per lane: VPL lane .. VPL lane + VPL - 1.  A warp takes every so many tokens; its next token's logits are on their way while it
-// chooses.  Instructions bound it: about 700 a token at 256 experts, 8 groups and a choice of 8.
+// VPL experts per lane: VPL lane .. VPL lane + VPL - 1.  A warp's next token's logits are on their way while it chooses.  Instructions
+// bound it: about 1000 a token at 256 experts, 8 groups and a choice of 8 (72 % of the issue slots), of which the nine rounds of the choice
+// are a quarter.
 constexpr int route_blocks(int vpl) { return vpl <= 4 ? 5 : vpl <= 8 ? 4 : vpl <= 16 ? 2 : 1; }   // per SM
 
 template <int DT, int VPL>
@@ -208,7 +213,7 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32, route_blocks(VPL)) route_ker
   const bool by_logit = p.bias == nullptr;   // sigmoid and softmax are increasing
   const bool by_sum = p.groups > 1 && p.top2;
   const bool by_score = !by_logit || by_sum;
-  const float tolerance = !p.sigmoid ? 2e-5f : VPL <= 8 ? 4e-6f : 1e-5f;
+  const Margin of_values = {p.sigmoid ? 1e-6f : 7e-6f, 1.4e-7f + 1.3e-7f * VPL}, of_sums = {p.sigmoid ? 2e-6f : 1.4e-5f, 3e-7f};
   // a block's tokens go to whichever of its warps is free: one that is in doubt about a token takes several times as long
   const int64_t begin = p.T / gridDim.x * blockIdx.x + min((int64_t)blockIdx.x, p.T % gridDim.x);
   const int64_t end = begin + p.T / gridDim.x + (blockIdx.x < p.T % gridDim.x);
@@ -319,7 +324,7 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32, route_blocks(VPL)) route_ker
         const float least = from_ordered(__reduce_min_sync(0xffffffffu, stays ? ordered(mine) : 0xffffffffu));
         const float most = from_ordered(__reduce_max_sync(0xffffffffu, real && !stays ? ordered(mine) : ordered(-CUDART_INF_F)));
         const float size = real && mine > -CUDART_INF_F ? fabsf(a) + (b > -CUDART_INF_F ? fabsf(b) : 0.0f) : 0.0f;
-        near = most > -CUDART_INF_F && too_near(least, most, tolerance, __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(size))));
+        near = most > -CUDART_INF_F && !of_sums.certain(least, most, __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(size))));
       }
     }
     // Keys: the number, its lowest bits replaced by which of the lane's experts it is, the first one highest.  Sorted, so that a lane offers its
@@ -372,7 +377,7 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32, route_blocks(VPL)) route_ker
     auto apart = [&](uint32_t ka, uint32_t kb) {     // whether ka is larger for sure
       if (by_logit) return ka != kb;
       const float a = from_ordered(ka), b = from_ordered(kb);
-      return !too_near(a, b, tolerance, fmaxf(fabsf(a), fabsf(b)));
+      return of_values.certain(a, b, fmaxf(fabsf(a), fabsf(b)));
     };
 #pragma unroll 4
     for (int r = 0; r < p.k + (exact ? 0 : 1); ++r) take(r);
@@ -455,7 +460,7 @@ int launch_route(const void* logits, RouteParams p, cudaStream_t st) {
   do {                                                                                                                    \
     const int lanes = p.group_size / VPL;                                                                                 \
     p.lanes_per_group = p.group_size % VPL == 0 && (lanes & (lanes - 1)) == 0 && lanes * p.groups <= 32 ? lanes : 0;      \
-    if (smem > 48 * 1024) MQ_CUDA(cudaFuncSetAttribute(route_kernel<DT, VPL>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)); \
+    if (smem > SMEM_AS_IS) MQ_CUDA(cudaFuncSetAttribute(route_kernel<DT, VPL>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)); \
     const int64_t blocks = ceil_div(p.T, ROUTE_WARPS), most = 148 * route_blocks(VPL);                                    \
     MQ_CUDA(launch_chained(true, route_kernel<DT, VPL>, dim3((unsigned)(blocks < most ? blocks : most)), dim3(ROUTE_WARPS * 32), smem, st, logits, p)); \
   } while (0)
@@ -474,7 +479,7 @@ int launch_route(const void* logits, RouteParams p, cudaStream_t st) {
 // A stable counting sort of the pairs by expert.  Every block takes a run of pairs; the first kernel counts them by expert, the
 // second adds up the blocks in front and ranks its own.  Within a block each warp takes a run of its own, 32 pairs at a
 // time; equal experts among the 32 are ranked by a match.
-constexpr int PLAN_THREADS = 512, PLAN_WARPS = PLAN_THREADS / 32, PLAN_KEEP = 8, PLAN_BLOCKS = 148;
+constexpr int PLAN_THREADS = 1024, PLAN_WARPS = PLAN_THREADS / 32, PLAN_KEEP = 4, PLAN_FETCH = 20, PLAN_BLOCKS = 148;
 
 struct PlanParams {
   const int32_t* ids;
@@ -525,27 +530,28 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_place_kernel(const PlanPara
   chain_wait();
   chain_release();
   if (p.counts) {
-    // all blocks' counts: every warp a share of the blocks, its loads independent of one another (one thread per expert that walks
-    // through the blocks waits for each in turn: 18 us for 524288 pairs)
-    for (int e0 = 0; e0 < p.E; e0 += 32) {
-      const int e = e0 + lane;
+    // All blocks' counts: a warp takes 32 experts and a share of the blocks, PLAN_FETCH loads at a time that do not wait for one another.  (One thread per
+    // expert that walks through the blocks, or 32 experts after the other with all blocks' counts shared out, cost 18 and 6 us of latency
+    // for 524288 pairs.)
+    const int slices = (p.E + 31) / 32, shares = slices < PLAN_WARPS ? PLAN_WARPS / slices : 1;
+    const int per_share = ((int)gridDim.x + shares - 1) / shares;
+    for (int slice = warp % (slices < PLAN_WARPS ? slices : PLAN_WARPS); slice < slices; slice += PLAN_WARPS) {
+      const int share = slices < PLAN_WARPS ? warp / slices : 0, e = slice * 32 + lane;
+      if (share >= shares || e >= p.E) continue;
+      const int first = share * per_share, last = min(first + per_share, (int)gridDim.x);
       int total = 0, before = 0;
-      if (e < p.E) {
-        constexpr int SHARE = (PLAN_BLOCKS + PLAN_WARPS - 1) / PLAN_WARPS;
-        int c[SHARE];
+      for (int b0 = first; b0 < last; b0 += PLAN_FETCH) {
+        int c[PLAN_FETCH];
 #pragma unroll
-        for (int i = 0; i < SHARE; ++i) {
-          const int b = warp + i * PLAN_WARPS;
-          c[i] = b < (int)gridDim.x ? __ldcg(p.counts + (int64_t)b * p.E + e) : 0;
-        }
+        for (int i = 0; i < PLAN_FETCH; ++i) c[i] = b0 + i < last ? __ldcg(p.counts + (int64_t)(b0 + i) * p.E + e) : 0;
 #pragma unroll
-        for (int i = 0; i < SHARE; ++i) {
+        for (int i = 0; i < PLAN_FETCH; ++i) {
           total += c[i];
-          before += warp + i * PLAN_WARPS < (int)blockIdx.x ? c[i] : 0;
+          before += b0 + i < (int)blockIdx.x ? c[i] : 0;
         }
-        atomicAdd(&totals[e], total);
-        atomicAdd(&befores[e], before);
       }
+      atomicAdd(&totals[e], total);
+      atomicAdd(&befores[e], before);
     }
   }
   // the experts of the warp's pairs, PLAN_KEEP at a time in registers; a run that is no longer stays there
@@ -674,7 +680,7 @@ int expert_plan(const int32_t* ids, int64_t pairs, int E, int first, int32_t* of
     MQ_LAUNCH_CHECK();
   }
   const size_t smem = (size_t)E * (PLAN_WARPS + 2) * 4;
-  if (smem > 48 * 1024) MQ_CUDA(cudaFuncSetAttribute(plan_place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  if (smem > SMEM_AS_IS) MQ_CUDA(cudaFuncSetAttribute(plan_place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   MQ_CUDA(launch_chained(true, plan_place_kernel, dim3(blocks), dim3(PLAN_THREADS), smem, st, p));
   MQ_LAUNCH_CHECK();
   return MQ_OK;

@@ -75,6 +75,22 @@ def test_route(cuda, c, dtype):
     _route_both(logits, 0.1 * torch.randn(c["E"], generator=g) if c.get("bias") else None, c, cuda)
 
 
+@pytest.mark.parametrize("E", [32, 255, 256, 257, 500, 504, 508, 510, 511, 512, 1023])
+def test_route_and_plan_of_every_size_of_scratch(cuda, E):
+    """Numbers of experts around the borders of what a kernel may take of shared memory without asking, and of its variants."""
+    g = _gen(E)
+    ids, _ = _route_both(torch.randn(9, E, generator=g), 0.1 * torch.randn(E, generator=g), dict(k=4, score="sigmoid"), cuda)
+    offsets, order, place = R.plan(ids, E)
+    got = ops.expert_plan(ids, E)
+    assert torch.equal(got.offsets.cpu().long(), torch.from_numpy(offsets)) and torch.equal(got.place.cpu().long(), torch.from_numpy(place))
+
+
+@pytest.mark.parametrize("E", range(340, 372))
+def test_plan_around_the_border_of_free_shared_memory(cuda, E):
+    ids = torch.randint(0, E, (50, 2), dtype=torch.int32, generator=_gen(E))
+    assert torch.equal(ops.expert_plan(ids.to(cuda), E).order.cpu().long(), torch.from_numpy(R.plan(ids, E)[1]))
+
+
 @pytest.mark.parametrize("c", ROUTES, ids=lambda c: "-".join(str(v) for v in c.values()))
 def test_route_masks(cuda, c):
     """-inf and NaN logits, rows that hold nothing else, experts switched off by their bias, logits of +inf and of the
