@@ -478,14 +478,16 @@ int launch_route(const void* logits, RouteParams p, cudaStream_t st) {
 // ---------------------------------------------------------------- the plan
 // A stable counting sort of the pairs by expert.  Every block takes a run of pairs; the first kernel counts them by expert, the
 // second adds up the blocks in front and ranks its own.  Within a block each warp takes a run of its own, 32 pairs at a
-// time; equal experts among the 32 are ranked by a match.
-constexpr int PLAN_THREADS = 1024, PLAN_WARPS = PLAN_THREADS / 32, PLAN_KEEP = 4, PLAN_FETCH = 20, PLAN_BLOCKS = 148;
+// time; which of the 32 have the same expert comes from a vote per bit of its number (the match instruction takes some 100 cycles of the SM
+// where all 32 differ: 3000 cycles for the 32 warps of a block, 25 us for 16384 pairs).
+constexpr int PLAN_THREADS = 1024, PLAN_WARPS = PLAN_THREADS / 32, PLAN_KEEP = 8, PLAN_FETCH = 20, PLAN_BLOCKS = 148;
 
 struct PlanParams {
   const int32_t* ids;
   int64_t pairs;
   int E, first;
   int run;      // pairs per block, a multiple of 32 * PLAN_WARPS
+  int bits;     // 2^bits > E
   int32_t* counts;
   int32_t *offsets, *order, *place;
 };
@@ -614,7 +616,12 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_place_kernel(const PlanPara
       const int64_t i = i0 + b * 32 + lane;
       if (i - lane >= w_end) break;
       const int e = mine[b];
-      const unsigned same = __match_any_sync(0xffffffffu, e);
+      unsigned same = 0xffffffffu;      // lanes with the same expert; -1 has all bits set, as no expert's number has
+      for (int bit = 0; bit < p.bits; ++bit) {
+        const bool set = e >> bit & 1;
+        const unsigned with = __ballot_sync(0xffffffffu, set);
+        same &= set ? with : ~with;
+      }
       const int rank = __popc(same & ((1u << lane) - 1u));
       int at = -1;
       if (e >= 0) at = next[e] + rank;
@@ -633,9 +640,11 @@ __global__ void __launch_bounds__(PLAN_THREADS) plan_place_kernel(const PlanPara
 }
 
 int plan_blocks(int64_t pairs) {
-  const int64_t run = 32 * PLAN_WARPS;
-  const int64_t b = ceil_div(pairs, 4 * run);
-  return (int)(b < 1 ? 1 : b > PLAN_BLOCKS ? PLAN_BLOCKS : b);
+  // one block, and one launch, up to four pairs a thread (7.4 us for 4096 pairs, where two launches take 9); beyond, one a thread while there are
+  // SMs: the scattered stores of `order` are what a block spends its time on
+  if (pairs <= 4 * PLAN_THREADS) return 1;
+  const int64_t b = ceil_div(pairs, PLAN_THREADS);
+  return (int)(b > PLAN_BLOCKS ? PLAN_BLOCKS : b);
 }
 
 }  // namespace
@@ -673,7 +682,8 @@ int expert_plan(const int32_t* ids, int64_t pairs, int E, int first, int32_t* of
                 cudaStream_t st) {
   const int blocks = plan_blocks(pairs);
   const int64_t unit = 32 * PLAN_WARPS;
-  PlanParams p = {ids, pairs, E, first, (int)(ceil_div(ceil_div(pairs > 0 ? pairs : 1, blocks), unit) * unit), nullptr, offsets, order, place};
+  PlanParams p = {ids, pairs, E, first, (int)(ceil_div(ceil_div(pairs > 0 ? pairs : 1, blocks), unit) * unit), 0, nullptr, offsets, order, place};
+  while ((1 << p.bits) <= E) ++p.bits;
   if (blocks > 1) {
     p.counts = static_cast<int32_t*>(workspace);
     MQ_CUDA(launch_chained(true, plan_count_kernel, dim3(blocks), dim3(PLAN_THREADS), (size_t)E * 4, st, p));

@@ -406,7 +406,8 @@ def _rows(t: Tensor, what: str) -> Tensor:
 
 def _pitch(t: Tensor) -> int:
     # the stride of a single row says nothing
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
+    rows, cols = t.shape
+    return t.stride()[0] if rows > 1 else cols
 
 
 def _scratch(device: torch.device, nbytes: int) -> Optional[Tensor]:
@@ -437,11 +438,13 @@ def _int8_codes(t: Tensor, dims: int, what: str) -> Tensor:
 
 def _code_pitch(t: Tensor) -> int:
     """Bytes from one row of codes to the next; of a single row its padded length, which is never read."""
-    if t.shape[-2] > 1:
-        if t.stride(-2) < t.shape[-1]:
+    rows, cols = t.shape[-2:]
+    if rows > 1:
+        pitch = t.stride()[-2]
+        if pitch < cols:
             raise MoeQuantError("rows of 8-bit codes must not overlap")
-        return t.stride(-2)
-    return (t.shape[-1] + 15) // 16 * 16
+        return pitch
+    return (cols + 15) // 16 * 16
 
 
 def _scales(t: Tensor, shape: Tuple[int, ...], what: str) -> Tensor:
@@ -529,7 +532,7 @@ def quantize_tokens(x: Tensor) -> Tuple[Tensor, Tensor]:
     scale = torch.empty(lead, dtype=torch.float32, device=x.device)
     with _lib.on_device(x.device):
         check(lib().mq_quantize_tokens(ptr(rows), code, T, K, _pitch(rows), ptr(codes), pitch, ptr(scale), stream_ptr(x.device)))
-    return codes[..., :K], scale
+    return codes if K == pitch else codes[..., :K], scale
 
 
 def int8_matmul(x: Tensor, weight: Tensor, weight_scale: Tensor, bias: Optional[Tensor] = None, x_scale: Optional[Tensor] = None,
