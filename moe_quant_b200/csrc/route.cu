@@ -7,7 +7,7 @@
 //
 // One warp per token, a run of experts per lane.  Which experts come first is decided on fp32 scores wherever these lie further apart than
 // they can be off, and in 64 bits in the rows where some do not (without a bias the logits themselves order the experts: exactly).
-// 65536 tokens, 256 experts in 8 groups with a bias: 88 us (0.76 TB/s of logits), 192 with every row in 64 bits.
+// 65536 tokens, 256 experts in 8 groups with a bias: 80 us (0.84 TB/s of logits), 192 with every row in 64 bits.
 #include <math_constants.h>
 
 #include "common.cuh"
@@ -196,7 +196,7 @@ __device__ __forceinline__ void sort_descending(uint32_t (&k)[N]) {
 }
 
 // VPL experts per lane: VPL lane .. VPL lane + VPL - 1.  A warp's next token's logits are on their way while it chooses.  Instructions
-// bound it: about 1000 a token at 256 experts, 8 groups and a choice of 8 (72 % of the issue slots), of which the nine rounds of the choice
+// bound it: about 900 a token at 256 experts, 8 groups and a choice of 8 (72 % of the issue slots), of which the nine rounds of the choice
 // are a quarter.
 constexpr int route_blocks(int vpl) { return vpl <= 4 ? 5 : vpl <= 8 ? 4 : vpl <= 16 ? 2 : 1; }   // per SM
 
@@ -223,7 +223,9 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32, route_blocks(VPL)) route_ker
   chain_wait();
   chain_release();
 
-  Word raw[VPL / WORD];
+  Word raw[VPL / WORD];      // experts behind the last one keep -inf
+#pragma unroll
+  for (int j = 0; j < VPL; ++j) raw[j / WORD].v[j % WORD] = from_float<T>(-CUDART_INF_F);
   auto load = [&](int64_t t) {
     const T* src = static_cast<const T*>(logits) + t * p.ld + e0;
 #pragma unroll
@@ -249,7 +251,7 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32, route_blocks(VPL)) route_ker
     t_next = begin + __shfl_sync(0xffffffffu, number, 0);
     float l[VPL];
 #pragma unroll
-    for (int j = 0; j < VPL; ++j) l[j] = e0 + j < p.E ? finite_logit(to_float(raw[j / WORD].v[j % WORD])) : -CUDART_INF_F;
+    for (int j = 0; j < VPL; ++j) l[j] = finite_logit(to_float(raw[j / WORD].v[j % WORD]));
     if (t_next < end) load(t_next);
 
     // softmax: its largest logit and sum, where scores are needed
@@ -313,6 +315,7 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32, route_blocks(VPL)) route_ker
       }
       const float mine = by_sum && b > -CUDART_INF_F ? a + b : a;
       int better = 0;
+#pragma unroll 4
       for (int g = 0; g < p.groups; ++g) {
         const float u = __shfl_sync(0xffffffffu, mine, g * first_of);
         better += u > mine || (u == mine && g < group);
@@ -379,7 +382,7 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32, route_blocks(VPL)) route_ker
       const float a = from_ordered(ka), b = from_ordered(kb);
       return of_values.certain(a, b, fmaxf(fabsf(a), fabsf(b)));
     };
-#pragma unroll 4
+#pragma unroll 2
     for (int r = 0; r < p.k + (exact ? 0 : 1); ++r) take(r);
     if (!exact) {
       uint32_t next = __shfl_down_sync(0xffffffffu, my_key, 1);
@@ -433,10 +436,10 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32, route_blocks(VPL)) route_ker
     const float chosen = mine >= 0 ? finite_logit(to_float(static_cast<const T*>(logits)[t * p.ld + mine])) : -CUDART_INF_F;
     float w = 0.0f;
     if (p.sigmoid) {
-      const float m = p.renormalise ? fminf(0.0f, warp_max(chosen)) : 0.0f;
+      const float m = p.renormalise ? fminf(0.0f, from_ordered(__reduce_max_sync(0xffffffffu, ordered(chosen)))) : 0.0f;
       if (mine >= 0) w = 1.0f / (expf(m) + expf(m - chosen));
     } else {
-      if (p.renormalise) top = warp_max(chosen);
+      if (p.renormalise) top = from_ordered(__reduce_max_sync(0xffffffffu, ordered(chosen)));
       if (mine >= 0) w = expf(chosen - top);
       if (!p.renormalise && mine >= 0) w /= total;
     }
