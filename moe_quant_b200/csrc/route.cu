@@ -29,6 +29,7 @@ struct RouteParams {
   float* weights;
   bool vec;               // rows of logits can be read 16 bytes at a time
   int lanes_per_group;    // lanes that hold a group, 0 where lanes and groups do not match
+  int lanes_to_search;    // as many as there are to a group, a power of two of them
 };
 
 // NaN is -inf, +inf the largest number
@@ -85,9 +86,7 @@ __device__ __noinline__ int choose(const RouteParams& p, const float* row, doubl
     for (int j = 0; j < VPL; ++j)
       if (e0 + j < p.E) value[e0 + j] = v[j];
     __syncwarp();
-    // as many lanes as there are to a group, a power of two of them
-    int share = 1;
-    while (2 * share * p.groups <= 32) share *= 2;
+    const int share = p.lanes_to_search;
     const int group = lane / share;
     double a = -CUDART_INF, b = -CUDART_INF;
     if (group < p.groups)
@@ -169,39 +168,40 @@ __device__ __forceinline__ float quick_sigmoid(float l) {
 }
 
 // How far a value may be off.  quick_sigmoid by 4e-7 at most (the exponential by 2^-22 and by 9e-8 |l|, times s (1 - s); sum and reciprocal by
-// 2^-23 each), a softmax score by 3.2e-6 (its sum over up to 1024 experts, 32 in a lane and five levels of lanes, and the exponentials); the sum
-// with the bias adds 2^-24 |v|.  So of two values the larger is certain where they are apart by 8e-7 (6.4e-6) + 1.2e-7 |v|, and by
-// 2^-23 VPL |v| more where low bits have given way to an index; of two sums of two values by 1.6e-6 (1.3e-5) + 2.4e-7 of what was summed.
+// 2^-23 each), a softmax score by 3.3e-6 of 1 / total, which no score exceeds (its sum over up to 1024 experts, 32 in a lane and five levels of
+// lanes, and the exponentials; 3.3e-6 for all sizes of `total` left 27 us where 636 tokens of 260 experts with a bias take 14); the sum
+// with the bias adds 2^-24 |v|.  So of two values the larger is certain where they are apart by 8e-7 (6.6e-6 / total) + 1.2e-7 |v|, and by
+// 2^-23 VPL |v| more where low bits have given way to an index; of two sums of two values by 1.6e-6 (1.33e-5 / total) + 2.4e-7 of what was summed.
+// (`total` is 1 for sigmoid.)
 struct Margin {
   float fixed, per_size;
-  __device__ __forceinline__ bool certain(float a, float b, float size) const { return a - b > fixed + per_size * size; }   // no for NaN
+  __device__ __forceinline__ bool certain(float a, float b, float total, float size) const { return a - b > __fdividef(fixed, total) + per_size * size; }   // no for NaN
 };
 
-// Descending, by a network of compare-exchanges (odd-even merges).
-template <int N>
+// Descending, by a network of compare-exchanges (odd-even merges of runs of P).  Steps by recursion: as loops, those of 16 and more keys are not
+// unrolled as a whole, and keys that are indexed at run time live in memory (20000 tokens, 400 experts: 50 us instead of 37).
+template <int N, int P = 1, int Q = P>
 __device__ __forceinline__ void sort_descending(uint32_t (&k)[N]) {
+  if constexpr (P < N) {
 #pragma unroll
-  for (int p = 1; p < N; p <<= 1)
-#pragma unroll
-    for (int q = p; q >= 1; q >>= 1)
-#pragma unroll
-      for (int j = q % p; j + q < N; j += 2 * q)
-#pragma unroll
-        for (int i = 0; i < q; ++i)
-          if (j + i + q < N && (j + i) / (2 * p) == (j + i + q) / (2 * p)) {
-            const uint32_t a = k[j + i], b = k[j + i + q];
-            k[j + i] = max(a, b);
-            k[j + i + q] = min(a, b);
-          }
+    for (int j = Q % P; j + Q < N; ++j)
+      if ((j - Q % P) % (2 * Q) < Q && j / (2 * P) == (j + Q) / (2 * P)) {
+        const uint32_t a = k[j], b = k[j + Q];
+        k[j] = max(a, b);
+        k[j + Q] = min(a, b);
+      }
+    if constexpr (Q > 1) sort_descending<N, P, Q / 2>(k);
+    else sort_descending<N, 2 * P>(k);
+  }
 }
 
 // VPL experts per lane: VPL lane .. VPL lane + VPL - 1.  A warp's next token's logits are on their way while it chooses.  Instructions
 // bound it: about 900 a token at 256 experts, 8 groups and a choice of 8 (72 % of the issue slots), of which the nine rounds of the choice
 // are a quarter.
-constexpr int route_blocks(int vpl) { return vpl <= 4 ? 5 : vpl <= 8 ? 4 : vpl <= 16 ? 2 : 1; }   // per SM
+constexpr int route_blocks(int vpl) { return vpl <= 4 ? 5 : vpl <= 8 ? 4 : vpl <= 16 ? 3 : 2; }   // per SM
 
 template <int DT, int VPL>
-__global__ void __launch_bounds__(ROUTE_WARPS * 32, route_blocks(VPL)) route_kernel(const void* __restrict__ logits, const RouteParams p) {
+__global__ void __launch_bounds__(ROUTE_WARPS * 32, route_blocks(VPL)) route_kernel(const void* __restrict__ logits, const __grid_constant__ RouteParams p) {
   using T = typename StorageOf<DT>::type;
   constexpr int WORD = VPL * sizeof(T) >= 16 ? 16 / sizeof(T) : 1;     // values per load
   struct alignas(WORD * sizeof(T)) Word { T v[WORD]; };
@@ -293,25 +293,28 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32, route_blocks(VPL)) route_ker
           b = fmaxf(b, fminf(a, v[j]));
           a = fmaxf(a, v[j]);
         }
-        for (int o = 1; o < first_of; o <<= 1) {
-          const float a2 = __shfl_xor_sync(0xffffffffu, a, o), b2 = __shfl_xor_sync(0xffffffffu, b, o);
-          b = fmaxf(fminf(a, a2), fmaxf(b, b2));
-          a = fmaxf(a, a2);
-        }
       } else {
-        group = lane;
+        first_of = p.lanes_to_search;
+        group = lane / first_of;
 #pragma unroll
         for (int j = 0; j < VPL; ++j)
           if (e0 + j < p.E) row[e0 + j] = v[j];
         __syncwarp();
-        if (lane < p.groups) {
-          for (int i = 0; i < p.group_size; ++i) {
-            const float u = row[lane * p.group_size + i];
+        if (group < p.groups) {
+          const float* of_group = row + group * p.group_size;
+#pragma unroll 4
+          for (int i = lane % first_of; i < p.group_size; i += first_of) {
+            const float u = of_group[i];
             b = fmaxf(b, fminf(a, u));
             a = fmaxf(a, u);
           }
         }
         __syncwarp();
+      }
+      for (int o = 1; o < first_of; o <<= 1) {
+        const float a2 = __shfl_xor_sync(0xffffffffu, a, o), b2 = __shfl_xor_sync(0xffffffffu, b, o);
+        b = fmaxf(fminf(a, a2), fmaxf(b, b2));
+        a = fmaxf(a, a2);
       }
       const float mine = by_sum && b > -CUDART_INF_F ? a + b : a;
       int better = 0;
@@ -327,7 +330,7 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32, route_blocks(VPL)) route_ker
         const float least = from_ordered(__reduce_min_sync(0xffffffffu, stays ? ordered(mine) : 0xffffffffu));
         const float most = from_ordered(__reduce_max_sync(0xffffffffu, real && !stays ? ordered(mine) : ordered(-CUDART_INF_F)));
         const float size = real && mine > -CUDART_INF_F ? fabsf(a) + (b > -CUDART_INF_F ? fabsf(b) : 0.0f) : 0.0f;
-        near = most > -CUDART_INF_F && !of_sums.certain(least, most, __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(size))));
+        near = most > -CUDART_INF_F && !of_sums.certain(least, most, total, __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(size))));
       }
     }
     // Keys: the number, its lowest bits replaced by which of the lane's experts it is, the first one highest.  Sorted, so that a lane offers its
@@ -352,7 +355,7 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32, route_blocks(VPL)) route_ker
           left = p.group_size;
         }
         --left;
-        if (!(kept >> (group & 31) & 1u)) key[j] = 0;
+        if (!(kept >> (group * p.lanes_to_search & 31) & 1u)) key[j] = 0;
       }
     }
     sort_descending(key);
@@ -380,7 +383,7 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32, route_blocks(VPL)) route_ker
     auto apart = [&](uint32_t ka, uint32_t kb) {     // whether ka is larger for sure
       if (by_logit) return ka != kb;
       const float a = from_ordered(ka), b = from_ordered(kb);
-      return of_values.certain(a, b, fmaxf(fabsf(a), fabsf(b)));
+      return of_values.certain(a, b, total, fmaxf(fabsf(a), fabsf(b)));
     };
 #pragma unroll 2
     for (int r = 0; r < p.k + (exact ? 0 : 1); ++r) take(r);
@@ -458,6 +461,8 @@ template <int DT>
 int launch_route(const void* logits, RouteParams p, cudaStream_t st) {
   const size_t smem = (size_t)ROUTE_WARPS * p.E * 12;
   const int64_t word = 16 / (int64_t)dtype_size(DT);
+  p.lanes_to_search = 1;
+  while (2 * p.lanes_to_search * p.groups <= 32) p.lanes_to_search *= 2;
   p.vec = aligned(logits, 16) && p.E % word == 0 && (p.ld % word == 0 || p.T == 1);
 #define MQ_ROUTE(VPL)                                                                                                     \
   do {                                                                                                                    \
