@@ -154,6 +154,19 @@ __device__ __forceinline__ void store_rows(uint32_t tile, int lane, S* out, int6
   __syncwarp();
 }
 
+// The same, each lane its column.
+template <typename S, typename Of>
+__device__ __forceinline__ void store_columns(S* to, int64_t ld, int left, Of value) {
+  if (left >= 32) {
+#pragma unroll
+    for (int j = 0; j < 32; ++j, to += ld) *to = value(j);
+  } else {
+#pragma unroll
+    for (int j = 0; j < 32; ++j, to += ld)
+      if (j < left) *to = value(j);
+  }
+}
+
 // The tokens' rows in boxes of 32, 64 and 128. A box costs the TMA unit time beside its bytes: 16384 pairs, 32 experts, 7168 to 2048 and back,
 // gate and up 364 us against 386 with boxes of 32 rows and of 16 gate and up rows, down 209 against 217.
 struct TokenMaps {
@@ -350,10 +363,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
         tmem_ld32_int(t_lane + (uint32_t)(b * I8_MAX_WIDTH + c * 32), r);
         const int t = u.t0 + c * 32, left = u.t_end - t;     // tokens of this chunk that exist
         if constexpr (KIND == INT8_SUMS) {
-          int* out = a.sums + ((int64_t)u.share * p.T + t) * a.ld_sums + col;
-#pragma unroll
-          for (int j = 0; j < 32; ++j)
-            if (col_in && j < left) out[j * a.ld_sums] = r[j];
+          store_columns(a.sums + ((int64_t)u.share * p.T + t) * a.ld_sums + col, a.ld_sums, col_in ? left : 0, [&](int j) { return r[j]; });
           continue;
         }
         float v[32];
@@ -413,9 +423,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
             if constexpr (TOKENS < 32)
               store_rows<TOKENS>(tile, lane, out + (int64_t)TOKENS * a.o.ldy, a.o.ldy, left - TOKENS, p.rows - (col - lane), [&](int j) { return v[TOKENS + j]; });
           } else {
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-              if (col_in && j < left) out[(int64_t)j * a.o.ldy + lane] = from_float<S>(v[j]);
+            store_columns(out + lane, a.o.ldy, col_in ? left : 0, [&](int j) { return from_float<S>(v[j]); });
           }
         }
       }
