@@ -154,7 +154,8 @@ __device__ __forceinline__ void store_rows(uint32_t tile, int lane, S* out, int6
   __syncwarp();
 }
 
-// The same, each lane its column.
+// The same, each lane its column: rows that cannot be stored 16 bytes at a time.  (A comparison in front of every store costs more than the
+// stores: 2914 x 9508 x 120, bf16 results, 46 us instead of 25.5; in 16-byte pieces 2914 x 9504 x 120 takes 21.5.)
 template <typename S, typename Of>
 __device__ __forceinline__ void store_columns(S* to, int64_t ld, int left, Of value) {
   if (left >= 32) {
@@ -503,8 +504,8 @@ namespace {
 // How wide a tile of tokens is at most and how many pairs of CTAs share its k, from what a tile costs (us, measured over 2048 to 7168 rows of
 // 1024 to 16384): a slab of 128 of k 0.225 up to 64 columns and 0.20 + 0.00035 a column above, 4.9 + 0.008 a column beside the slabs; where k
 // is shared, 3.3 for the second kernel and 10 MB/us for the sums' way through the L2.  Picked / best of all shapes tried: 16 tokens
-// through 2048 x 7168 9.9 / 9.9 (not shared 17.1), 512 tokens 18.1 / 17.4, 2048 tokens 23.5 / 23.5 (128 wide 34.0), 1011 x 1008 x 1072 7.2 / 7.2 (256
-// wide 9.5).
+// through 2048 x 7168 9.7 / 9.6 (not shared 16.3), 512 tokens 16.1 / 15.5, 2048 tokens 23.9 / 23.8 (128 wide 31.0), 1011 x 1008 x 1072 7.1 / 7.1 (256
+// wide 9.6).
 struct Shape {
   int width, splits;
 };
