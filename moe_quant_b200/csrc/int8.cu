@@ -207,7 +207,7 @@ int quantize_rows(int dtype, RowsParams p, cudaStream_t st) {
 // ---------------------------------------------------------------- products
 // y[t] = sum over the token's pairs, in the order of its slots, of weight * (the pair's down product).  The products are short of the
 // factor h_scale[pair] (fp32), or h_scale[pair] * power[expert, column / 32] (fp16; see INT8_PAIRS).  One block per token, eight columns a
-// thread.
+// thread; smaller blocks for short rows (20000 tokens of 512, 2 of 8 experts: 92 us the whole call instead of 102 with 256 threads).
 struct CombineParams {
   const void* pairs;
   int64_t ldp;
@@ -245,7 +245,7 @@ __global__ void __launch_bounds__(256) combine_kernel(const CombineParams p) {
     }
     __syncthreads();
     const int n_pairs = found[turn];
-    for (int n = threadIdx.x * 8; n < p.N; n += 256 * 8) {
+    for (int n = threadIdx.x * 8; n < p.N; n += blockDim.x * 8) {
       float sum[8] = {};
 #pragma unroll 2
       for (int i = 0; i < n_pairs; ++i) {
@@ -390,8 +390,9 @@ size_t experts_buffers(int dtype, int64_t T, int k, int E, int64_t K, int64_t I,
 template <int DT>
 int launch_combine(const CombineParams& p, cudaStream_t st) {
   const bool vec = p.N % 8 == 0 && p.ldy % 8 == 0 && aligned(p.y, 16);
-  const unsigned grid = (unsigned)(p.T < 148 * 16 ? p.T : 148 * 16);
-  MQ_CUDA(launch_chained(true, vec ? combine_kernel<DT, true> : combine_kernel<DT, false>, dim3(grid), dim3(256), 0, st, p));
+  const int threads = p.N <= 512 ? 64 : p.N <= 1024 ? 128 : 256;
+  const int64_t most = 148 * 4096 / threads;
+  MQ_CUDA(launch_chained(true, vec ? combine_kernel<DT, true> : combine_kernel<DT, false>, dim3((unsigned)(p.T < most ? p.T : most)), dim3(threads), 0, st, p));
   MQ_LAUNCH_CHECK();
   return MQ_OK;
 }
