@@ -387,50 +387,51 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32, route_blocks(VPL)) route_ker
     };
 #pragma unroll 2
     for (int r = 0; r < p.k + (exact ? 0 : 1); ++r) take(r);
+    bool in_doubt = near;
     if (!exact) {
       uint32_t next = __shfl_down_sync(0xffffffffu, my_key, 1);
       if (lane == p.k - 1) next = last;     // (lane 32 of k = 32)
-      const bool in_doubt = __any_sync(0xffffffffu, lane < p.k && next != 0 && !apart(my_key, next));
-      if (near || in_doubt) {
-        // A few more, as far as these have surely left the k-th behind: then the choice is among them, and a lane each finds their values in
-        // 64 bits.  Otherwise (or where a group or a softmax's sum is in doubt) all of the token's values are formed anew.
-        const int n = p.k + EXTRA;
-        bool among = !near && (by_logit || p.sigmoid) && n <= 32;
-        if (among) {
+      in_doubt |= __any_sync(0xffffffffu, lane < p.k && next != 0 && !apart(my_key, next)) != 0;
+    }
+    if (in_doubt) {
+      // A few more, as far as these have surely left the k-th behind: then the choice is among them, and a lane each finds their values in
+      // 64 bits.  Otherwise (or where a group or a softmax's sum is in doubt) all of the token's values are formed anew.
+      const int n = p.k + EXTRA;
+      bool among = !near && (by_logit || p.sigmoid) && n <= 32;
+      if (among) {
 #pragma unroll 1
-          for (int r = p.k + 1; r < n; ++r) take(r);
-          among = last == 0 || apart(__shfl_sync(0xffffffffu, my_key, p.k - 1), last);
+        for (int r = p.k + 1; r < n; ++r) take(r);
+        among = last == 0 || apart(__shfl_sync(0xffffffffu, my_key, p.k - 1), last);
+      }
+      if (among) {
+        double d = -CUDART_INF;
+        if (mine >= 0) {
+          d = finite_logit(to_float(static_cast<const T*>(logits)[t * p.ld + mine]));
+          if (!by_logit) d = 1.0 / (1.0 + exp(-d)) + (double)p.bias[mine];
         }
-        if (among) {
-          double d = -CUDART_INF;
-          if (mine >= 0) {
-            d = finite_logit(to_float(static_cast<const T*>(logits)[t * p.ld + mine]));
-            if (!by_logit) d = 1.0 / (1.0 + exp(-d)) + (double)p.bias[mine];
-          }
-          int rank = 0;
+        int rank = 0;
 #pragma unroll 1
-          for (int c = 0; c < n; ++c) {
-            const double u = __shfl_sync(0xffffffffu, d, c);
-            const int i = __shfl_sync(0xffffffffu, mine, c);
-            rank += u > d || (u == d && i < mine);
-          }
-          if (mine < 0) rank = 32;
-          const int found = mine;
-          mine = -1;
+        for (int c = 0; c < n; ++c) {
+          const double u = __shfl_sync(0xffffffffu, d, c);
+          const int i = __shfl_sync(0xffffffffu, mine, c);
+          rank += u > d || (u == d && i < mine);
+        }
+        if (mine < 0) rank = 32;
+        const int found = mine;
+        mine = -1;
 #pragma unroll 1
-          for (int c = 0; c < p.k; ++c) {
-            const unsigned who = __ballot_sync(0xffffffffu, rank == c);
-            const int i = __shfl_sync(0xffffffffu, found, who ? __ffs(who) - 1 : 0);
-            if (lane == c && who) mine = i;
-          }
-        } else {
+        for (int c = 0; c < p.k; ++c) {
+          const unsigned who = __ballot_sync(0xffffffffu, rank == c);
+          const int i = __shfl_sync(0xffffffffu, found, who ? __ffs(who) - 1 : 0);
+          if (lane == c && who) mine = i;
+        }
+      } else {
 #pragma unroll
-          for (int j = 0; j < VPL; ++j)
-            if (e0 + j < p.E) row[e0 + j] = l[j];
-          __syncwarp();
-          mine = choose<VPL>(p, row, value, lane);
-          __syncwarp();
-        }
+        for (int j = 0; j < VPL; ++j)
+          if (e0 + j < p.E) row[e0 + j] = l[j];
+        __syncwarp();
+        mine = choose<VPL>(p, row, value, lane);
+        __syncwarp();
       }
     }
     if (lane >= p.k) mine = -1;

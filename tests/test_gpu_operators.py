@@ -144,6 +144,25 @@ def test_route_values_next_to_one_another(cuda):
     _route_both(torch.randn(40, E, generator=g), torch.full((E,), 1000.0), c, cuda)
 
 
+@pytest.mark.parametrize("dtype", [FP32, BF16, FP16])
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+def test_route_groups_whose_sums_lie_next_to_one_another(cuda, score, dtype):
+    """Sums of two scores that differ by less than fp32 can tell: the group is the one of 64-bit sums, for logits of every type."""
+    v = torch.arange(1.0, 4.0, 2.0 ** -6).to(dtype)
+    i, j = torch.triu_indices(len(v), len(v), 1)
+    s = torch.sigmoid(v.double()) if score == "sigmoid" else torch.exp(v.double() - 4)
+    order = torch.argsort(s[i] + s[j])
+    i, j, sums = i[order], j[order], (s[i] + s[j])[order]
+    gap = (sums[1:] - sums[:-1]).where(sums[1:] - sums[:-1] > 1e-12, torch.tensor(1.0, dtype=torch.float64))     # (64 bits tell these apart)
+    at = torch.argsort(gap)[:300]
+    rows = torch.full((2, 300, 2, 4), -4.0, dtype=dtype)
+    for n, (low, high) in enumerate([(at, at + 1), (at + 1, at)]):
+        rows[n, :, 0, 1], rows[n, :, 0, 2] = v[i[low]], v[j[low]]
+        rows[n, :, 1, 0], rows[n, :, 1, 3] = v[i[high]], v[j[high]]
+    c = dict(T=600, E=8, k=2, score=score, groups=2, keep=1, group_score="top2")
+    _route_both(rows.reshape(600, 8), None, c, cuda)
+
+
 def test_route_sigmoid_weights_of_very_negative_logits(cuda):
     """Every score underflows, their ratios do not."""
     logits = -200 - 3 * torch.rand(6, 32, generator=_gen(2))
