@@ -148,6 +148,23 @@ __device__ __noinline__ int choose(const RouteParams& p, const float* row, doubl
   return mine;
 }
 
+// Without a bias: whether a group whose two largest logits are a and b stays, by 64-bit sums of their scores (softmax without its common
+// factor).  Groups are first_of lanes each.  16-bit logits come here often, since different groups have the same two: 28375 tokens of 332
+// experts in 4 groups 93 us with all of the token's values formed anew.
+__device__ __noinline__ bool stays_by_logits(const RouteParams& p, float a, float b, float top, int group, int first_of) {
+  double sum = -CUDART_INF;
+  if (a > -CUDART_INF_F) {
+    sum = p.sigmoid ? 1.0 / (1.0 + exp(-(double)a)) : exp((double)a - top);
+    if (b > -CUDART_INF_F) sum += p.sigmoid ? 1.0 / (1.0 + exp(-(double)b)) : exp((double)b - top);
+  }
+  int better = 0;
+  for (int g = 0; g < p.groups; ++g) {
+    const double u = __shfl_sync(0xffffffffu, sum, g * first_of);
+    better += u > sum || (u == sum && g < group);
+  }
+  return better < p.keep;
+}
+
 // fp32 numbers as unsigned integers of the same order; 0 stands for an expert that cannot be chosen
 __device__ __forceinline__ uint32_t ordered(float v) {
   const int b = __float_as_int(v);
@@ -266,18 +283,16 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32, route_blocks(VPL)) route_ker
       for (int j = 0; j < VPL; ++j) total += l[j] > -CUDART_INF_F ? expf(l[j] - top) : 0.0f;
       total = warp_sum(total);
     }
-    // v: what groups and, with a bias, experts are compared by
+    // v: what experts are compared by, the score with its bias or the logit
     float v[VPL];
-    if (!by_score) {
+    auto score = [&](float logit, float inv) { return p.sigmoid ? quick_sigmoid(logit) : quick_exp(logit - top) * inv; };
+    if (by_logit) {
 #pragma unroll
       for (int j = 0; j < VPL; ++j) v[j] = l[j];
     } else {
       const float inv = __fdividef(1.0f, total);
 #pragma unroll
-      for (int j = 0; j < VPL; ++j) {
-        const float s = p.sigmoid ? quick_sigmoid(l[j]) : quick_exp(l[j] - top) * inv;
-        v[j] = l[j] > -CUDART_INF_F ? s + bias[j] : -CUDART_INF_F;
-      }
+      for (int j = 0; j < VPL; ++j) v[j] = l[j] > -CUDART_INF_F ? score(l[j], inv) + bias[j] : -CUDART_INF_F;
     }
     bool near = false;
     bool whole_lane = true;           // groups keep or drop all of a lane's experts
@@ -316,7 +331,13 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32, route_blocks(VPL)) route_ker
         b = fmaxf(fminf(a, a2), fmaxf(b, b2));
         a = fmaxf(a, a2);
       }
-      const float mine = by_sum && b > -CUDART_INF_F ? a + b : a;
+      float va = a, vb = b;
+      if (by_logit && by_sum) {      // the largest logits have the largest scores
+        const float inv = __fdividef(1.0f, total);
+        if (a > -CUDART_INF_F) va = score(a, inv);
+        if (b > -CUDART_INF_F) vb = score(b, inv);
+      }
+      const float mine = by_sum && vb > -CUDART_INF_F ? va + vb : va;
       int better = 0;
 #pragma unroll 4
       for (int g = 0; g < p.groups; ++g) {
@@ -329,8 +350,13 @@ __global__ void __launch_bounds__(ROUTE_WARPS * 32, route_blocks(VPL)) route_ker
       if (by_score) {
         const float least = from_ordered(__reduce_min_sync(0xffffffffu, stays ? ordered(mine) : 0xffffffffu));
         const float most = from_ordered(__reduce_max_sync(0xffffffffu, real && !stays ? ordered(mine) : ordered(-CUDART_INF_F)));
-        const float size = real && mine > -CUDART_INF_F ? fabsf(a) + (b > -CUDART_INF_F ? fabsf(b) : 0.0f) : 0.0f;
+        const float size = real && mine > -CUDART_INF_F ? fabsf(va) + (vb > -CUDART_INF_F ? fabsf(vb) : 0.0f) : 0.0f;
         near = most > -CUDART_INF_F && !of_sums.certain(least, most, total, __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(size))));
+        if (near && by_logit) {
+          const bool stays64 = stays_by_logits(p, a, b, top, group, first_of);     // (all lanes: it shuffles)
+          kept = __ballot_sync(0xffffffffu, real && stays64);
+          near = false;
+        }
       }
     }
     // Keys: the number, its lowest bits replaced by which of the lane's experts it is, the first one highest.  Sorted, so that a lane offers its
