@@ -205,15 +205,15 @@ int quantize_rows(int dtype, RowsParams p, cudaStream_t st) {
 }
 
 // ---------------------------------------------------------------- products
-// y[t] = sum over the token's pairs, in the order of its slots, of weight * (the pair's down product).  The products are short of the
-// factor h_scale[pair] (fp32), or h_scale[pair] * power[expert, column / 32] (fp16; see INT8_PAIRS).  One block per token, eight columns a
+// y[t] = sum over the token's pairs, in the order of its slots, of weight * (the pair's down product).  The products are fp32 and short of the
+// factor h_scale[pair] (INT8_PAIRS).  One block per token, eight columns a
 // thread; smaller blocks for short rows (20000 tokens of 512, 2 of 8 experts: 92 us the whole call instead of 102 with 256 threads).
 struct CombineParams {
-  const void* pairs;
+  const float* pairs;
   int64_t ldp;
-  const float *power, *h_scale, *weights;
-  const int32_t *place, *ids;
-  int first, top_k, N, powers;   // powers per expert
+  const float *h_scale, *weights;
+  const int32_t* place;
+  int top_k, N;
   int64_t T;
   void* y;
   int64_t ldy;
@@ -222,9 +222,7 @@ struct CombineParams {
 template <int DT, bool VEC>
 __global__ void __launch_bounds__(256) combine_kernel(const CombineParams p) {
   using S = typename StorageOf<DT>::type;
-  constexpr bool SCALED = DT == MQ_BF16;     // products in fp16
-  using P = typename StorageOf<SCALED ? MQ_F16 : MQ_F32>::type;
-  __shared__ int row_of[2][32], power_of[2][32];
+  __shared__ int row_of[2][32];
   __shared__ float factor_of[2][32];
   __shared__ int found[2];
   chain_wait();
@@ -238,7 +236,6 @@ __global__ void __launch_bounds__(256) combine_kernel(const CombineParams p) {
       if (at >= 0) {
         const int i = __popc(have & ((1u << s) - 1u));
         row_of[turn][i] = at;
-        if (SCALED) power_of[turn][i] = (p.ids[t * p.top_k + s] - p.first) * p.powers;
         factor_of[turn][i] = p.weights[t * p.top_k + s] * __ldcg(p.h_scale + at);
       }
       if (s == 0) found[turn] = __popc(have);
@@ -249,12 +246,11 @@ __global__ void __launch_bounds__(256) combine_kernel(const CombineParams p) {
       float sum[8] = {};
 #pragma unroll 2
       for (int i = 0; i < n_pairs; ++i) {
-        const P* src = static_cast<const P*>(p.pairs) + (int64_t)row_of[turn][i] * p.ldp + n;
-        const float f = factor_of[turn][i] * (SCALED ? __ldcg(p.power + power_of[turn][i] + (n >> 5)) : 1.0f);
+        const float f = factor_of[turn][i];
         // (rows of products have room for a multiple of sixteen)
-        const Eight<P> a = *reinterpret_cast<const Eight<P>*>(src);
+        const Eight<float> a = *reinterpret_cast<const Eight<float>*>(p.pairs + (int64_t)row_of[turn][i] * p.ldp + n);
 #pragma unroll
-        for (int j = 0; j < 8; ++j) sum[j] = fmaf(f, to_float(a.v[j]), sum[j]);
+        for (int j = 0; j < 8; ++j) sum[j] = fmaf(f, a.v[j], sum[j]);
       }
       S* out = static_cast<S*>(p.y) + t * p.ldy + n;
       if (VEC) {
@@ -331,7 +327,7 @@ extern "C" int mq_int8_matmul(const void* x, int x_dtype, const float* x_scale, 
   Int8Product p = dense_product(T, N, K);
   p.x_scale = x_scale;
   p.w = w; p.ldw = ldw; p.w_scale = w_scale;
-  const Int8Out o = {INT8_Y, out_dtype, y, ldy, bias, nullptr};
+  const Int8Out o = {INT8_Y, out_dtype, y, ldy, bias};
   if (int8_few_fits(T, K)) return int8_few(x, x_dtype, ldx, p, o, st);
   Workspace ws(workspace, workspace_bytes);
   const size_t n_sums = int8_umma_scratch_bytes(p, INT8_Y);
@@ -356,12 +352,11 @@ struct ExpertsBuffers {
   int32_t *offsets, *order, *place;
   void* plan;
   int8_t *x_codes, *h_codes;
-  float *x_scale, *h_scale, *h, *power;
-  void* pairs;
+  float *x_scale, *h_scale, *h, *pairs;
 };
 // Carves the buffers out of ws, or adds up their bytes where there is none.  The products of the pairs take the place of the tokens'
 // codes and of the gated values, which have been read by then.
-size_t experts_buffers(int dtype, int64_t T, int k, int E, int64_t K, int64_t I, Workspace* ws, ExpertsBuffers* b) {
+size_t experts_buffers(int64_t T, int k, int E, int64_t K, int64_t I, Workspace* ws, ExpertsBuffers* b) {
   const size_t P = (size_t)T * k;
   size_t total = 0;
   auto take = [&](size_t bytes) -> char* {
@@ -376,13 +371,12 @@ size_t experts_buffers(int dtype, int64_t T, int k, int E, int64_t K, int64_t I,
   x.plan = take(mq_expert_plan_workspace_bytes((int64_t)P, E));
   x.x_scale = reinterpret_cast<float*>(take(P * 4));
   x.h_scale = reinterpret_cast<float*>(take(P * 4));
-  x.power = reinterpret_cast<float*>(take((size_t)E * ceil_div(K, 32) * 4));
   x.h_codes = reinterpret_cast<int8_t*>(take(P * (size_t)pitch_of(I)));
-  const size_t codes = align_up(P * (size_t)pitch_of(K), 256), h = align_up(P * (size_t)pitch_of(I) * 4, 256), pairs = align_up(P * (size_t)pitch_of(K) * (dtype == MQ_BF16 ? 2 : 4), 256);
+  const size_t codes = align_up(P * (size_t)pitch_of(K), 256), h = align_up(P * (size_t)pitch_of(I) * 4, 256), pairs = align_up(P * (size_t)pitch_of(K) * 4, 256);
   char* shared = take(codes + h > pairs ? codes + h : pairs);
   x.x_codes = reinterpret_cast<int8_t*>(shared);
   x.h = reinterpret_cast<float*>(shared + codes);
-  x.pairs = shared;
+  x.pairs = reinterpret_cast<float*>(shared);
   if (b) *b = x;
   return total;
 }
@@ -399,8 +393,8 @@ int launch_combine(const CombineParams& p, cudaStream_t st) {
 }  // namespace
 }  // namespace mq
 
-extern "C" size_t mq_int8_experts_workspace_bytes(int dtype, int64_t T, int top_k, int64_t E, int64_t K, int64_t I) {
-  return experts_buffers(dtype, T, top_k, (int)E, K, I, nullptr, nullptr);
+extern "C" size_t mq_int8_experts_workspace_bytes(int /*dtype*/, int64_t T, int top_k, int64_t E, int64_t K, int64_t I) {
+  return experts_buffers(T, top_k, (int)E, K, I, nullptr, nullptr);
 }
 
 extern "C" int mq_int8_experts(const void* x, int dtype, int64_t T, int64_t K, int64_t ldx, const int32_t* ids, const float* weights, int top_k,
@@ -425,7 +419,7 @@ extern "C" int mq_int8_experts(const void* x, int dtype, int64_t T, int64_t K, i
              workspace_bytes, need);
   Workspace ws(workspace, workspace_bytes);
   ExpertsBuffers b;
-  experts_buffers(dtype, T, top_k, (int)E, K, I, &ws, &b);
+  experts_buffers(T, top_k, (int)E, K, I, &ws, &b);
   const int64_t P = T * top_k;
   Int8Product up = {}, dn = {};
   up.w = gate_up; up.ldw = ld_gate_up; up.w_expert = gate_up_expert; up.w_scale = gate_up_scale;
@@ -447,10 +441,10 @@ extern "C" int mq_int8_experts(const void* x, int dtype, int64_t T, int64_t K, i
   }
   MQ_TRY(quantize_rows(dtype, rows, st));
   up.x = b.x_codes; up.ldx = pitch_of(K); up.x_rows = P; up.x_scale = b.x_scale; up.offsets = b.offsets;
-  MQ_TRY(int8_product_umma(up, Int8Out{INT8_GATED, MQ_F32, b.h, pitch_of(I), nullptr, nullptr}, nullptr, st));
+  MQ_TRY(int8_product_umma(up, Int8Out{INT8_GATED, MQ_F32, b.h, pitch_of(I), nullptr}, nullptr, st));
   MQ_TRY(quantize_rows(MQ_F32, RowsParams{b.h, pitch_of(I), P, b.offsets + E, nullptr, 0, (int)I, b.h_codes, pitch_of(I), b.h_scale}, st));
   dn.x = b.h_codes; dn.ldx = pitch_of(I); dn.x_rows = P; dn.x_scale = b.h_scale; dn.offsets = b.offsets;
-  MQ_TRY(int8_product_umma(dn, Int8Out{INT8_PAIRS, dtype == MQ_BF16 ? MQ_F16 : MQ_F32, b.pairs, pitch_of(K), nullptr, b.power}, nullptr, st));
-  const CombineParams c = {b.pairs, pitch_of(K), b.power, b.h_scale, weights, b.place, ids, (int)first, top_k, (int)K, (int)ceil_div(K, 32), T, y, ldy};
+  MQ_TRY(int8_product_umma(dn, Int8Out{INT8_PAIRS, MQ_F32, b.pairs, pitch_of(K), nullptr}, nullptr, st));
+  const CombineParams c = {b.pairs, pitch_of(K), b.h_scale, weights, b.place, top_k, (int)K, T, y, ldy};
   return dtype == MQ_BF16 ? launch_combine<MQ_BF16>(c, st) : launch_combine<MQ_F16>(c, st);
 }

@@ -27,11 +27,8 @@ struct Int8Product {
 enum Int8Result {
   INT8_Y = 0,      // y = sum * x_scale * w_scale + bias, in the result's type
   INT8_GATED = 1,  // weights are gate rows and up rows, `rows` of either: h = silu(gate) * up, fp32
-  // The products of the pairs, short of x_scale: sum * w_scale in fp32, or (for results of 8 significant bits) short of a power of two per
-  // 32 columns in fp16: sum * w_scale / power[e, n / 32] with power = 2^k p, p the power of two above the 32 scales and 2^k the one
-  // that brings any sum (at most 127 * 128 * K) to 2^15.  It cannot overflow, and keeps 11 bits down to a sum of 1 (for K up to 32768)
-  // times a scale of the column's neighbours; what is smaller is off by 2^-25 of the power.  Half the bytes, and against the 2^-8 of the
-  // results' own rounding nothing; for fp16 results it would raise the error by 1.4.
+  // The products of the pairs, short of x_scale: sum * w_scale in fp32.  (In fp16 they would be half the bytes, but 11 bits of each product
+  // show in the results: 1e-3 of them in bf16, 2^-10 on average, beside the 2^-9 of their own rounding.)
   INT8_PAIRS = 2,
   INT8_SUMS = 3,   // the sums themselves, of a share of k (within int8_umma.cu)
 };
@@ -41,7 +38,6 @@ struct Int8Out {
   void* y;
   int64_t ldy;
   const float* bias;
-  float* power;    // INT8_PAIRS in fp16: (E, ceil(rows / 32)), written by the product
 };
 
 // On the tensor cores (int8_umma.cu).  `scratch`: int8_umma_scratch_bytes bytes on a 16-byte boundary, or NULL (then no tile's k is shared

@@ -34,7 +34,6 @@ struct PairArgs {
   Int8Product p;
   Int8Out o;
   int max_width, m_tiles;
-  int sum_shift;   // INT8_PAIRS: 2^sum_shift brings the largest sum down to 2^15
   int stages, stage_bytes;
   int gated_box;   // gate and up rows of a CTA come in one box (rows in whole sixteens), otherwise in four
   int packed;      // rows of results can be stored 16 bytes at a time
@@ -174,7 +173,7 @@ struct TokenMaps {
   CUtensorMap rows32, rows64, rows128;
 };
 
-// DT: type of what is stored (INT8_Y, INT8_PAIRS)
+// DT: type of what is stored (INT8_Y)
 template <int KIND, int DT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
     int8_pair_kernel(const __grid_constant__ CUtensorMap map_w, const __grid_constant__ TokenMaps maps, const PairArgs a) {
@@ -334,16 +333,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
       const int col = KIND == INT8_GATED ? u.m * TILE_ROWS + rank * 64 + q * 16 + (lane & 15) : u.m * TILE_ROWS + rank * 128 + q * 32 + lane;
       const bool col_in = col < p.rows;
       const int w_row = KIND == INT8_GATED ? (lane >> 4) * p.rows + col : col;
-      float ws = col_in ? __ldg(p.w_scale + (int64_t)u.e * SETS * p.rows + w_row) : 0.0f;
-      if constexpr (KIND == INT8_PAIRS && DT == MQ_F16) {
-        const uint32_t most = __reduce_max_sync(0xffffffffu, __float_as_uint(ws) & 0x7FFFFFFFu);
-        // the power of two above the 32 scales; nothing to take out of zeros, and nothing that helps infinities and NaN
-        const int e2 = most == 0u || most >= 0x7F800000u ? 127 : min((int)(most >> 23) + 1, 253);
-        const float power = __uint_as_float((uint32_t)max(e2, 1) << 23);
-        ws = ws / power * __uint_as_float((uint32_t)(127 - a.sum_shift) << 23);
-        // (all tiles of the expert's tokens write the same)
-        if (lane == 0 && col_in) a.o.power[(int64_t)u.e * ((p.rows + 31) >> 5) + (col >> 5)] = power * __uint_as_float((uint32_t)(127 + a.sum_shift) << 23);
-      }
+      const float ws = col_in ? __ldg(p.w_scale + (int64_t)u.e * SETS * p.rows + w_row) : 0.0f;
       const float bias = KIND == INT8_Y && a.o.bias && col_in ? __ldg(a.o.bias + col) : 0.0f;
       const int chunks = u.width >> 5;
       float xs[4];
@@ -594,11 +584,9 @@ int int8_product_umma(const Int8Product& p, const Int8Out& o, void* scratch, cud
     return MQ_OK;
   }
   const int64_t piece = o.kind == INT8_GATED ? 4 : 16 / (int64_t)dtype_size(o.dtype);
-  while ((int64_t)p.K > (2ll << a.sum_shift)) ++a.sum_shift;   // 127 * 128 * K / 2^shift < 2^14 K / 2^shift <= 2^15
   a.packed = p.rows % piece == 0 && o.ldy % piece == 0 && aligned(o.y, 16);
   if (o.kind == INT8_GATED) return launch<INT8_GATED>(map_w, map_x, a, pairs, st);
-  if (o.kind == INT8_PAIRS && o.dtype == MQ_F32) return launch<INT8_PAIRS, MQ_F32>(map_w, map_x, a, pairs, st);
-  if (o.kind == INT8_PAIRS) return launch<INT8_PAIRS, MQ_F16>(map_w, map_x, a, pairs, st);
+  if (o.kind == INT8_PAIRS) return launch<INT8_PAIRS>(map_w, map_x, a, pairs, st);
   if (o.dtype == MQ_F32) return launch<INT8_Y, MQ_F32>(map_w, map_x, a, pairs, st);
   if (o.dtype == MQ_BF16) return launch<INT8_Y, MQ_BF16>(map_w, map_x, a, pairs, st);
   return launch<INT8_Y, MQ_F16>(map_w, map_x, a, pairs, st);
