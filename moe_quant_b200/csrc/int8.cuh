@@ -27,8 +27,8 @@ struct Int8Product {
 enum Int8Result {
   INT8_Y = 0,      // y = sum * x_scale * w_scale + bias, in the result's type
   INT8_GATED = 1,  // weights are gate rows and up rows, `rows` of either: h = silu(gate) * up, fp32
-  // The products of the pairs, short of x_scale: sum * w_scale in fp32.  (In fp16 they would be half the bytes, but 11 bits of each product
-  // show in the results: 1e-3 of them in bf16, 2^-10 on average, beside the 2^-9 of their own rounding.)
+  // The products of the pairs, short of x_scale: sum * w_scale in fp32.  (In fp16 they would be half the bytes, but their 11 bits
+  // show beside the 8 of a bf16 result: they moved it by 1e-3 of its norm, its own rounding by 1.7e-3.)
   INT8_PAIRS = 2,
   INT8_SUMS = 3,   // the sums themselves, of a share of k (within int8_umma.cu)
 };
@@ -39,6 +39,10 @@ struct Int8Out {
   int64_t ldy;
   const float* bias;
 };
+
+// silu(g) u, the same in every kernel: a token's result does not depend on how many others are in the call.  (With __expf and __fdividef the exponential
+// is off by 1.2 |g| steps more.)
+__device__ __forceinline__ float gated(float g, float u) { return g / (1.0f + expf(-g)) * u; }
 
 // On the tensor cores (int8_umma.cu).  `scratch`: int8_umma_scratch_bytes bytes on a 16-byte boundary, or NULL (then no tile's k is shared
 // among CTAs).

@@ -235,8 +235,6 @@ struct OneParams {
   int* fault;
 };
 
-__device__ __forceinline__ float gated(float g, float u) { return g / (1.0f + expf(-g)) * u; }
-
 // bytes in front of the rings: codes of h and a product per row and pair
 __host__ __device__ __forceinline__ size_t one_token_down_codes(int top_k, int64_t K, int64_t I) {
   return ((size_t)top_k * few_pitch((int)I) + (size_t)(K / FEW_BLOCKS + 1) * top_k * 4 + 127) / 128 * 128;
@@ -347,13 +345,13 @@ __global__ void __launch_bounds__(ONE_THREADS, 1) one_token_down_kernel(const On
     if (!stream.ok) break;
     __syncwarp();
     sum = __reduce_add_sync(0xffffffffu, sum);
-    if (lane == 0) products[u] = (float)sum * factor[v] * __ldg(p.down_scale + (int64_t)expert[v] * p.K + n);
+    if (lane == 0) products[u] = (float)sum * __ldg(p.down_scale + (int64_t)expert[v] * p.K + n);
   }
   stream.end();
   __syncthreads();
   for (int r = threadIdx.x; r < end - begin; r += ONE_THREADS) {
     float sum = 0.0f;
-    for (int v = 0; v < n_pairs; ++v) sum += products[r * n_pairs + v];
+    for (int v = 0; v < n_pairs; ++v) sum = fmaf(factor[v], products[r * n_pairs + v], sum);      // as combine_kernel does
     put(p.y, DT, begin + r, sum);
   }
 }

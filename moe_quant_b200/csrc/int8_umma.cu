@@ -122,9 +122,6 @@ struct Unit {
   }
 };
 
-// silu(g) u; the exponential is off by 2 + 1.2 |g| steps at most, the quotient by 2
-__device__ __forceinline__ float gated(float g, float u) { return __fdividef(g, 1.0f + __expf(-g)) * u; }
-
 __device__ __forceinline__ uint16_t bits16(__nv_bfloat16 v) { return __bfloat16_as_ushort(v); }
 __device__ __forceinline__ uint16_t bits16(__half v) { return __half_as_ushort(v); }
 

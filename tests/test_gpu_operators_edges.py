@@ -4,7 +4,7 @@ import torch
 
 from moe_quant_b200 import ops
 from tests import operator_reference as R
-from tests.test_gpu_operators import BF16, FP16, _gen, _on
+from tests.test_gpu_operators import BF16, FP16, _experts_case, _gen, _on
 
 pytestmark = pytest.mark.gpu
 
@@ -27,3 +27,15 @@ def test_a_channel_keeps_its_digits_beside_larger_ones(cuda, T, dtype):
     y = ops.int8_experts(**_on(c, cuda)).cpu().double()
     want, _ = R.experts(**c)
     assert torch.all((y - want).abs() <= want.abs() * (1.01 * R.HALF_STEP[dtype] + 60 * 2.0 ** -24) + R.SMALLEST[dtype])
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16])
+@pytest.mark.parametrize("T, k, E, K, I", [(9, 2, 4, 256, 128), (33, 4, 4, 264, 72), (300, 8, 8, 512, 520), (5, 3, 6, 130, 1000), (6, 2, 3, 7168, 2048)])
+def test_a_token_gets_the_same_result_alone(cuda, T, k, E, K, I, dtype):
+    c = _on(_experts_case(T, k, E, E, 0, K, I, dtype, T + K), cuda)
+    c["gate_up_scale"] *= 8        # gates of some size
+    c["ids"][T // 2, 0] = -1
+    together = ops.int8_experts(**c)
+    for t in range(0, T, max(1, T // 20)):
+        alone = ops.int8_experts(**{**c, "x": c["x"][t:t + 1], "ids": c["ids"][t:t + 1], "weights": c["weights"][t:t + 1]})
+        assert torch.equal(alone[0], together[t]), t
