@@ -3,7 +3,7 @@
 // Routing, per token: scores s = sigmoid(logit) or softmax(logits); values v = s + bias; the groups with the largest
 // sum of two values (or largest value) stay; the top_k largest v of those are chosen, ties to the lowest index; weights are
 // the scores without bias, normalised over the chosen ones where asked.  An expert whose logit is -inf or NaN, or whose bias is
-// -inf or NaN, is never chosen.  +inf counts as the largest finite number.
+// -inf or NaN, is never chosen.  +inf counts as the largest finite number, -0 as 0.
 //
 // One warp per token, a run of experts per lane.  Which experts come first is decided on fp32 scores wherever these lie further apart than
 // they can be off, and in 64 bits in the rows where some do not (without a bias the logits themselves order the experts: exactly).
@@ -32,8 +32,8 @@ struct RouteParams {
   int lanes_to_search;    // as many as there are to a group, a power of two of them
 };
 
-// NaN is -inf, +inf the largest number
-__device__ __forceinline__ float finite_logit(float l) { return fminf(fmaxf(l, -CUDART_INF_F), 3.402823466e38f); }
+// NaN is -inf, +inf the largest number, -0 is +0 (the sum): keys order bits, and zeros of either sign have the same score
+__device__ __forceinline__ float finite_logit(float l) { return fminf(fmaxf(l, -CUDART_INF_F), 3.402823466e38f) + 0.0f; }
 
 template <typename F>
 __device__ __forceinline__ F warp_sum(F v) {

@@ -4,7 +4,7 @@ import torch
 
 from moe_quant_b200 import ops
 from tests import operator_reference as R
-from tests.test_gpu_operators import BF16, FP16, _experts_case, _gen, _on
+from tests.test_gpu_operators import BF16, FP16, FP32, _experts_case, _gen, _on, _route_both
 
 pytestmark = pytest.mark.gpu
 
@@ -39,3 +39,31 @@ def test_a_token_gets_the_same_result_alone(cuda, T, k, E, K, I, dtype):
     for t in range(0, T, max(1, T // 20)):
         alone = ops.int8_experts(**{**c, "x": c["x"][t:t + 1], "ids": c["ids"][t:t + 1], "weights": c["weights"][t:t + 1]})
         assert torch.equal(alone[0], together[t]), t
+
+
+# ------------------------------------------------------------------ routing
+@pytest.mark.parametrize("dtype", [FP32, BF16, FP16])
+@pytest.mark.parametrize("c", [
+    dict(E=8, k=1, score="sigmoid"), dict(E=8, k=3, score="softmax"), dict(E=64, k=6, score="softmax", renormalise=False), dict(E=60, k=8, score="sigmoid"),
+    dict(E=256, k=8, score="sigmoid"), dict(E=400, k=5, score="softmax"), dict(E=1000, k=30, score="sigmoid"),
+    dict(E=64, k=4, score="sigmoid", groups=8, keep=3, group_score="top2"), dict(E=256, k=8, score="softmax", groups=8, keep=4),
+    dict(E=60, k=4, score="sigmoid", groups=4, keep=2, group_score="top2"), dict(E=60, k=4, score="softmax", groups=4, keep=2)],
+    ids=lambda c: "-".join(str(v) for v in c.values()))
+def test_route_zeros_of_either_sign_are_a_tie(cuda, c, dtype):
+    """-0.0 and +0.0 have one score: the lowest index comes first, at the cut behind the k-th too."""
+    E = c["E"]
+    g = _gen(E + c["k"])
+    zeros = torch.where(torch.rand(40, E, generator=g) < 0.5, 0.0, -0.0)
+    logits = torch.where(torch.rand(40, E, generator=g) < 0.3, -1.0, zeros)      # mostly zeros, more than k of them
+    logits[:10] = zeros[:10]
+    logits[10:20] = torch.where(torch.rand(10, E, generator=g) < 2.0 / E, zeros[10:20], -torch.rand(10, E, generator=g) - 0.5)     # a few
+    logits[20:25] = torch.where(torch.rand(5, E, generator=g) < 0.1, 1.0, zeros[20:25])     # behind others
+    logits = logits.to(dtype)
+    assert torch.any(torch.signbit(logits) & (logits == 0)) and torch.any(~torch.signbit(logits) & (logits == 0))
+    _route_both(logits, None, c, cuda)
+    _route_both(logits, torch.where(torch.rand(E, generator=g) < 0.5, 0.0, -0.0), c, cuda)
+    # one negative zero in front of a positive one
+    logits = torch.full((1, E), -1.0, dtype=dtype)
+    logits[0, 2], logits[0, E - 1] = -0.0, 0.0
+    ids, _ = _route_both(logits, None, c, cuda)
+    assert int(ids[0, 0]) == 2
