@@ -301,7 +301,7 @@ int mq_expert_plan(const int32_t* ids, int64_t pairs, int64_t E, int64_t first, 
 size_t mq_expert_plan_workspace_bytes(int64_t pairs, int64_t E);
 
 /* 8-bit codes of each row of x (T, K): scale = max|x| / 127, code = round-half-even(127 x / max|x|).  A row of zeros has the scale
- * 0; one with an infinity or a NaN the scale NaN and codes 0.  ldx in elements, ldc in bytes.  */
+ * 0; one with an infinity or a NaN the scale NaN and codes 0.  ldx in elements, ldc in bytes.  K <= 2^30.  */
 int mq_quantize_tokens(const void* x, int dtype, int64_t T, int64_t K, int64_t ldx, int8_t* codes, int64_t ldc, float* scale,
                        void* stream);
 

@@ -268,6 +268,7 @@ __global__ void __launch_bounds__(256) combine_kernel(const CombineParams p) {
 }
 
 constexpr int64_t INT8_MAX_K = 131072;   // 127 * 128 * K stays below 2^31
+constexpr int64_t ROWS_MAX_K = 1 << 30;  // quantize_rows_kernel counts columns in 32 bits, up to 32768 beyond the last
 
 int64_t pitch_of(int64_t K) { return ceil_div(K, 16) * 16; }
 
@@ -279,8 +280,9 @@ using namespace mq;
 extern "C" int mq_quantize_tokens(const void* x, int dtype, int64_t T, int64_t K, int64_t ldx, int8_t* codes, int64_t ldc, float* scale,
                                   void* stream) {
   MQ_REQUIRE(valid_dtype(dtype), MQ_ERR_ARGUMENT, "mq_quantize_tokens: unknown dtype %d", dtype);
-  MQ_REQUIRE(T >= 0 && K >= 1 && K < (1ll << 31) && ldx >= K && ldc >= K, MQ_ERR_ARGUMENT,
+  MQ_REQUIRE(T >= 0 && K >= 1 && ldx >= K && ldc >= K, MQ_ERR_ARGUMENT,
              "mq_quantize_tokens: bad sizes T=%lld K=%lld ldx=%lld ldc=%lld", (long long)T, (long long)K, (long long)ldx, (long long)ldc);
+  MQ_REQUIRE(K <= ROWS_MAX_K, MQ_ERR_UNSUPPORTED, "mq_quantize_tokens: K is at most 2^30 (got %lld)", (long long)K);
   if (T == 0) return MQ_OK;
   MQ_REQUIRE(x && codes && scale, MQ_ERR_ARGUMENT, "mq_quantize_tokens: null pointer");
   return quantize_rows(dtype, RowsParams{x, ldx, T, nullptr, nullptr, 0, (int)K, codes, ldc, scale}, static_cast<cudaStream_t>(stream));
