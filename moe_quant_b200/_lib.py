@@ -129,6 +129,16 @@ def engine_fault() -> int:
     return out.value
 
 
+def require_no_fault(device: torch.device) -> None:
+    """Raises if a wait has run out on `device`: what the kernels stored since is no result.  Synchronises."""
+    with torch.cuda.device(device) if device.type == "cuda" else _NOTHING:
+        code = engine_fault()
+    if code != 0:
+        raise MoeQuantError(
+            f"a tensor-core kernel gave up on a bounded wait (code {code}) on {device}: results computed since "
+            "are invalid; call moe_quant_b200._lib.engine_fault_clear() before reusing the device")
+
+
 PROFILE_KINDS = ["umma_gemm", "simt_gemm", "sweep_tile", "chol_diag", "trsm_rows", "split_planes", "pack_int4", "other", "umma_deep"]
 
 

@@ -18,7 +18,7 @@ import torch
 import torch.nn as nn
 from torch import Tensor
 
-from . import dist_utils, model_utils, quant_utils
+from . import _lib, dist_utils, model_utils, quant_utils
 from ._lib import MoeQuantError
 from .int8 import int8_block
 from .gptq import GPTQ, quantize_many, quantize_shared
@@ -59,7 +59,8 @@ def quantize_block(
     'layers': names in quantization order, 'issues': {'zero_samples','nan_hessian','non_invertible'},
     'relative_error': {name: float} when log_error}.
     int8_outputs: the outputs come from the block as it is served in 8-bit integers, activations rounded to 8 bits per token
-    (8 bits and one group per row; the dequantized weights stay in the block as ever)."""
+    (8 bits and one group per row; the dequantized weights stay in the block as ever).  Fails if a wait of a kernel ran out
+    meanwhile."""
     forward_kwargs = forward_kwargs or {}
     if int8_outputs and (bits != 8 or group_size is not None):
         raise MoeQuantError("int8_outputs needs bits=8 and group_size=None")
@@ -142,6 +143,11 @@ def quantize_block(
 
     with int8_block(block, int8_results):                                                    # as it is, without results
         outputs = [block(x, **forward_kwargs) for x in inputs]                               # quant.py:414-416
+    if int8_outputs:      # the integer products leave memory as it was where a wait ran out, and what it held may be finite
+        for device in {o.device for o in outputs}:
+            if device.type == "cuda":
+                torch.cuda.synchronize(device)
+            _lib.require_no_fault(device)
     for o in outputs:
         if not bool(torch.isfinite(o).all()):
             raise RuntimeError("block outputs are not finite after quantization")

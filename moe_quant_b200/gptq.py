@@ -96,15 +96,7 @@ class GPTQ:
         # The read-back above synchronised with the layer's kernels, so this is the place where an
         # expired device-side wait of the tensor-core kernels shows: the layer's codes are garbage
         # then and must not be saved as if they were a result.
-        if device.type == "cuda":
-            with torch.cuda.device(device):
-                code = _lib.engine_fault()
-        else:
-            code = _lib.engine_fault()
-        if code != 0:
-            raise MoeQuantError(
-                f"a tensor-core kernel gave up on a bounded wait (code {code}) on {device}: results computed since "
-                "are invalid; call moe_quant_b200._lib.engine_fault_clear() before reusing the device")
+        _lib.require_no_fault(device)
 
     @property
     def issue_nan_hessian(self) -> bool:

@@ -1,6 +1,10 @@
 """Operators of the quantized layers at the ends of what they take: what needs no device.  Refusals are decided on the host, before any launch."""
 import pytest
+import torch
+import torch.nn as nn
 
+from moe_quant_b200 import _lib, block_driver, ops
+from moe_quant_b200._lib import MoeQuantError
 from tests.test_operators import P, _status
 
 
@@ -9,3 +13,50 @@ def test_rows_longer_than_the_kernel_counts_are_refused(K):
     """Columns are counted in 32 bits in steps of up to 16384, and looked at up to as many behind the last step: near 2^31 the count would wrap."""
     status, message = _status("mq_quantize_tokens", P, 1, 1, K, K, P, K, P, None)
     assert status == 3 and b"2^30" in message
+
+
+# ------------------------------------------------------------------ the block driver
+class _Handle:
+    """Stands in for a GPTQ handle: keeps the layer's weight, with codes of one group per row."""
+
+    issue_zero_samples = issue_nan_hessian = issue_non_invertible = False
+
+    def __init__(self, layer, *args, **kwargs):
+        self.layer = layer
+
+    def update(self, x):
+        pass
+
+    def reset(self):
+        pass
+
+
+def _results_of(handles, bits, streams=8, want_error=False):
+    out = []
+    for h in handles:
+        rows, cols = h.layer.weight.shape
+        out.append((torch.full((rows, cols), 130, dtype=torch.uint8), torch.full((rows, 1), 0.01), torch.full((rows, 1), 128.0)))
+    return (out, [None] * len(out)) if want_error else out
+
+
+@pytest.mark.parametrize("code", [0, 94])
+def test_block_driver_reports_a_wait_that_ran_out_in_the_integer_products(monkeypatch, code):
+    """The kernels of the served block leave what memory held when a wait runs out, finite or not: outputs are given only after the word that waits
+    record their codes in has been read."""
+    monkeypatch.setattr(block_driver, "GPTQ", _Handle)
+    monkeypatch.setattr(block_driver, "quantize_shared", _results_of)
+    monkeypatch.setattr(block_driver, "quantize_many", _results_of)
+    monkeypatch.setattr(block_driver.quant_utils, "dequantize_linear_weight", lambda q, s, z: (q.float() - z) * s)
+    monkeypatch.setattr(ops, "int8_matmul", lambda x, w, s, bias=None: x @ (w.to(x.dtype) * s[:, None].to(x.dtype)).t())
+    asked = []
+    monkeypatch.setattr(_lib, "engine_fault", lambda: asked.append(1) or code)
+    block = nn.Sequential(nn.Linear(32, 16, bias=False), nn.Linear(16, 32, bias=False))
+    run = lambda **kw: block_driver.quantize_block(block, [torch.ones(4, 32)], bits=8, group_size=None, **kw)
+    run()
+    assert not asked
+    if code:
+        with pytest.raises(MoeQuantError, match="bounded wait .code 94"):
+            run(int8_outputs=True)
+    else:
+        assert run(int8_outputs=True)["outputs"][0].shape == (4, 32)
+    assert asked
