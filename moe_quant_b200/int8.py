@@ -30,7 +30,20 @@ def int8_layout(qweight: Tensor, scale: Tensor, zero: Optional[Tensor] = None) -
     return codes.view(torch.int8), scale.reshape(R).to(torch.float32)
 
 
-class Int8Linear(nn.Module):
+class _Int8Module(nn.Module):
+    """Scales and biases stay in fp32 whatever type a module or the model around it is converted to: they follow it to other
+    devices alone."""
+
+    def _apply(self, fn, *args, **kwargs):
+        kept = {n: b for n, b in self._buffers.items() if b is not None and b.is_floating_point()}
+        super()._apply(fn, *args, **kwargs)
+        for n, b in kept.items():
+            if self._buffers[n].dtype != b.dtype:
+                self._buffers[n] = b.to(self._buffers[n].device)
+        return self
+
+
+class Int8Linear(_Int8Module):
     """Stands in for an nn.Linear whose weight has been quantized to 8 bits per output channel."""
 
     def __init__(self, qweight: Tensor, scale: Tensor, zero: Optional[Tensor] = None, bias: Optional[Tensor] = None):
@@ -45,7 +58,7 @@ class Int8Linear(nn.Module):
         return ops.int8_matmul(x, self.codes, self.scale, bias=self.bias)
 
 
-class Int8Experts(nn.Module):
+class Int8Experts(_Int8Module):
     """The gated MLPs of the experts first .. first + E - 1, one (qweight, scale, zero) per projection and expert."""
 
     def __init__(self, gate: Sequence, up: Sequence, down: Sequence, first: int = 0):

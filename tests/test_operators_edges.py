@@ -3,7 +3,7 @@ import pytest
 import torch
 import torch.nn as nn
 
-from moe_quant_b200 import _lib, block_driver, ops
+from moe_quant_b200 import Int8Experts, Int8Linear, _lib, block_driver, ops
 from moe_quant_b200._lib import MoeQuantError
 from tests.test_operators import P, _status
 
@@ -60,3 +60,28 @@ def test_block_driver_reports_a_wait_that_ran_out_in_the_integer_products(monkey
     else:
         assert run(int8_outputs=True)["outputs"][0].shape == (4, 32)
     assert asked
+
+
+# ------------------------------------------------------------------ the modules
+def _layer(rows, cols, seed):
+    g = torch.Generator().manual_seed(seed)
+    return torch.randint(0, 256, (rows, cols), dtype=torch.uint8, generator=g), 0.01 * torch.rand(rows, 1, generator=g) + 0.003
+
+
+def _modules():
+    experts = Int8Experts([_layer(12, 20, i) for i in range(3)], [_layer(12, 20, 10 + i) for i in range(3)], [_layer(20, 12, 20 + i) for i in range(3)])
+    return Int8Linear(*_layer(9, 20, 5), bias=torch.linspace(-1, 1, 9) / 3), experts
+
+
+@pytest.mark.parametrize("convert", [lambda m: m.half(), lambda m: m.to(torch.bfloat16), lambda m: m.double(), lambda m: nn.Sequential(m).bfloat16()[0],
+                                     lambda m: m.to("cpu", torch.float16)])
+def test_conversions_leave_scales_alone(convert):
+    """They are fp32 numbers, whose rounding to fewer bits would go into every result."""
+    for was, now in zip(_modules(), [convert(m) for m in _modules()]):
+        for name, buffer in was.named_buffers():
+            assert now.get_buffer(name).dtype == buffer.dtype and torch.equal(now.get_buffer(name), buffer), name
+
+
+def test_scales_follow_their_module_to_other_devices():
+    for m in _modules():
+        assert {b.device.type for b in m.to("meta", torch.bfloat16).buffers()} == {"meta"}
