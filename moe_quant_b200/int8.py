@@ -50,9 +50,13 @@ class Int8Linear(_Int8Module):
         super().__init__()
         codes, scale = int8_layout(qweight, scale, zero)
         self.out_features, self.in_features = codes.shape
-        self.register_buffer("codes", codes, persistent=False)
+        self.register_buffer("padded", _whole(codes), persistent=False)      # (a view would lose its row stride on the way to another device)
         self.register_buffer("scale", scale, persistent=False)
         self.register_buffer("bias", None if bias is None else bias.detach().to(torch.float32), persistent=False)
+
+    @property
+    def codes(self) -> Tensor:
+        return _columns(self.padded, self.in_features)
 
     def forward(self, x: Tensor) -> Tensor:
         return ops.int8_matmul(x, self.codes, self.scale, bias=self.bias)
@@ -68,14 +72,26 @@ class Int8Experts(_Int8Module):
         self.first = int(first)
         gates, ups, downs = ([int8_layout(*r) for r in side] for side in (gate, up, down))
         both = [(torch.cat([_whole(g), _whole(u)]), torch.cat([gs, us])) for (g, gs), (u, us) in zip(gates, ups)]
-        hidden, inner = gates[0][0].shape[1], gates[0][0].shape[0]
-        self.register_buffer("gate_up", torch.stack([c for c, _ in both])[..., :hidden], persistent=False)
+        self.inner, self.hidden = gates[0][0].shape
+        self.register_buffer("padded_gate_up", torch.stack([c for c, _ in both]), persistent=False)
         self.register_buffer("gate_up_scale", torch.stack([s for _, s in both]), persistent=False)
-        self.register_buffer("down", torch.stack([_whole(c) for c, _ in downs])[..., :inner], persistent=False)
+        self.register_buffer("padded_down", torch.stack([_whole(c) for c, _ in downs]), persistent=False)
         self.register_buffer("down_scale", torch.stack([s for _, s in downs]), persistent=False)
+
+    @property
+    def gate_up(self) -> Tensor:
+        return _columns(self.padded_gate_up, self.hidden)
+
+    @property
+    def down(self) -> Tensor:
+        return _columns(self.padded_down, self.inner)
 
     def forward(self, x: Tensor, ids: Tensor, weights: Tensor) -> Tensor:
         return ops.int8_experts(x, ids, weights, self.gate_up, self.gate_up_scale, self.down, self.down_scale, first=self.first)
+
+
+def _columns(padded: Tensor, n: int) -> Tensor:
+    return padded if padded.shape[-1] == n else padded[..., :n]
 
 
 def _whole(codes: Tensor) -> Tensor:

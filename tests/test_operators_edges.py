@@ -1,4 +1,6 @@
 """Operators of the quantized layers at the ends of what they take: what needs no device.  Refusals are decided on the host, before any launch."""
+import copy
+
 import pytest
 import torch
 import torch.nn as nn
@@ -85,3 +87,16 @@ def test_conversions_leave_scales_alone(convert):
 def test_scales_follow_their_module_to_other_devices():
     for m in _modules():
         assert {b.device.type for b in m.to("meta", torch.bfloat16).buffers()} == {"meta"}
+
+
+@pytest.mark.parametrize("move", [lambda m: m.to("meta"), lambda m: m.to("meta", torch.float16), copy.deepcopy, lambda m: m._apply(torch.clone)])
+def test_rows_of_codes_keep_their_padding_on_the_way(move):
+    """Rows start 16 bytes apart or a multiple of it, also of a module that was built on one device and moved to another."""
+    linear, experts = _modules()
+    for codes in (linear.codes, experts.gate_up, experts.down):
+        assert codes.stride()[-2:] == (-(-codes.shape[-1] // 16) * 16, 1)
+    shapes = linear.codes.shape, experts.gate_up.shape, experts.down.shape
+    strides = linear.codes.stride(), experts.gate_up.stride(), experts.down.stride()
+    linear, experts = move(linear), move(experts)
+    assert shapes == (linear.codes.shape, experts.gate_up.shape, experts.down.shape)
+    assert strides == (linear.codes.stride(), experts.gate_up.stride(), experts.down.stride())
