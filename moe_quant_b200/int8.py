@@ -71,8 +71,11 @@ class Int8Experts(_Int8Module):
             raise MoeQuantError("Int8Experts: as many gate as up and down projections, and at least one")
         self.first = int(first)
         gates, ups, downs = ([int8_layout(*r) for r in side] for side in (gate, up, down))
+        inner, hidden = gates[0][0].shape
+        if any(c.shape != (inner, hidden) for c, _ in gates + ups) or any(c.shape != (hidden, inner) for c, _ in downs):
+            raise MoeQuantError(f"Int8Experts: gate and up projections are not all {inner} x {hidden}, or down projections {hidden} x {inner}")
         both = [(torch.cat([_whole(g), _whole(u)]), torch.cat([gs, us])) for (g, gs), (u, us) in zip(gates, ups)]
-        self.inner, self.hidden = gates[0][0].shape
+        self.inner, self.hidden = inner, hidden
         self.register_buffer("padded_gate_up", torch.stack([c for c, _ in both]), persistent=False)
         self.register_buffer("gate_up_scale", torch.stack([s for _, s in both]), persistent=False)
         self.register_buffer("padded_down", torch.stack([_whole(c) for c, _ in downs]), persistent=False)

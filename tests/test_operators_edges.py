@@ -100,3 +100,14 @@ def test_rows_of_codes_keep_their_padding_on_the_way(move):
     linear, experts = move(linear), move(experts)
     assert shapes == (linear.codes.shape, experts.gate_up.shape, experts.down.shape)
     assert strides == (linear.codes.stride(), experts.gate_up.stride(), experts.down.stride())
+
+
+@pytest.mark.parametrize("side, expert, shape", [(0, 1, (12, 24)), (1, 2, (12, 24)), (1, 0, (16, 20)), (2, 1, (20, 14)), (2, slice(None), (20, 14)), (2, 0, (21, 12))])
+def test_experts_of_unlike_sizes_are_refused(side, expert, shape):
+    """Also where the padded rows have one length."""
+    sides = [[_layer(12, 20, i) for i in range(3)], [_layer(12, 20, i) for i in range(3)], [_layer(20, 12, i) for i in range(3)]]
+    Int8Experts(*sides)
+    for i in range(3)[expert] if isinstance(expert, slice) else [expert]:
+        sides[side][i] = _layer(*shape, i)
+    with pytest.raises(MoeQuantError, match="Int8Experts"):
+        Int8Experts(*sides)
