@@ -10,6 +10,7 @@ from typing import Optional, Sequence, Tuple
 import ctypes
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import MATH_COMPACT, MATH_FP32, MATH_MANY_TOKENS, MATH_TENSOR, MQ_I8, MoeQuantError, check, dtype_code, lib, ptr, require_cuda, require_one_device, stream_ptr
@@ -384,6 +385,10 @@ def _forward_only(what: str, *tensors: Optional[Tensor]) -> None:
         for t in tensors:
             if t is not None and t.requires_grad:
                 raise MoeQuantError(f"{what} has no backward pass: call it under torch.no_grad() or detach its inputs")
+    if forward_ad._current_level >= 0:      # (within forward_ad.dual_level; torch.no_grad() does not switch tangents off)
+        for t in tensors:
+            if t is not None and forward_ad.unpack_dual(t).tangent is not None:
+                raise MoeQuantError(f"{what} has no derivative: its inputs carry tangents, unpack them first")
 
 
 def _same_device(what: str, device: torch.device, *tensors: Optional[Tensor]) -> None:

@@ -4,6 +4,7 @@ import copy
 import pytest
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad
 
 from moe_quant_b200 import Int8Experts, Int8Linear, _lib, block_driver, ops
 from moe_quant_b200._lib import MoeQuantError
@@ -111,3 +112,17 @@ def test_experts_of_unlike_sizes_are_refused(side, expert, shape):
         sides[side][i] = _layer(*shape, i)
     with pytest.raises(MoeQuantError, match="Int8Experts"):
         Int8Experts(*sides)
+
+
+def test_tangents_are_refused():
+    """A result without its tangent would be taken for a constant."""
+    x, w = torch.zeros(2, 16), torch.ones(3)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(x, torch.ones_like(x))
+        for call in (lambda: ops._forward_only("op", dual, None), lambda: ops._forward_only("op", x, None, dual[:1])):
+            with pytest.raises(MoeQuantError, match="tangents"):
+                call()
+            with torch.no_grad(), pytest.raises(MoeQuantError, match="tangents"):
+                call()
+        ops._forward_only("op", x, None, w, forward_ad.unpack_dual(dual).primal)
+    ops._forward_only("op", x, None, w)
