@@ -8,7 +8,9 @@ from torch.autograd import forward_ad
 
 from moe_quant_b200 import Int8Experts, Int8Linear, _lib, block_driver, ops
 from moe_quant_b200._lib import MoeQuantError
-from tests.test_operators import P, _status
+from moe_quant_b200.int8 import int8_block
+from moe_quant_b200.synthetic_block import SyntheticMoEBlock
+from tests.test_operators import P, _results, _status
 
 
 @pytest.mark.parametrize("K", [2 ** 30 + 1, 2 ** 31 - 16384, 2 ** 31 - 1, 2 ** 31, 2 ** 40])
@@ -126,3 +128,17 @@ def test_tangents_are_refused():
                 call()
         ops._forward_only("op", x, None, w, forward_ad.unpack_dual(dual).primal)
     ops._forward_only("op", x, None, w)
+
+
+# ------------------------------------------------------------------ blocks whose layers are swapped
+def _block():
+    return SyntheticMoEBlock(hidden=32, inter=16, n_experts=4, top_k=2, q_rank=16, kv_rank=16, n_heads=2, nope_dim=8, rope_dim=8, v_dim=8)
+
+
+def test_experts_with_biases_keep_them():
+    block = _block()
+    block.mlp.experts[1].up_proj.bias = nn.Parameter(torch.linspace(-1, 1, 16))
+    with int8_block(block, _results(block)):
+        assert block.mlp.int8_experts is None
+        assert torch.equal(block.mlp.experts[1].up_proj.bias, torch.linspace(-1, 1, 16)) and block.mlp.experts[0].up_proj.bias is None
+        assert all(isinstance(getattr(e, side), Int8Linear) for e in block.mlp.experts for side in ("gate_proj", "up_proj", "down_proj"))
