@@ -123,8 +123,8 @@ def int8_block(block: nn.Module, results: Mapping[str, Tuple[Tensor, Tensor, Ten
             biased = any(getattr(block.get_submodule(n), "bias", None) is not None for n in mine.values())     # (Int8Experts has none)
             if biased or not ids or ids != local or ids != list(range(ids[0], ids[-1] + 1)) or any(r is None for side in sides for r in side):
                 continue
+            undo.append((moe, "int8_experts", moe.int8_experts))
             moe.int8_experts = Int8Experts(*sides, first=ids[0])
-            undo.append((moe, "int8_experts", None))
             for n in mine.values():
                 del left[n]
         for name, result in left.items():

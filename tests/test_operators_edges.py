@@ -142,3 +142,14 @@ def test_experts_with_biases_keep_them():
         assert block.mlp.int8_experts is None
         assert torch.equal(block.mlp.experts[1].up_proj.bias, torch.linspace(-1, 1, 16)) and block.mlp.experts[0].up_proj.bias is None
         assert all(isinstance(getattr(e, side), Int8Linear) for e in block.mlp.experts for side in ("gate_proj", "up_proj", "down_proj"))
+
+
+def test_experts_that_were_there_before_come_back():
+    block = _block()
+    block.mlp.int8_experts = mine = Int8Experts(*([r] * 4 for r in (_layer(16, 32, 0), _layer(16, 32, 1), _layer(32, 16, 2))))
+    with int8_block(block, _results(block)):
+        assert isinstance(block.mlp.int8_experts, Int8Experts) and block.mlp.int8_experts is not mine
+        with int8_block(block, _results(block)):
+            pass
+        assert block.mlp.int8_experts is not None and block.mlp.int8_experts is not mine
+    assert block.mlp.int8_experts is mine
