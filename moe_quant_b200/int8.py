@@ -121,7 +121,8 @@ def int8_block(block: nn.Module, results: Mapping[str, Tuple[Tensor, Tensor, Ten
             if any(left[n][1].dtype == torch.float32 for n in mine.values()):
                 continue
             biased = any(getattr(block.get_submodule(n), "bias", None) is not None for n in mine.values())     # (Int8Experts has none)
-            if biased or not ids or ids != local or ids != list(range(ids[0], ids[-1] + 1)) or any(r is None for side in sides for r in side):
+            others = len(mine) > 3 * len(ids)      # an expert with more layers than a gated MLP has
+            if biased or others or not ids or ids != local or ids != list(range(ids[0], ids[-1] + 1)) or any(r is None for side in sides for r in side):
                 continue
             undo.append((moe, "int8_experts", moe.int8_experts))
             moe.int8_experts = Int8Experts(*sides, first=ids[0])

@@ -153,3 +153,13 @@ def test_experts_that_were_there_before_come_back():
             pass
         assert block.mlp.int8_experts is not None and block.mlp.int8_experts is not mine
     assert block.mlp.int8_experts is mine
+
+
+def test_experts_with_other_layers_run_layer_by_layer():
+    """What int8_experts computes is a gated MLP of three projections; a fourth layer would be left out."""
+    block = _block()
+    block.mlp.experts[2].mix_proj = nn.Linear(16, 16, bias=False)
+    with int8_block(block, _results(block)):
+        assert block.mlp.int8_experts is None
+        assert isinstance(block.mlp.experts[2].mix_proj, Int8Linear) and isinstance(block.mlp.experts[0].gate_proj, Int8Linear)
+    assert isinstance(block.mlp.experts[2].mix_proj, nn.Linear)
