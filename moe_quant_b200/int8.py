@@ -102,6 +102,9 @@ def _whole(codes: Tensor) -> Tensor:
     return codes.as_strided((codes.shape[0], codes.stride(0)), codes.stride())
 
 
+_HOOKS = ("_forward_hooks", "_forward_hooks_with_kwargs", "_forward_hooks_always_called", "_forward_pre_hooks", "_forward_pre_hooks_with_kwargs")
+
+
 @contextmanager
 def int8_block(block: nn.Module, results: Mapping[str, Tuple[Tensor, Tensor, Tensor]]):
     """Within the context the block's quantized layers run in 8-bit integers: `results` maps their names to what quantize(8)
@@ -122,7 +125,8 @@ def int8_block(block: nn.Module, results: Mapping[str, Tuple[Tensor, Tensor, Ten
                 continue
             biased = any(getattr(block.get_submodule(n), "bias", None) is not None for n in mine.values())     # (Int8Experts has none)
             others = len(mine) > 3 * len(ids)      # an expert with more layers than a gated MLP has
-            if biased or others or not ids or ids != local or ids != list(range(ids[0], ids[-1] + 1)) or any(r is None for side in sides for r in side):
+            hooked = any(m._forward_hooks or m._forward_pre_hooks for e in moe.experts if e is not None for m in e.modules())
+            if biased or others or hooked or not ids or ids != local or ids != list(range(ids[0], ids[-1] + 1)) or any(r is None for side in sides for r in side):
                 continue
             undo.append((moe, "int8_experts", moe.int8_experts))
             moe.int8_experts = Int8Experts(*sides, first=ids[0])
@@ -134,7 +138,10 @@ def int8_block(block: nn.Module, results: Mapping[str, Tuple[Tensor, Tensor, Ten
             layer = getattr(parent, leaf)
             if not isinstance(layer, nn.Linear):
                 raise MoeQuantError(f"int8_block: {name} is no nn.Linear")
-            setattr(parent, leaf, Int8Linear(*result, bias=layer.bias))
+            stand_in = Int8Linear(*result, bias=layer.bias)
+            for hooks in _HOOKS:      # the same dicts: what is registered or removed meanwhile counts for both
+                setattr(stand_in, hooks, getattr(layer, hooks))
+            setattr(parent, leaf, stand_in)
             undo.append((parent, leaf, layer))
         yield block
     finally:

@@ -163,3 +163,34 @@ def test_experts_with_other_layers_run_layer_by_layer():
         assert block.mlp.int8_experts is None
         assert isinstance(block.mlp.experts[2].mix_proj, Int8Linear) and isinstance(block.mlp.experts[0].gate_proj, Int8Linear)
     assert isinstance(block.mlp.experts[2].mix_proj, nn.Linear)
+
+
+def test_hooks_of_swapped_layers_fire(monkeypatch):
+    monkeypatch.setattr(ops, "int8_matmul", lambda x, w, s, bias=None: x @ (w.to(x.dtype) * s[:, None].to(x.dtype)).t())
+    block, seen = _block(), []
+    layer = block.mlp.shared_experts.up_proj
+    layer.register_forward_hook(lambda m, i, o: seen.append(("after", type(m))))
+    layer.register_forward_pre_hook(lambda m, args, kwargs: seen.append(("before", type(m))), with_kwargs=True)
+    x = torch.ones(2, 32)
+    with int8_block(block, _results(block)):
+        swapped = block.mlp.shared_experts.up_proj
+        swapped(x)
+        assert seen == [("before", Int8Linear), ("after", Int8Linear)]
+        late = swapped.register_forward_hook(lambda m, i, o: seen.append("late"))
+        swapped(x)
+        assert seen.pop() == "late"
+        late.remove()
+    del seen[:]
+    block.mlp.shared_experts.up_proj(x)
+    assert seen == [("before", nn.Linear), ("after", nn.Linear)]
+
+
+@pytest.mark.parametrize("where", ["", "down_proj"])
+def test_experts_with_hooks_run_layer_by_layer(where):
+    block = _block()
+    handle = block.mlp.experts[3].get_submodule(where).register_forward_hook(lambda m, i, o: None)
+    with int8_block(block, _results(block)):
+        assert block.mlp.int8_experts is None and isinstance(block.mlp.experts[3].down_proj, Int8Linear)
+    handle.remove()
+    with int8_block(block, _results(block)):
+        assert block.mlp.int8_experts is not None
