@@ -121,6 +121,9 @@ def int8_block(block: nn.Module, results: Mapping[str, Tuple[Tensor, Tensor, Ten
             ids = sorted({int(m.group(1)) for m in (re.fullmatch(r"(\d+)\.(gate|up|down)_proj", n) for n in mine) if m})
             sides = [[left.get(f"{prefix}{i}.{side}_proj") for i in ids] for side in ("gate", "up", "down")]
             local = [i for i, e in enumerate(moe.experts) if e is not None]
+            if mine and moe.int8_experts is not None:      # of other weights
+                undo.append((moe, "int8_experts", moe.int8_experts))
+                moe.int8_experts = None
             if any(left[n][1].dtype == torch.float32 for n in mine.values()):
                 continue
             biased = any(getattr(block.get_submodule(n), "bias", None) is not None for n in mine.values())     # (Int8Experts has none)
@@ -128,7 +131,7 @@ def int8_block(block: nn.Module, results: Mapping[str, Tuple[Tensor, Tensor, Ten
             hooked = any(m._forward_hooks or m._forward_pre_hooks for e in moe.experts if e is not None for m in e.modules())
             if biased or others or hooked or not ids or ids != local or ids != list(range(ids[0], ids[-1] + 1)) or any(r is None for side in sides for r in side):
                 continue
-            undo.append((moe, "int8_experts", moe.int8_experts))
+            undo.append((moe, "int8_experts", None))
             moe.int8_experts = Int8Experts(*sides, first=ids[0])
             for n in mine.values():
                 del left[n]

@@ -194,3 +194,18 @@ def test_experts_with_hooks_run_layer_by_layer(where):
     handle.remove()
     with int8_block(block, _results(block)):
         assert block.mlp.int8_experts is not None
+
+
+@pytest.mark.parametrize("scale_type", [torch.float32, torch.bfloat16])
+def test_experts_that_were_there_before_do_not_stand_in_for_new_ones(scale_type):
+    """Experts that run layer by layer (here of fp32 layers, or with a hook) do so although the module had some of its own."""
+    block = _block()
+    block.mlp.int8_experts = mine = Int8Experts(*([r] * 4 for r in (_layer(16, 32, 0), _layer(16, 32, 1), _layer(32, 16, 2))))
+    if scale_type != torch.float32:
+        block.mlp.experts[0].register_forward_hook(lambda m, i, o: None)
+    with int8_block(block, {n: (q, s.to(scale_type), z) for n, (q, s, z) in _results(block).items()}):
+        assert block.mlp.int8_experts is None
+    assert block.mlp.int8_experts is mine
+    with int8_block(block, {n: r for n, r in _results(block).items() if "experts." not in n}):
+        assert block.mlp.int8_experts is mine
+    assert block.mlp.int8_experts is mine
