@@ -71,6 +71,20 @@ inline cudaError_t launch_chained(bool chained, void (*kernel)(KArgs...), dim3 g
     if (_s != MQ_OK) return _s;   \
   } while (0)
 
+// Lets a kernel take up to `bytes` of shared memory, once per device.  Always the most that any call of the kernel needs: the limit is the
+// kernel's, so a smaller one set for a call of another thread could come between this call's and its launch.
+template <auto KERNEL>
+inline int allow_smem(size_t bytes) {
+  static bool ready[64] = {};
+  int dev = 0;
+  MQ_CUDA(cudaGetDevice(&dev));
+  if (dev >= 64 || !ready[dev]) {
+    MQ_CUDA(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
+    if (dev < 64) ready[dev] = true;
+  }
+  return MQ_OK;
+}
+
 inline bool aligned(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p) % a) == 0; }
 inline size_t align_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }

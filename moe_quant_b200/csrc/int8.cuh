@@ -58,8 +58,8 @@ bool int8_one_token_fits(int top_k, int64_t K, int64_t I);
 int int8_one_token(const void* x, int dtype, const int32_t* ids, const float* weights, int top_k, int first, const Int8Product& up,
                    const Int8Product& down, float* h, void* y, cudaStream_t st);
 
-// Once per device: the word that waits record their codes in, and the shared memory that a kernel may take.  Looking them up in every
-// call cost 2 us of the 6 of a call.
+// Once per device: the word that waits record their codes in.  (Looking it up in every call, and asking for shared memory in each, cost 2 us
+// of the 6 of a call.)
 inline int fault_word(int** out) {
   static int* word[64] = {};
   int dev = 0;
@@ -67,17 +67,6 @@ inline int fault_word(int** out) {
   if (dev >= 64) return engine_fault_word(out);
   if (!word[dev]) MQ_TRY(engine_fault_word(&word[dev]));
   *out = word[dev];
-  return MQ_OK;
-}
-template <auto KERNEL>
-int allow_smem(size_t bytes) {
-  static bool ready[64] = {};
-  int dev = 0;
-  MQ_CUDA(cudaGetDevice(&dev));
-  if (dev >= 64 || !ready[dev]) {
-    MQ_CUDA(cudaFuncSetAttribute(KERNEL, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
-    if (dev < 64) ready[dev] = true;
-  }
   return MQ_OK;
 }
 

@@ -16,7 +16,7 @@
 namespace mq {
 namespace {
 
-constexpr int ROUTE_WARPS = 8, EXTRA = 4;
+constexpr int ROUTE_WARPS = 8, EXTRA = 4, MAX_EXPERTS = 1024;
 constexpr size_t SMEM_AS_IS = 47 * 1024;   // of the 48 KB that need no permission, beside what a kernel has of its own
 
 struct RouteParams {
@@ -494,7 +494,7 @@ int launch_route(const void* logits, RouteParams p, cudaStream_t st) {
   do {                                                                                                                    \
     const int lanes = p.group_size / VPL;                                                                                 \
     p.lanes_per_group = p.group_size % VPL == 0 && (lanes & (lanes - 1)) == 0 && lanes * p.groups <= 32 ? lanes : 0;      \
-    if (smem > SMEM_AS_IS) MQ_CUDA(cudaFuncSetAttribute(route_kernel<DT, VPL>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem)); \
+    if (smem > SMEM_AS_IS) MQ_TRY((allow_smem<route_kernel<DT, VPL>>((size_t)ROUTE_WARPS * 32 * VPL * 12)));               \
     const int64_t blocks = ceil_div(p.T, ROUTE_WARPS), most = 148 * route_blocks(VPL);                                    \
     MQ_CUDA(launch_chained(true, route_kernel<DT, VPL>, dim3((unsigned)(blocks < most ? blocks : most)), dim3(ROUTE_WARPS * 32), smem, st, logits, p)); \
   } while (0)
@@ -692,7 +692,7 @@ extern "C" int mq_route_tokens(const void* logits, int dtype, int64_t T, int64_t
   MQ_REQUIRE(valid_dtype(dtype), MQ_ERR_ARGUMENT, "mq_route_tokens: unknown dtype %d", dtype);
   MQ_REQUIRE(T >= 0 && E >= 1 && ld >= E, MQ_ERR_ARGUMENT, "mq_route_tokens: bad sizes T=%lld E=%lld ld=%lld", (long long)T, (long long)E,
              (long long)ld);
-  MQ_REQUIRE(E <= 1024, MQ_ERR_UNSUPPORTED, "mq_route_tokens: at most 1024 experts (got %lld)", (long long)E);
+  MQ_REQUIRE(E <= MAX_EXPERTS, MQ_ERR_UNSUPPORTED, "mq_route_tokens: at most 1024 experts (got %lld)", (long long)E);
   MQ_REQUIRE(top_k >= 1 && top_k <= 32 && top_k <= E, MQ_ERR_ARGUMENT, "mq_route_tokens: top_k must be in [1, min(32, E)] (got %d)", top_k);
   MQ_REQUIRE((score == 0 || score == 1) && (group_score == 0 || group_score == 1), MQ_ERR_ARGUMENT,
              "mq_route_tokens: unknown score %d or group score %d", score, group_score);
@@ -724,7 +724,7 @@ int expert_plan(const int32_t* ids, int64_t pairs, int E, int first, int32_t* of
     MQ_LAUNCH_CHECK();
   }
   const size_t smem = (size_t)E * (PLAN_WARPS + 2) * 4;
-  if (smem > SMEM_AS_IS) MQ_CUDA(cudaFuncSetAttribute(plan_place_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  if (smem > SMEM_AS_IS) MQ_TRY(allow_smem<plan_place_kernel>((size_t)MAX_EXPERTS * (PLAN_WARPS + 2) * 4));
   MQ_CUDA(launch_chained(true, plan_place_kernel, dim3(blocks), dim3(PLAN_THREADS), smem, st, p));
   MQ_LAUNCH_CHECK();
   return MQ_OK;
@@ -735,7 +735,7 @@ extern "C" int mq_expert_plan(const int32_t* ids, int64_t pairs, int64_t E, int6
                               void* workspace, size_t workspace_bytes, void* stream) {
   MQ_REQUIRE(pairs >= 0 && E >= 1 && first >= 0 && first < (1ll << 31), MQ_ERR_ARGUMENT, "mq_expert_plan: bad sizes pairs=%lld E=%lld first=%lld",
              (long long)pairs, (long long)E, (long long)first);
-  MQ_REQUIRE(E <= 1024 && pairs < (1ll << 31) - (1 << 20), MQ_ERR_UNSUPPORTED, "mq_expert_plan: at most 1024 experts and 2^31 - 2^20 pairs");
+  MQ_REQUIRE(E <= MAX_EXPERTS && pairs < (1ll << 31) - (1 << 20), MQ_ERR_UNSUPPORTED, "mq_expert_plan: at most 1024 experts and 2^31 - 2^20 pairs");
   MQ_REQUIRE(offsets && (pairs == 0 || (ids && order && place)), MQ_ERR_ARGUMENT, "mq_expert_plan: null pointer");
   MQ_REQUIRE(plan_blocks(pairs) == 1 || (workspace && workspace_bytes >= mq_expert_plan_workspace_bytes(pairs, E)), MQ_ERR_WORKSPACE,
              "mq_expert_plan: the workspace has %zu bytes and needs %zu", workspace_bytes, mq_expert_plan_workspace_bytes(pairs, E));

@@ -1,8 +1,10 @@
 """Operators of the quantized layers where their results could depend on what they should not."""
+import threading
+
 import pytest
 import torch
 
-from moe_quant_b200 import ops
+from moe_quant_b200 import _lib, ops
 from tests import operator_reference as R
 from tests.test_gpu_operators import BF16, FP16, FP32, _experts_case, _gen, _on, _route_both
 
@@ -67,3 +69,43 @@ def test_route_zeros_of_either_sign_are_a_tie(cuda, c, dtype):
     logits[0, 2], logits[0, E - 1] = -0.0, 0.0
     ids, _ = _route_both(logits, None, c, cuda)
     assert int(ids[0, 0]) == 2
+
+
+# ------------------------------------------------------------------ calls of several threads
+@pytest.mark.parametrize("what", ["plan", "route"])
+@pytest.mark.parametrize("n_threads", [2, 6])
+def test_threads_with_different_numbers_of_experts(cuda, what, n_threads):
+    """What one thread's call lets a kernel take of shared memory must not take away what another's needs."""
+    L, failures = _lib.lib(), []
+    gate = threading.Barrier(n_threads)
+
+    def work(i):
+        E = (1024, 520)[i % 2]
+        stream = torch.cuda.Stream()
+        ids = torch.randint(0, E, (64,), dtype=torch.int32, generator=_gen(i)).to(cuda)
+        order, place = torch.empty_like(ids), torch.empty_like(ids)
+        offsets = torch.empty(E + 1, dtype=torch.int32, device=cuda)
+        logits = torch.randn(16, E, device=cuda)
+        chosen, weights = torch.empty(16, 4, dtype=torch.int32, device=cuda), torch.empty(16, 4, device=cuda)
+        torch.cuda.synchronize()
+        gate.wait()
+        for _ in range(20000):
+            if what == "plan":
+                status = L.mq_expert_plan(ids.data_ptr(), 64, E, 0, offsets.data_ptr(), order.data_ptr(), place.data_ptr(), None, 0, stream.cuda_stream)
+            else:
+                status = L.mq_route_tokens(logits.data_ptr(), 0, 16, E, E, 4, 1, None, 1, 1, 0, 1, 1.0, chosen.data_ptr(), weights.data_ptr(),
+                                           stream.cuda_stream)
+            if status:
+                failures.append((E, L.mq_last_error()))
+        stream.synchronize()
+        right = torch.equal(order.long(), torch.sort(ids, stable=True)[1]) if what == "plan" else torch.equal(
+            chosen.long(), torch.sort(logits, descending=True, stable=True)[1][:, :4])
+        if not right:
+            failures.append((E, "wrong result"))
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(n_threads)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failures, (len(failures), failures[0])
