@@ -295,7 +295,7 @@ int mq_route_tokens(const void* logits, int dtype, int64_t T, int64_t E, int64_t
 
 /* A stable counting sort of pairs by expert: ids[i] - first in [0, E) is the expert of pair i, every other id belongs to no expert here.
  *   offsets (E + 1): where an expert's pairs begin;  order (pairs): the pairs, by (expert, i), -1 behind the last;
- *   place (pairs): where pair i stands in order, -1 for none.  E <= 1024.  */
+ *   place (pairs): where pair i stands in order, -1 for none.  E <= 1024, first + E < 2^31.  */
 int mq_expert_plan(const int32_t* ids, int64_t pairs, int64_t E, int64_t first, int32_t* offsets, int32_t* order, int32_t* place,
                    void* workspace, size_t workspace_bytes, void* stream);
 size_t mq_expert_plan_workspace_bytes(int64_t pairs, int64_t E);
@@ -317,7 +317,7 @@ size_t mq_int8_matmul_workspace_bytes(int x_dtype, int64_t T, int64_t N, int64_t
  *   weights[t, s] * down_e(silu(gate_e(x[t])) * up_e(x[t])),
  * every product as in mq_int8_matmul, the gated values kept in fp32 until they get their codes.  gate_up (E, 2 I, K): gate rows, then
  * up rows; down (E, K, I); row strides ld_* and expert strides *_expert in bytes, multiples of 16; scales contiguous.
- * A token without an expert here gets zeros.  */
+ * A token without an expert here gets zeros.  first + E < 2^31.  */
 int mq_int8_experts(const void* x, int dtype, int64_t T, int64_t K, int64_t ldx, const int32_t* ids, const float* weights, int top_k,
                     int64_t first, int64_t E, int64_t I, const int8_t* gate_up, int64_t ld_gate_up, int64_t gate_up_expert,
                     const float* gate_up_scale, const int8_t* down, int64_t ld_down, int64_t down_expert, const float* down_scale,

@@ -405,7 +405,7 @@ extern "C" int mq_int8_experts(const void* x, int dtype, int64_t T, int64_t K, i
                                void* y, int64_t ldy, void* workspace, size_t workspace_bytes, void* stream) {
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   MQ_REQUIRE(dtype == MQ_BF16 || dtype == MQ_F16, MQ_ERR_ARGUMENT, "mq_int8_experts: tokens are bf16 or fp16 (got dtype %d)", dtype);
-  MQ_REQUIRE(T >= 0 && K >= 1 && I >= 1 && E >= 1 && top_k >= 1 && top_k <= 32 && first >= 0 && first < (1ll << 31) && ldx >= K && ldy >= K &&
+  MQ_REQUIRE(T >= 0 && K >= 1 && I >= 1 && E >= 1 && top_k >= 1 && top_k <= 32 && first >= 0 && first < (1ll << 31) - E && ldx >= K && ldy >= K &&
                  ld_gate_up >= K && ld_down >= I && gate_up_expert >= 0 && down_expert >= 0,
              MQ_ERR_ARGUMENT, "mq_int8_experts: bad sizes T=%lld K=%lld I=%lld E=%lld top_k=%d first=%lld", (long long)T, (long long)K, (long long)I,
              (long long)E, top_k, (long long)first);

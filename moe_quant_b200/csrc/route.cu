@@ -733,7 +733,8 @@ int expert_plan(const int32_t* ids, int64_t pairs, int E, int first, int32_t* of
 
 extern "C" int mq_expert_plan(const int32_t* ids, int64_t pairs, int64_t E, int64_t first, int32_t* offsets, int32_t* order, int32_t* place,
                               void* workspace, size_t workspace_bytes, void* stream) {
-  MQ_REQUIRE(pairs >= 0 && E >= 1 && first >= 0 && first < (1ll << 31), MQ_ERR_ARGUMENT, "mq_expert_plan: bad sizes pairs=%lld E=%lld first=%lld",
+  // (2^31 - 1 is no expert: wider ids that are clamped to it stay without one)
+  MQ_REQUIRE(pairs >= 0 && E >= 1 && first >= 0 && first < (1ll << 31) - E, MQ_ERR_ARGUMENT, "mq_expert_plan: bad sizes pairs=%lld E=%lld first=%lld",
              (long long)pairs, (long long)E, (long long)first);
   MQ_REQUIRE(E <= MAX_EXPERTS && pairs < (1ll << 31) - (1 << 20), MQ_ERR_UNSUPPORTED, "mq_expert_plan: at most 1024 experts and 2^31 - 2^20 pairs");
   MQ_REQUIRE(offsets && (pairs == 0 || (ids && order && place)), MQ_ERR_ARGUMENT, "mq_expert_plan: null pointer");

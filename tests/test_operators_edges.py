@@ -10,7 +10,7 @@ from moe_quant_b200 import Int8Experts, Int8Linear, _lib, block_driver, ops
 from moe_quant_b200._lib import MoeQuantError
 from moe_quant_b200.int8 import int8_block
 from moe_quant_b200.synthetic_block import SyntheticMoEBlock
-from tests.test_operators import P, _results, _status
+from tests.test_operators import P, _experts, _results, _status
 
 
 @pytest.mark.parametrize("K", [2 ** 30 + 1, 2 ** 31 - 16384, 2 ** 31 - 1, 2 ** 31, 2 ** 40])
@@ -18,6 +18,17 @@ def test_rows_longer_than_the_kernel_counts_are_refused(K):
     """Columns are counted in 32 bits in steps of up to 16384, and looked at up to as many behind the last step: near 2^31 the count would wrap."""
     status, message = _status("mq_quantize_tokens", P, 1, 1, K, K, P, K, P, None)
     assert status == 3 and b"2^30" in message
+
+
+@pytest.mark.parametrize("first, status", [(2 ** 31 - 9, 0), (2 ** 31 - 8, 1), (2 ** 31 - 1, 1), (2 ** 31, 1), (2 ** 62, 1)])
+def test_experts_are_numbered_below_the_largest_id(first, status):
+    """Ids of 64 bits that lie outside 32 are clamped to their ends, which must not be an expert's number.  (Accepted calls are refused for their workspace next: nothing is launched.)"""
+    if status == 0:
+        assert _status("mq_expert_plan", P, 10 ** 6, 8, first, P, P, P, None, 0, None)[0] == 4
+        assert _experts(first=first, E=8, ws=None)[0] == 4
+    else:
+        assert _status("mq_expert_plan", P, 10 ** 6, 8, first, P, P, P, None, 0, None)[0] == status
+        assert _experts(first=first, E=8, ws=None)[0] == status
 
 
 # ------------------------------------------------------------------ the block driver
