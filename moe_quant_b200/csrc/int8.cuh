@@ -40,6 +40,9 @@ struct Int8Out {
   const float* bias;
 };
 
+// The result with its bias, two roundings in every kernel (a fused sum in some of them would make a token's result depend on how many
+// others are in the call).
+__device__ __forceinline__ float plus_bias(float v, float bias) { return __fadd_rn(v, bias); }
 // silu(g) u, the same in every kernel: a token's result does not depend on how many others are in the call.  (With __expf and __fdividef the exponential
 // is off by 1.2 |g| steps more.)
 __device__ __forceinline__ float gated(float g, float u) { return g / (1.0f + expf(-g)) * u; }

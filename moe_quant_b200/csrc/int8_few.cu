@@ -212,7 +212,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 1) int8_few_kernel(const FewParam
     if (lane < p.T) {
       const int n = first + r * FEW_WARPS;
       float v = (float)mine * x_scale[lane] * __ldg(p.w_scale + n);
-      if (p.bias) v += __ldg(p.bias + n);
+      if (p.bias) v = plus_bias(v, __ldg(p.bias + n));
       put(p.y, p.out_dtype, lane * p.ldy + n, v);
     }
   }

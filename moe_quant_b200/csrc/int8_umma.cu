@@ -402,7 +402,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(I8_THREADS, 1)
           using S = typename StorageOf<DT>::type;
           if constexpr (KIND == INT8_Y) {
 #pragma unroll
-            for (int j = 0; j < 32; ++j) v[j] += bias;
+            for (int j = 0; j < 32; ++j) v[j] = plus_bias(v[j], bias);
           }
           S* out = static_cast<S*>(a.o.y) + (int64_t)t * a.o.ldy + (col - lane);
           if (a.packed) {
@@ -459,7 +459,7 @@ __global__ void __launch_bounds__(256) finish_kernel(const PairArgs a) {
     for (int j = 0; j < 4; ++j) {
       if (n + j >= p.rows) break;
       float v = (float)r[j] * xs * __ldg(p.w_scale + n + j);
-      if (a.o.bias) v += __ldg(a.o.bias + n + j);
+      if (a.o.bias) v = plus_bias(v, __ldg(a.o.bias + n + j));
       const int64_t at = t * a.o.ldy + n + j;
       if (a.o.dtype == MQ_F32) static_cast<float*>(a.o.y)[at] = v;
       else if (a.o.dtype == MQ_BF16) static_cast<__nv_bfloat16*>(a.o.y)[at] = __float2bfloat16_rn(v);

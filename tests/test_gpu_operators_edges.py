@@ -6,7 +6,7 @@ import torch
 
 from moe_quant_b200 import _lib, ops
 from tests import operator_reference as R
-from tests.test_gpu_operators import BF16, FP16, FP32, _experts_case, _gen, _on, _route_both
+from tests.test_gpu_operators import BF16, FP16, FP32, _codes, _experts_case, _gen, _on, _route_both, _tokens
 
 pytestmark = pytest.mark.gpu
 
@@ -41,6 +41,20 @@ def test_a_token_gets_the_same_result_alone(cuda, T, k, E, K, I, dtype):
     for t in range(0, T, max(1, T // 20)):
         alone = ops.int8_experts(**{**c, "x": c["x"][t:t + 1], "ids": c["ids"][t:t + 1], "weights": c["weights"][t:t + 1]})
         assert torch.equal(alone[0], together[t]), t
+
+
+# ------------------------------------------------------------------ the product
+@pytest.mark.parametrize("dtype", [FP32, BF16, FP16])
+@pytest.mark.parametrize("N, K", [(520, 1024), (2048, 7168), (100, 300)])
+def test_tokens_get_the_same_product_in_calls_of_any_size(cuda, N, K, dtype):
+    """With a bias and without: few tokens, tiles whose k is shared, tiles of their own."""
+    x = _tokens(2100, K, dtype, N).to(cuda)
+    whole, scale = _codes((N, K), K)
+    w, scale, bias = whole.to(cuda)[:, :K], scale.to(cuda), torch.randn(N, generator=_gen(2)).to(cuda)
+    for b in (None, bias):
+        full = ops.int8_matmul(x, w, scale, bias=b)
+        for T in (1, 2, 4, 5, 37, 300, 1011):
+            assert torch.equal(ops.int8_matmul(x[:T], w, scale, bias=b), full[:T]), T
 
 
 # ------------------------------------------------------------------ routing
