@@ -1,6 +1,7 @@
 """Operators of the quantized layers at the ends of what they take: what needs no device.  Refusals are decided on the host, before any launch."""
 import copy
 
+import numpy as np
 import pytest
 import torch
 import torch.nn as nn
@@ -29,6 +30,30 @@ def test_experts_are_numbered_below_the_largest_id(first, status):
     else:
         assert _status("mq_expert_plan", P, 10 ** 6, 8, first, P, P, P, None, 0, None)[0] == status
         assert _experts(first=first, E=8, ws=None)[0] == status
+
+
+# ------------------------------------------------------------------ codes of 16-bit values
+@pytest.mark.parametrize("bits", [8, 11])
+def test_codes_of_every_pair_of_significands(bits):
+    """The kernel's arithmetic for bf16 (8 bits of significand) and fp16 (11), step by step in fp32: x * (127 / top), rounded to 20 bits, plus
+    1.5 * 2^23.  Against round-half-even of 127 x / top in integers, for every significand of x and of the row's largest value, and every power of two
+    between them up to the one from which all codes are zero.  (Powers of two that both share change no step.)"""
+    half = 1 << bits - 1
+    ties = 0
+    for top in range(half, 2 * half):
+        for down in range(9):
+            x = np.arange(half, 2 * half, dtype=np.int64)
+            x = x[x <= top << down]           # x / 2^down is at most top
+            inv = np.float32(127.0) / np.float32(top)
+            product = (x.astype(np.float32) * np.float32(2.0 ** -down)) * inv
+            rounded = ((product.view(np.uint32) + np.uint32(8)) & ~np.uint32(15)).view(np.float32)
+            code = (rounded + np.float32(12582912.0)) - np.float32(12582912.0)
+            over, under = 127 * x, top << down
+            whole, rest = over // under, over % under
+            want = whole + ((2 * rest > under) | ((2 * rest == under) & (whole % 2 == 1)))
+            ties += int((2 * rest == under).sum())
+            assert np.array_equal(code.astype(np.int64), want), (top, down)
+    assert ties > 0
 
 
 # ------------------------------------------------------------------ the block driver
