@@ -307,7 +307,9 @@ int mq_quantize_tokens(const void* x, int dtype, int64_t T, int64_t K, int64_t l
 
 /* y[t, n] = (sum over k of code[t, k] w[n, k]) x_scale[t] w_scale[n] + bias[n], the sum exact in 32-bit integers (K <= 131072, for MQ_I8 one less).
  * x (T, K) of x_dtype gets its codes as mq_quantize_tokens gives them (x_scale is not read), or is codes already (MQ_I8) with
- * their scales.  w (N, K) int8; rows of codes start on 16-byte boundaries.  bias may be NULL.  y (T, N) of out_dtype.  */
+ * their scales.  w (N, K) int8; rows of codes start on 16-byte boundaries.  bias may be NULL.  y (T, N) of out_dtype.
+ * The factors are multiplied in this order, in fp32: |sum| x_scale must stay below 3.4e38, which it does while K max|x| < 2.6e36.
+ * A token's result does not depend on the others in the call.  */
 int mq_int8_matmul(const void* x, int x_dtype, const float* x_scale, int64_t T, int64_t K, int64_t ldx, const int8_t* w, int64_t N,
                    int64_t ldw, const float* w_scale, const float* bias, int out_dtype, void* y, int64_t ldy, void* workspace,
                    size_t workspace_bytes, void* stream);
@@ -315,7 +317,7 @@ size_t mq_int8_matmul_workspace_bytes(int x_dtype, int64_t T, int64_t N, int64_t
 
 /* The experts' MLPs of T tokens (bf16 or fp16): y[t] = sum over slots s with ids[t, s] - first = e in [0, E) of
  *   weights[t, s] * down_e(silu(gate_e(x[t])) * up_e(x[t])),
- * every product as in mq_int8_matmul, the gated values kept in fp32 until they get their codes.  gate_up (E, 2 I, K): gate rows, then
+ * every product as in mq_int8_matmul, the gated values and the pairs' products kept in fp32.  gate_up (E, 2 I, K): gate rows, then
  * up rows; down (E, K, I); row strides ld_* and expert strides *_expert in bytes, multiples of 16; scales contiguous.
  * A token without an expert here gets zeros.  first + E < 2^31.  */
 int mq_int8_experts(const void* x, int dtype, int64_t T, int64_t K, int64_t ldx, const int32_t* ids, const float* weights, int top_k,

@@ -6,8 +6,8 @@
 //   experts           h = silu(gate product) * up product per pair of token and expert, codes of h as above, and
 //                     y[t] = sum over the token's pairs of weight * down product
 //
-// Here: the codes (bound by memory and by instructions: 16384 x 2048 fp32 5.9 TB/s, 32768 x 2048 bf16 4.8, 16384 x 7168 bf16 4.5), the sum over a
-// token's pairs (5.1 TB/s), and the calls.  The products are in int8_umma.cu (tensor cores, bound by them) and int8_few.cu (up to four tokens,
+// Here: the codes (bound by memory and by instructions: 16384 x 2048 fp32 5.9 TB/s, 32768 x 2048 bf16 4.8, 16384 x 7168 bf16 4.3 to 4.5 with 16
+// instructions a value and 70 % of the issue slots), the sum over a token's pairs (bound by memory: 6.4 TB/s), and the calls.  The products are in int8_umma.cu (tensor cores, bound by them) and int8_few.cu (up to four tokens,
 // and the experts of one: bound by the weights' bytes).
 #include <math_constants.h>
 
@@ -207,7 +207,7 @@ int quantize_rows(int dtype, RowsParams p, cudaStream_t st) {
 // ---------------------------------------------------------------- products
 // y[t] = sum over the token's pairs, in the order of its slots, of weight * (the pair's down product).  The products are fp32 and short of the
 // factor h_scale[pair] (INT8_PAIRS).  One block per token, eight columns a
-// thread; smaller blocks for short rows (20000 tokens of 512, 2 of 8 experts: 92 us the whole call instead of 102 with 256 threads).
+// thread; smaller blocks for short rows (20000 tokens of 512, 2 of 8 experts: 115 us the whole call instead of 131 with 256 threads).
 struct CombineParams {
   const float* pairs;
   int64_t ldp;

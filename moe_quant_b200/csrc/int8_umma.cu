@@ -9,8 +9,8 @@
 //                          way meanwhile); the bytes of both CTAs count on the leader's barrier
 //   warp 1 of the leader : tcgen05.mma for both SMs, two accumulators of 256 columns by turns
 //   warps 4 .. 11        : epilogue, a quarter of the CTA's weight rows each, chunks of 32 tokens by turns
-// What bounds it: 8192 tokens through 7168 x 7168 take 263 to 278 us, 3.0 to 3.2 PFLOP/s (bf16 by cuBLAS 1.66); the tensor pipe is busy 93.5 % of
-// the SMs' active cycles, and 84 % of all: 896 tiles are 12.1 rounds of 74, so the thirteenth is nearly empty.
+// What bounds it: 8192 tokens through 7168 x 7168 take 259 us, 3.25 PFLOP/s (bf16 by cuBLAS 1.66); the tensor pipe is busy 95.4 % of
+// the SMs' active cycles, and 86.4 % of all: 896 tiles are 12.1 rounds of 74, so the thirteenth is nearly empty.
 // Persistent: a pair of CTAs takes every 74th tile.  Eight tiles of weight rows at a time go with all tiles of tokens, so that the
 // SMs that run side by side share rows of either in the L2.
 // Where there are fewer tiles than pairs of CTAs, several take a share of k each (`splits`) and store their sums as integers; a second kernel
@@ -165,7 +165,7 @@ __device__ __forceinline__ void store_columns(S* to, int64_t ld, int left, Of va
 }
 
 // The tokens' rows in boxes of 32, 64 and 128. A box costs the TMA unit time beside its bytes: 16384 pairs, 32 experts, 7168 to 2048 and back,
-// gate and up 364 us against 386 with boxes of 32 rows and of 16 gate and up rows, down 209 against 217.
+// gate and up 364 us against 386 with boxes of 32 rows and of 16 gate and up rows, down 209 against 217 (with products stored in fp16).
 struct TokenMaps {
   CUtensorMap rows32, rows64, rows128;
 };

@@ -7,7 +7,7 @@
 //
 // One warp per token, a run of experts per lane.  Which experts come first is decided on fp32 scores wherever these lie further apart than
 // they can be off, and in 64 bits in the rows where some do not (without a bias the logits themselves order the experts: exactly).
-// 65536 tokens, 256 experts in 8 groups with a bias: 82 us (0.82 TB/s of logits), 192 with every row in 64 bits.
+// 65536 tokens, 256 experts in 8 groups with a bias: 84 us (0.80 TB/s of logits), 192 with every row in 64 bits.
 #include <math_constants.h>
 
 #include "common.cuh"
@@ -213,8 +213,7 @@ __device__ __forceinline__ void sort_descending(uint32_t (&k)[N]) {
 }
 
 // VPL experts per lane: VPL lane .. VPL lane + VPL - 1.  A warp's next token's logits are on their way while it chooses.  Instructions
-// bound it: about 900 a token at 256 experts, 8 groups and a choice of 8 (72 % of the issue slots), of which the nine rounds of the choice
-// are a quarter.
+// bound it: 1085 a token at 256 experts, 8 groups and a choice of 8 (76 % of the issue slots; memory at 10 %).
 constexpr int route_blocks(int vpl) { return vpl <= 4 ? 5 : vpl <= 8 ? 4 : vpl <= 16 ? 3 : 2; }   // per SM
 
 template <int DT, int VPL>

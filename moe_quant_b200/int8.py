@@ -1,6 +1,7 @@
 """Layers that run in 8-bit integers on what `GPTQ(layer, None, ...).quantize(8)` returns: codes of 8 bits with one scale per
 output channel.  Activations get their codes token by token on the way in.  Forward only: the modules hold no
-parameters, and their calls refuse inputs that ask for gradients."""
+parameters, and their calls refuse inputs that ask for gradients.  Their buffers are not persistent: what is saved of a model is the
+quantizer's codes, scales and zero points, from which the modules are built."""
 from __future__ import annotations
 
 import re
@@ -109,7 +110,8 @@ _HOOKS = ("_forward_hooks", "_forward_hooks_with_kwargs", "_forward_hooks_always
 def int8_block(block: nn.Module, results: Mapping[str, Tuple[Tensor, Tensor, Tensor]]):
     """Within the context the block's quantized layers run in 8-bit integers: `results` maps their names to what quantize(8)
     returned.  A module whose experts are all among them, and which has a place for it (`int8_experts`), runs them through
-    ops.int8_experts (in bf16 and fp16 blocks); every other layer becomes an Int8Linear."""
+    ops.int8_experts (in bf16 and fp16 blocks) if they are plain gated MLPs: three layers each, without biases or forward hooks.  Every
+    other layer becomes an Int8Linear that keeps its bias and shares its forward hooks."""
     undo = []
     left = dict(results)
     try:

@@ -378,7 +378,8 @@ def pack_int4(codes: Tensor, zero_i8: Optional[Tensor] = None, group: int = 0) -
 
 
 # ---------------------------------------------------------------- running the quantized layers
-# Forward only.  Scratch comes from the caching allocator with every call: a buffer kept per stream would be shared by two graphs captured
+# Forward only.  A kernel whose wait ran out (a fault of the hardware or of the engine) leaves results as memory held them; no call waits for
+# its kernels to see that, so a program that wants to know asks _lib.require_no_fault(device), as quantize_block does.  Scratch comes from the caching allocator with every call: a buffer kept per stream would be shared by two graphs captured
 # on one stream, whose replays may overlap.
 def _forward_only(what: str, *tensors: Optional[Tensor]) -> None:
     if torch.is_grad_enabled():
@@ -544,7 +545,8 @@ def int8_matmul(x: Tensor, weight: Tensor, weight_scale: Tensor, bias: Optional[
                 out_dtype: Optional[torch.dtype] = None) -> Tensor:
     """y = x @ (weight * weight_scale)^T + bias with x rounded to 8-bit codes per token and the sum taken in integers.
     x (..., K) fp32/bf16/fp16, or int8 codes with their x_scale (...); weight (N, K) int8 with rows 16-byte aligned (int8_layout of
-    the int8 module makes it from GPTQ codes), weight_scale (N).  y has x's type, or out_dtype."""
+    the int8 module makes it from GPTQ codes), weight_scale (N).  y has x's type, or out_dtype.  A token's result is the same in calls of any
+    size.  K max|x| must stay below 2.6e36, where sum * x_scale, formed first, would leave fp32."""
     require_cuda(x, "x")
     _int8_codes(weight, 2, "weight")
     _forward_only("int8_matmul", x, weight_scale, bias, x_scale)
@@ -583,7 +585,8 @@ def int8_experts(x: Tensor, ids: Tensor, weights: Tensor, gate_up: Tensor, gate_
     """Sum over a token's experts of weight * down(silu(gate(x)) * up(x)), the products in 8-bit integers as in int8_matmul.
     x (..., K) bf16/fp16; ids and weights (..., top_k) as route_tokens gives them; gate_up (E, 2 I, K) int8, gate rows first, with
     gate_up_scale (E, 2 I); down (E, K, I) int8 with down_scale (E, K).  The experts here are first .. first + E - 1, others'
-    pairs add nothing."""
+    pairs add nothing.  Gated values and products stay fp32 until y; a token's result is the same in calls of any size.  Scratch is that of
+    T top_k pairs, whether their experts are here or not: 4 K + I bytes each, or K + 5 I where that is more."""
     require_cuda(x, "x")
     _int8_codes(gate_up, 3, "gate_up")
     _int8_codes(down, 3, "down")

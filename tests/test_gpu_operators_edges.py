@@ -85,6 +85,37 @@ def test_route_zeros_of_either_sign_are_a_tie(cuda, c, dtype):
     assert int(ids[0, 0]) == 2
 
 
+def _choice_on_the_device(logits, k, score, bias, groups, keep, top2):
+    """The choice by scores in 64 bits, in torch."""
+    l = logits.double() + 0.0
+    s = torch.sigmoid(l) if score == "sigmoid" else torch.softmax(l, -1)
+    v = s if bias is None else s + bias.double()
+    by = l if bias is None else v
+    if groups > 1:
+        worth = v if bias is not None or top2 else l
+        best = worth.view(len(l), groups, -1).topk(2, -1).values
+        kept = torch.sort(best.sum(-1) if top2 else best[..., 0], dim=-1, descending=True, stable=True)[1][:, :keep]
+        stays = torch.zeros(len(l), groups, dtype=torch.bool, device=l.device).scatter_(1, kept, True)
+        by = by.view(len(l), groups, -1).masked_fill(~stays[..., None], -float("inf")).view(l.shape)
+    return torch.sort(by, dim=-1, descending=True, stable=True)[1][:, :k]
+
+
+@pytest.mark.parametrize("grid", [False, True])
+@pytest.mark.parametrize("E", [60, 256, 332, 900])
+def test_route_many_random_rows(cuda, E, grid):
+    """4000 rows each of 72 configurations; on a grid of values there are ties and zeros of either sign in every row."""
+    g = torch.Generator(device=cuda).manual_seed(E)
+    for score in ("sigmoid", "softmax"):
+        for scale, dtype in ((0.01, FP32), (1.0, FP16), (40.0, BF16)):
+            for bias_scale in (None, 0.0, 0.1):
+                for groups, keep, top2 in ((1, 1, False), (4, 3, True), (2, 1, True), (4, 2, False)):
+                    logits = scale * torch.randn(4000, E, device=cuda, generator=g)
+                    logits = ((logits * (2 / scale)).round() * (scale / 2) if grid else logits).to(dtype)
+                    bias = None if bias_scale is None else bias_scale * torch.randn(E, device=cuda, generator=g)
+                    ids, _ = ops.route_tokens(logits, 8, score=score, bias=bias, groups=groups, keep_groups=keep, group_score="top2" if top2 else "max")
+                    assert torch.equal(ids.long(), _choice_on_the_device(logits, 8, score, bias, groups, keep, top2)), (score, scale, bias_scale, groups)
+
+
 # ------------------------------------------------------------------ calls of several threads
 @pytest.mark.parametrize("what", ["plan", "route"])
 @pytest.mark.parametrize("n_threads", [2, 6])
